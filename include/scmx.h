@@ -434,6 +434,54 @@ int scmx_select_token(const void* logits, int is_f32, int64_t V, int64_t* tok, i
  * [n + number of SMs].  0 switches it off.  Process-wide; no counterpart in the reference. */
 int scmx_set_decode_trace(unsigned long long* device_buf, int n_and_link);
 
+/* ---- INT8 key/value cache and speculative decoding ----------------------------------------------------------------- */
+
+/* Keys and values of L new tokens, k and v bf16 (head and row strides in elements, multiples of 8; unit column stride), go to rows pos ..
+ * pos + L - 1 of an INT8 cache, codes int8 [hk, capacity, d] and one float32 scale per vector [hk, capacity]: s = amax / 127, code =
+ * rint(x (1 / s)).  pos_dev non-null: one device int32 instead of pos (rows beyond the cache are dropped).  A vector with a value that is
+ * not finite reads back as NaN, one below 127 * 2^-126 as zero.  d a multiple of 16 up to 256.  No counterpart in the reference. */
+int scmx_kv_append(const uint16_t* k, int64_t k_head_stride, int64_t k_row_stride, const uint16_t* v, int64_t v_head_stride, int64_t v_row_stride,
+                   int64_t L, int hk, int d, int64_t pos, const int32_t* pos_dev, int64_t capacity, int8_t* k_codes, float* k_scales, int8_t* v_codes,
+                   float* v_scales, void* stream);
+
+/* Rows start .. start + n - 1 of an INT8 cache as bf16 [hk, n, d]: T(code * scale). */
+int scmx_kv_read(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int64_t start, int64_t n, int hk, int d,
+                 int64_t capacity, uint16_t* k, uint16_t* v, void* stream);
+
+/* A layer's cache: k, v [hk, capacity, d], bf16 or int8; ks, vs its scales (int8 only). */
+typedef struct scmx_kv_layer {
+    void *k, *v;
+    float *ks, *vs;
+} scmx_kv_layer;
+
+/* In every layer row pos + rows[j] becomes row pos + j (rows int32 [n] on the device, n <= 64; a negative entry, or one that is not
+ * below n, leaves its row).  All rows are read before one is written.  layers: host array; 64 layers a launch. */
+int scmx_kv_keep(const scmx_kv_layer* layers, int n_layers, const int32_t* rows, int n, int64_t pos, const int32_t* pos_dev, int hk, int d,
+                 int64_t capacity, int int8, void* stream);
+
+/* Attention of n <= 64 new rows to a cache that already holds their keys and values at rows pos .. pos + n - 1: q bf16, heads and rows
+ * q_head_stride and q_row_stride elements apart (multiples of 4), out bf16 [n, hq * d].  Row i sees all positions before pos, and new row j
+ * if bit j of mask[i] is set (mask null: j <= i); a row that sees nothing gives zeros.  k, v [hk, capacity, d]: bf16, or int8 with scales.
+ * pos_dev non-null: one device int32 instead of pos.  scratch: scmx_cache_attn_scratch(pos + n, or capacity with pos_dev; ..) bytes, 16-byte
+ * aligned, used by this call alone.  float32 softmax and sums, weights rounded to bf16.  d 64 or 128. */
+int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int hk, int d);
+int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,
+                    const float* v_scales, int int8, const int64_t* mask, int n, int64_t pos, const int32_t* pos_dev, int64_t capacity, int hq, int hk,
+                    int d, float scale, uint16_t* out, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Verification of a tree of drafted tokens.  logits [n, V] (rows ld apart): row 0 after the last chosen token, row c after tokens[c], which
+ * continues row parents[c] < c.  At a node with probabilities p = softmax(logits / temperature) its children are tested in ascending
+ * order: c is accepted if u[c] q(tokens[c]) < p(tokens[c]), q = probs[node] (float32 [n, V], children drawn from it independently) or 1
+ * (probs null: a draft without chance); a rejected one leaves p <- max(p - q, 0) / Z, or p without its token (unchanged where Z = 0).  The path goes
+ * on from an accepted row; at its end *token is the first index whose cumulative p exceeds u[0].  temperature 0: a child is
+ * accepted if it is the largest logit of its parent (lowest index of equal ones), u unused.  rows int32 [n]: the accepted rows, first 0, then
+ * -1; count int32 [1].  Tokens outside 0 .. V - 1 are rejected; without probabilities (all logits -inf, NaN) *token = 0.
+ * n <= 64; scratch: scmx_verify_scratch bytes, 16-byte aligned, used by this call alone. */
+int64_t scmx_verify_scratch(int n, int64_t V);
+int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, float temperature,
+                const float* probs, int64_t ldp, int n, int64_t V, int32_t* rows, int32_t* count, int64_t* token, void* scratch, int64_t scratch_bytes,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

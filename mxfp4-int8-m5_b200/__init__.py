@@ -3,7 +3,7 @@ dense and grouped-MoE GEMMs, decode GEMV.  Python modules mirror the reference's
 sc_moe.py, sc_decode.py and w4a8_mlx.py; all arithmetic runs in libscmx.so (include/scmx.h).  No CPU fallback."""
 import sys as _sys
 
-from . import _lib, sc_format, sc_kernels, sc_moe, sc_decode, w4a8, fused_dense, fused_moe, parallel  # noqa: F401
+from . import _lib, sc_format, sc_kernels, sc_moe, sc_decode, sc_cache, sc_draft, w4a8, fused_dense, fused_moe, parallel  # noqa: F401
 from . import host_model, packed_io, fused_qwen3, fused_olmoe, decode  # noqa: F401
 from . import sc_mixers, hybrid_mixers, fused_hybrid, registry, engine  # noqa: F401
 

@@ -41,6 +41,11 @@ class ScmxF4Job(ctypes.Structure):
     _fields_ = [("bcodes", ctypes.c_void_p), ("factors", ctypes.c_void_p), ("E", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64)]
 
 
+class ScmxKvLayer(ctypes.Structure):
+    """Mirror of `scmx_kv_layer` in include/scmx.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p)]
+
+
 class ScmxError(RuntimeError):
     """A libscmx entry point returned a non-zero status."""
 
@@ -116,6 +121,14 @@ SIGNATURES = {
     "scmx_head_bf16": [c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp],
     "scmx_route_token": [c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp],
     "scmx_norm_route_token": [c_vp, c_vp, c_float, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "scmx_kv_append": [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "scmx_kv_read": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_i64, c_vp, c_vp, c_vp],
+    "scmx_kv_keep": [ctypes.POINTER(ScmxKvLayer), c_int, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp],
+    "scmx_cache_attn_scratch": [c_i64, c_int, c_int, c_int, c_int],
+    "scmx_cache_attn": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_float, c_vp, c_vp, c_i64,
+                        c_vp],
+    "scmx_verify_scratch": [c_int, c_i64],
+    "scmx_verify": [c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_float, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
     "scmx_gemv_pro": [c_vp, c_int, c_vp, c_float, c_vp, c_vp, c_vp, c_i64, c_i64, _FMT_P, c_int, c_vp, c_vp, c_int, c_int, c_int,
                       c_vp, c_int, c_vp],
     "scmx_gemv_multi_plan": [c_vp, c_int, _FMT_P],
@@ -171,7 +184,8 @@ MIXER_SIGNATURES = {
     "scmx_gemv_x": [c_vp, c_i64, c_int, c_vp, c_i64, c_i64, c_int, c_float, c_float, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_vp],
     "scmx_last_error_string": [],
 }
-_RESTYPE = {"scmx_last_error_string": ctypes.c_char_p, "scmx_retention_scratch": c_i64, "scmx_delta_scratch": c_i64, "scmx_decode_step_scratch": c_i64}
+_RESTYPE = {"scmx_last_error_string": ctypes.c_char_p, "scmx_retention_scratch": c_i64, "scmx_delta_scratch": c_i64, "scmx_decode_step_scratch": c_i64,
+            "scmx_cache_attn_scratch": c_i64, "scmx_verify_scratch": c_i64}
 
 _lib = None
 _mixers = None
@@ -257,6 +271,16 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous()):
             raise TypeError("expected contiguous CUDA tensors; this package has no CPU path")
+
+
+def require_here(*tensors, contiguous=True):
+    """CUDA tensors of the current device, whose stream a call is launched on."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda) or (contiguous and not t.is_contiguous()):
+            raise TypeError(f"expected {'contiguous ' if contiguous else ''}CUDA tensors; this package has no CPU path")
+        if t.get_device() != here:
+            raise ValueError(f"a tensor on device {t.get_device()}, the current device is {here}")
 
 
 _sms = {}

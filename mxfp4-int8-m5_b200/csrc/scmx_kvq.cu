@@ -1,0 +1,195 @@
+// INT8 key/value cache: vectors of new tokens are quantized as they are written, cached rows are read back as bfloat16, and the rows of
+// accepted drafts are moved together.  A head's vector at one position has one float32 scale: s = amax / 127, code = rint(x (1 / s)),
+// the recipe of the activations' INT8.  Bound by memory: every value is loaded and stored once, 16 bytes a load.
+#include "scmx_common.cuh"
+
+namespace scmx {
+
+constexpr int KV_THREADS = 256;
+
+struct KvWriteArgs {
+    const uint16_t *src[2];          // bf16 keys, values
+    int64_t hs[2], rs[2];            // their head and row strides in elements
+    int8_t* codes[2];                // [hk, cap, d]
+    float* scales[2];                // [hk, cap]
+    const int32_t* pos_dev;
+    int64_t pos, cap, vectors;       // vectors: hk * L
+    int L, d;
+};
+
+// A vector belongs to G lanes of 8 values each (G the power of two from d / 8 on); blockIdx.y: 0 keys, 1 values.
+template <int G>
+__global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const KvWriteArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int which = blockIdx.y, l = threadIdx.x % G;
+    const int64_t i = (int64_t)blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
+    const int64_t pos = a.pos_dev ? (int64_t)a.pos_dev[0] : a.pos;
+    const int64_t head = i / a.L, row = i - head * a.L, at = pos + row;
+    const bool on = i < a.vectors && 8 * l < a.d;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (on) w = *reinterpret_cast<const uint4*>(a.src[which] + head * a.hs[which] + row * a.rs[which] + 8 * l);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    uint32_t top = 0;                // magnitudes of bfloat16 order like their bits, infinities and NaN last
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float s, qi;
+    quant_scale(__uint_as_float(top << 16), s, qi);
+    if (s < 1.17549435e-38f) s = qi = 0.0f;                  // 1 / s would overflow: such a vector is stored as zero
+    if (top >= 0x7F80u) { s = __uint_as_float(0x7FC00000u); qi = 0.0f; }      // a value that is not finite: the vector reads back as NaN
+    if (!on || at < 0 || at >= a.cap) return;                // a device-side position beyond the cache: the row is dropped
+    uint32_t q[2] = {0, 0};
+    if (qi > 0.0f) {
+        q[0] = quant4(bf16_lo(u[0]), bf16_hi(u[0]), bf16_lo(u[1]), bf16_hi(u[1]), qi);
+        q[1] = quant4(bf16_lo(u[2]), bf16_hi(u[2]), bf16_lo(u[3]), bf16_hi(u[3]), qi);
+    }
+    *reinterpret_cast<uint2*>(a.codes[which] + (head * a.cap + at) * a.d + 8 * l) = make_uint2(q[0], q[1]);
+    if (l == 0) a.scales[which][head * a.cap + at] = s;
+}
+
+struct KvReadArgs {
+    const int8_t* codes[2];
+    const float* scales[2];
+    uint16_t* out[2];                // bf16 [hk, n, d]
+    int64_t start, cap, n, pieces;   // pieces of 8 values: hk * n * d / 8
+    int per;                         // d / 8
+};
+
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvReadArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int which = blockIdx.y;
+    const int64_t i = (int64_t)blockIdx.x * KV_THREADS + threadIdx.x;
+    if (i >= a.pieces) return;
+    const int64_t vec = i / a.per, head = vec / a.n, row = a.start + vec - head * a.n;
+    const int l = (int)(i - vec * a.per);
+    const uint2 c = *reinterpret_cast<const uint2*>(a.codes[which] + (head * a.cap + row) * (8 * a.per) + 8 * l);
+    const float s = a.scales[which][head * a.cap + row];
+    const uint32_t u[2] = {c.x, c.y};
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int lo = (int8_t)(u[j / 2] >> (16 * (j & 1))), hi = (int8_t)(u[j / 2] >> (16 * (j & 1) + 8));
+        o[j] = pack_bf16x2(__fmul_rn((float)lo, s), __fmul_rn((float)hi, s));
+    }
+    *reinterpret_cast<uint4*>(a.out[which] + 8 * i) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+constexpr int KEEP_LAYERS = 64, KEEP_ROWS = 64, KEEP_THREADS = 128;
+
+struct KvKeepArgs {
+    scmx_kv_layer layer[KEEP_LAYERS];
+    const int32_t* rows;             // [n]
+    const int32_t* pos_dev;
+    int64_t pos, cap;
+    int n, row_bytes;
+};
+
+// One CTA per (head, layer, keys or values): every kept row is loaded before the first one is stored, so rows may change places.
+__global__ void __launch_bounds__(KEEP_THREADS) kv_keep_kernel(const __grid_constant__ KvKeepArgs a) {
+    constexpr int PER = KEEP_ROWS * 32 / KEEP_THREADS;      // 16-byte pieces of a thread: rows of 512 bytes at most
+    pdl_launch_dependents();
+    pdl_wait();
+    const scmx_kv_layer ly = a.layer[blockIdx.y];
+    const int64_t pos = a.pos_dev ? (int64_t)a.pos_dev[0] : a.pos;
+    if (pos < 0 || pos + a.n > a.cap) return;
+    const int tid = threadIdx.x, pieces = a.row_bytes / 16;
+    char* base = static_cast<char*>(blockIdx.z ? ly.v : ly.k) + ((int64_t)blockIdx.x * a.cap + pos) * a.row_bytes;
+    float* scales = blockIdx.z ? ly.vs : ly.ks;
+    auto source = [&](int j) { const int r = __ldg(a.rows + j); return r >= 0 && r < a.n ? r : j; };
+    uint4 w[PER];
+    float s = 0.0f;
+    int from = tid;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const int i = p * KEEP_THREADS + tid, j = i / pieces;
+        const int r = j < a.n ? source(j) : j;
+        if (r != j) w[p] = *reinterpret_cast<const uint4*>(base + (int64_t)r * a.row_bytes + 16 * (i - j * pieces));
+    }
+    if (scales != nullptr) {
+        scales += (int64_t)blockIdx.x * a.cap + pos;
+        if (tid < a.n) {
+            from = source(tid);
+            s = scales[from];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const int i = p * KEEP_THREADS + tid, j = i / pieces;
+        if (j < a.n && source(j) != j) *reinterpret_cast<uint4*>(base + (int64_t)j * a.row_bytes + 16 * (i - j * pieces)) = w[p];
+    }
+    if (scales != nullptr && tid < a.n && from != tid) scales[tid] = s;
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace scmx
+
+using namespace scmx;
+
+extern "C" int scmx_kv_append(const uint16_t* k, int64_t k_head_stride, int64_t k_row_stride, const uint16_t* v, int64_t v_head_stride,
+                              int64_t v_row_stride, int64_t L, int hk, int d, int64_t pos, const int32_t* pos_dev, int64_t capacity, int8_t* k_codes,
+                              float* k_scales, int8_t* v_codes, float* v_scales, void* stream) {
+    SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_append: null buffer");
+    SCMX_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, SCMX_EINVAL, "kv_append: head size %d (a multiple of 16 up to 256)", d);
+    SCMX_REQUIRE(hk > 0 && L >= 0 && L < (1ll << 31) && capacity >= 1, SCMX_EINVAL, "kv_append: L=%lld hk=%d capacity=%lld", (long long)L, hk, (long long)capacity);
+    SCMX_REQUIRE(pos_dev != nullptr || (pos >= 0 && pos + L <= capacity), SCMX_EINVAL, "kv_append: rows %lld .. %lld of a cache of %lld", (long long)pos,
+                 (long long)(pos + L), (long long)capacity);
+    SCMX_REQUIRE(k_head_stride % 8 == 0 && k_row_stride % 8 == 0 && v_head_stride % 8 == 0 && v_row_stride % 8 == 0 && aligned16(k) && aligned16(v) &&
+                     aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_append: vectors must start on 16-byte boundaries");
+    if (L == 0) return SCMX_OK;
+    KvWriteArgs a;
+    a.src[0] = k; a.src[1] = v; a.hs[0] = k_head_stride; a.hs[1] = v_head_stride; a.rs[0] = k_row_stride; a.rs[1] = v_row_stride;
+    a.codes[0] = k_codes; a.codes[1] = v_codes; a.scales[0] = k_scales; a.scales[1] = v_scales;
+    a.pos_dev = pos_dev; a.pos = pos; a.cap = capacity; a.vectors = (int64_t)hk * L; a.L = (int)L; a.d = d;
+    const int G = d <= 16 ? 2 : d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
+    void (*kern)(KvWriteArgs) = G == 2 ? kv_append_kernel<2> : G == 4 ? kv_append_kernel<4> : G == 8 ? kv_append_kernel<8> : G == 16 ? kv_append_kernel<16>
+                                                                                                                               : kv_append_kernel<32>;
+    const int64_t blocks = (a.vectors * G + KV_THREADS - 1) / KV_THREADS;
+    SCMX_REQUIRE(blocks < (1ll << 31), SCMX_ELIMIT, "kv_append: %lld vectors", (long long)a.vectors);
+    SCMX_PDL_OK("kv_append_kernel", launch_pdl(kern, dim3((unsigned)blocks, 2), dim3(KV_THREADS), 0, (cudaStream_t)stream, a));
+    return SCMX_OK;
+}
+
+extern "C" int scmx_kv_read(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int64_t start, int64_t n, int hk, int d,
+                            int64_t capacity, uint16_t* k, uint16_t* v, void* stream) {
+    SCMX_REQUIRE(hk > 0 && n >= 0 && start >= 0 && start + n <= capacity, SCMX_EINVAL, "kv_read: rows %lld .. %lld of a cache of %lld", (long long)start,
+                 (long long)(start + n), (long long)capacity);
+    SCMX_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, SCMX_EINVAL, "kv_read: head size %d (a multiple of 16 up to 256)", d);
+    if (n == 0) return SCMX_OK;
+    SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_read: null buffer");
+    SCMX_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_read: buffers must be 16-byte aligned");
+    KvReadArgs a;
+    a.codes[0] = k_codes; a.codes[1] = v_codes; a.scales[0] = k_scales; a.scales[1] = v_scales; a.out[0] = k; a.out[1] = v;
+    a.start = start; a.cap = capacity; a.n = n; a.per = d / 8; a.pieces = (int64_t)hk * n * a.per;
+    const int64_t blocks = (a.pieces + KV_THREADS - 1) / KV_THREADS;
+    SCMX_REQUIRE(blocks < (1ll << 31), SCMX_ELIMIT, "kv_read: %lld rows of %d heads", (long long)n, hk);
+    SCMX_PDL_OK("kv_read_kernel", launch_pdl(kv_read_kernel, dim3((unsigned)blocks, 2), dim3(KV_THREADS), 0, (cudaStream_t)stream, a));
+    return SCMX_OK;
+}
+
+extern "C" int scmx_kv_keep(const scmx_kv_layer* layers, int n_layers, const int32_t* rows, int n, int64_t pos, const int32_t* pos_dev, int hk, int d,
+                            int64_t capacity, int int8, void* stream) {
+    SCMX_REQUIRE(n_layers >= 0 && (n_layers == 0 || layers != nullptr) && rows, SCMX_EINVAL, "kv_keep: %d layers", n_layers);
+    SCMX_REQUIRE(n >= 1 && n <= KEEP_ROWS, SCMX_ELIMIT, "kv_keep: %d rows (1 .. %d)", n, KEEP_ROWS);
+    SCMX_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, SCMX_EINVAL, "kv_keep: head size %d (a multiple of 16 up to 256)", d);
+    SCMX_REQUIRE(hk > 0 && capacity >= n && (pos_dev != nullptr || (pos >= 0 && pos + n <= capacity)), SCMX_EINVAL, "kv_keep: rows %lld .. %lld of a cache of %lld",
+                 (long long)pos, (long long)(pos + n), (long long)capacity);
+    for (int i = 0; i < n_layers; ++i)
+        SCMX_REQUIRE(layers[i].k && layers[i].v && aligned16(layers[i].k) && aligned16(layers[i].v) && (!int8 || (layers[i].ks && layers[i].vs)), SCMX_EINVAL,
+                     "kv_keep: layer %d: null or unaligned buffer", i);
+    KvKeepArgs a;
+    a.rows = rows; a.pos_dev = pos_dev; a.pos = pos; a.cap = capacity; a.n = n; a.row_bytes = int8 ? d : 2 * d;
+    for (int i0 = 0; i0 < n_layers; i0 += KEEP_LAYERS) {
+        const int m = n_layers - i0 < KEEP_LAYERS ? n_layers - i0 : KEEP_LAYERS;
+        for (int i = 0; i < m; ++i) {
+            a.layer[i] = layers[i0 + i];
+            if (!int8) a.layer[i].ks = a.layer[i].vs = nullptr;
+        }
+        SCMX_PDL_OK("kv_keep_kernel", launch_pdl(kv_keep_kernel, dim3((unsigned)hk, (unsigned)m, 2), dim3(KEEP_THREADS), 0, (cudaStream_t)stream, a));
+    }
+    return SCMX_OK;
+}

@@ -12,6 +12,7 @@ import torch
 import torch.nn.functional as TF
 import torch.nn.modules.module as MODULE
 
+from . import sc_cache as C
 from . import sc_kernels as S
 
 _LINEAR_FORWARD = torch.nn.Linear.forward      # as torch defines it
@@ -90,6 +91,31 @@ class KVCache:
         self.v[:, self.offset:self.offset + L] = v.reshape(self.k.shape[0], L, -1)
         self.offset += L
         return self.k[:, :self.offset], self.v[:, :self.offset]
+
+
+class QuantKVCache:
+    """KVCache in INT8: codes k and v int8 [heads, capacity, d], a float32 scale per vector ks and vs [heads, capacity] (sc_cache.kv_append).  What a prompt
+    attends to is read back from it, so that a prompt may be cut anywhere."""
+
+    def __init__(self, heads, d, capacity, device="cuda"):
+        self.k, self.v = (torch.empty((heads, capacity, d), dtype=torch.int8, device=device) for _ in range(2))
+        self.ks, self.vs = (torch.empty((heads, capacity), dtype=torch.float32, device=device) for _ in range(2))
+        self.offset, self.capacity = 0, capacity
+
+    def reset(self):
+        """Forget the sequence; rows past `offset` are never read."""
+        self.offset = 0
+
+    def carried(self):
+        return []
+
+    def update_and_fetch(self, k, v):
+        """Appends bfloat16 k and v [heads, L, d]; the whole sequence's keys and values, read back."""
+        L = k.shape[-2]
+        assert self.offset + L <= self.capacity, "KV cache capacity exceeded"
+        C.kv_append(k.reshape(self.k.shape[0], L, -1), v.reshape(self.v.shape[0], L, -1), self)
+        self.offset += L
+        return C.kv_read(self)
 
 
 class StateCache:

@@ -1,0 +1,70 @@
+"""CPU: refusals of the cache and draft calls, before anything is launched, and the host side of draft trees."""
+import ctypes
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+
+def test_trees(scmx):
+    D = scmx.sc_draft
+    parents = [-1, 0, 0, 1, 3, 2]
+    assert D.draft_mask(parents, device="cpu").tolist() == [1, 3, 5, 11, 27, 37]
+    assert D.draft_depths(parents) == [0, 1, 1, 2, 3, 2]
+    chain = D.draft_mask([-1] + list(range(63)), device="cpu")
+    assert chain[62].item() == 2 ** 63 - 1 and chain[63].item() == -1          # all 64 bits
+    for bad in ([], [0], [-1, 1], [-1, -1], [-1, 0, 5], [-1] + [0] * 64):
+        with pytest.raises(ValueError):
+            D.check_tree(bad)
+
+
+def test_cpu_tensors_are_refused(scmx):
+    C, D = scmx.sc_cache, scmx.sc_draft
+    c = scmx.host_model.QuantKVCache(2, 64, 16, device="cpu")
+    k = torch.zeros((2, 3, 64), dtype=torch.bfloat16)
+    for call in (lambda: C.kv_append(k, k, c), lambda: C.kv_read(c, 0, 2), lambda: C.cache_attention(k, c, 1.0),
+                 lambda: C.kv_keep([c], torch.zeros(3, dtype=torch.int32)), lambda: c.update_and_fetch(k, k),
+                 lambda: D.verify_draft(torch.zeros(3, 9), torch.zeros(3, dtype=torch.long), torch.zeros(3, dtype=torch.int32), torch.zeros(3))):
+        with pytest.raises(TypeError):
+            call()
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(TypeError):
+            C.cache_attention(k, SimpleNamespace(k=torch.zeros(2, 4, 64, dtype=dtype), v=torch.zeros(2, 4, 64, dtype=dtype), offset=0), 1.0)
+
+
+P = ctypes.c_void_p(1 << 20)          # never read: every call below is refused on the host
+
+
+def _refused(scmx, name, args, text):
+    rc = getattr(scmx._lib.lib(), name)(*args)
+    assert rc < 0 and text in scmx._lib.lib().scmx_last_error_string().decode(), scmx._lib.lib().scmx_last_error_string()
+
+
+def test_entry_points_refuse(scmx):
+    def append(k=P, khs=64, krs=64, L=3, hk=2, d=64, pos=0, dev=None, cap=16, codes=P):
+        return (k, khs, krs, P, 64, 64, L, hk, d, pos, dev, cap, codes, P, P, P, None)
+    for kw, text in ((dict(k=None), "null"), (dict(d=24), "head size"), (dict(d=272), "head size"), (dict(d=0), "head size"), (dict(pos=14), "rows 14"),
+                     (dict(pos=-1), "rows -1"), (dict(krs=12), "16-byte"), (dict(k=ctypes.c_void_p((1 << 20) + 8)), "16-byte"), (dict(hk=0), "hk=0"),
+                     (dict(L=-1), "L=-1"), (dict(codes=ctypes.c_void_p((1 << 20) + 4)), "16-byte")):
+        _refused(scmx, "scmx_kv_append", append(**kw), text)
+    assert scmx._lib.lib().scmx_kv_append(*append(L=0)) == 0
+    for start, n, hk, d, text in ((0, 17, 2, 64, "rows 0"), (-1, 2, 2, 64, "rows -1"), (0, 2, 0, 64, "rows"), (0, 2, 2, 20, "head size")):
+        _refused(scmx, "scmx_kv_read", (P, P, P, P, start, n, hk, d, 16, P, P, None), text)
+    layers = (scmx._lib.ScmxKvLayer * 2)()
+    for n, pos, d, text in ((0, 0, 64, "0 rows"), (65, 0, 64, "65 rows"), (4, 13, 64, "rows 13"), (4, 0, 40, "head size"), (4, 0, 64, "layer 0")):
+        _refused(scmx, "scmx_kv_keep", (layers, 2, P, n, pos, None, 2, d, 16, 0, None), text)
+
+    def attn(q=P, qhs=64, qrs=64, int8=0, ks=None, n=3, pos=0, cap=100, hq=4, hk=2, d=64, scratch=P, size=1 << 20):
+        return (q, qhs, qrs, P, P, ks, ks, int8, None, n, pos, None, cap, hq, hk, d, 1.0, P, scratch, size, None)
+    for kw, text in ((dict(q=None), "null"), (dict(int8=1), "null"), (dict(n=0), "0 rows"), (dict(n=65), "65 rows"), (dict(d=96), "head size"), (dict(hq=5), "hq=5"),
+                     (dict(hk=0), "hk=0"), (dict(pos=98), "rows 98"), (dict(pos=-1), "rows -1"), (dict(cap=2), "rows"), (dict(qhs=66), "aligned"),
+                     (dict(q=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(pos=5000, cap=9000, size=8), "scratch"), (dict(pos=5000, cap=9000, scratch=None), "scratch")):
+        _refused(scmx, "scmx_cache_attn", attn(**kw), text)
+    assert scmx._lib.lib().scmx_cache_attn_scratch(5000, 3, 5, 2, 64) == 0
+
+    def check(n=3, V=100, ld=100, u=P, t=1.0, probs=None, ldp=0, size=1 << 20, tokens=P):
+        return (P, 1, ld, tokens, P, u, t, probs, ldp, n, V, P, P, P, P, size, None)
+    for kw, text in ((dict(n=0), "0 rows"), (dict(n=65), "65 rows"), (dict(V=0), "0 logits"), (dict(ld=99), "99"), (dict(probs=P, ldp=99), "99"), (dict(t=-1.0), "temperature"),
+                     (dict(t=float("nan")), "temperature"), (dict(t=float("inf")), "temperature"), (dict(t=1e-42), "temperature"), (dict(u=None), "random"),
+                     (dict(size=8), "scratch"), (dict(tokens=None), "null")):
+        _refused(scmx, "scmx_verify", check(**kw), text)

@@ -275,12 +275,11 @@ def require_cuda(*tensors):
 
 def require_here(*tensors, contiguous=True):
     """CUDA tensors of the current device, whose stream a call is launched on."""
-    here = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
     for t in tensors:
         if not (isinstance(t, torch.Tensor) and t.is_cuda) or (contiguous and not t.is_contiguous()):
             raise TypeError(f"expected {'contiguous ' if contiguous else ''}CUDA tensors; this package has no CPU path")
-        if t.get_device() != here:
-            raise ValueError(f"a tensor on device {t.get_device()}, the current device is {here}")
+        if t.get_device() != torch._C._cuda_getDevice():
+            raise ValueError(f"a tensor on device {t.get_device()}, the current device is {torch._C._cuda_getDevice()}")
 
 
 _sms = {}

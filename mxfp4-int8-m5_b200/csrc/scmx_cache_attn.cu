@@ -2,19 +2,23 @@
 // keys and values:  o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  j over the positions before `pos` and those
 // of the new rows that row i's mask names.
 //
-// The G query heads of a key/value head and the n rows are G n query rows that read the same keys: tiles of 16 of them meet the cache in
-// one pass (mma.sync m16n8k16, bfloat16, float32 sums).  The positions are cut into ranges, one CTA each; in a CTA every warp takes blocks of
-// 16 positions of its own, brought into its own ring in shared memory by asynchronous copies, and keeps a running maximum, sum and output
-// in registers.  The warps' states are joined in shared memory, the ranges' by a second launch.
+// The G query heads of a key/value head and the n rows are G n query rows that read the same keys: they meet the cache in one pass, up to 32 of
+// them in a CTA.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16, bfloat16, float32 sums): keys
+// and values are the 16-row operand, query rows come eight at a time, so one row costs eight and an INT8 code is converted once for
+// all rows.  The positions are cut into ranges, one CTA each; in a CTA every warp takes blocks of 16 positions of its own, brought into its own ring
+// in shared memory by asynchronous copies, and keeps a running maximum, sum and output in registers.  The maximum is only raised when a
+// score exceeds it by 2^8, so that most blocks neither exchange nor rescale anything.  The warps' states are joined in shared memory, the
+// ranges' by a second launch.
 // INT8 codes become bfloat16 exactly (8 significant bits); a position's key scale multiplies its scores, its value scale its weights.
 #include "scmx_common.cuh"
 #include "scmx_ptx.cuh"
 
 namespace scmx {
 
-constexpr int CA_WARPS = 8, CA_THREADS = 32 * CA_WARPS, CA_KEYS = 16, CA_ROWS = 16;
+constexpr int CA_KEYS = 16;             // positions of a block
 constexpr int CA_MAX_ROWS = 64;
 constexpr float CA_LOG2E = 1.4426950408889634f;
+constexpr float CA_GROWTH = 8.0f;      // log2 of how far a weight may exceed one before the maximum is raised
 
 struct CaArgs {
     const uint16_t* q;               // bf16, heads q_hs and rows q_rs elements apart
@@ -22,33 +26,40 @@ struct CaArgs {
     const float *ks, *vs;            // [hk, cap] (INT8)
     const int64_t* mask;             // [n] or null: row i sees rows 0 .. i
     const int32_t* pos_dev;
-    float* part;                     // [hk, tiles, nsplit, 16, D + 2] or null (nsplit 1)
+    float* part;                     // [hk, tiles, nsplit, rows of a tile, D + 2] or null (nsplit 1)
     uint16_t* out;                   // bf16 [n, hq d]
     int64_t q_hs, q_rs, pos, cap;
     int n, hq, hk, nsplit;
     float scale;                     // times log2(e)
 };
 
-// Positions of a call and of one range: ranges are multiples of 128, so a short cache uses the first few only.
+// Positions of a call and of one range: ranges are whole blocks and no shorter than four, so a short cache uses the first few only.
 __device__ __forceinline__ int64_t ca_pos(const int32_t* pos_dev, int64_t pos, int64_t cap, int n) {
     int64_t p = pos_dev ? (int64_t)pos_dev[0] : pos;
     return p < 0 ? 0 : p > cap - n ? cap - n : p;
 }
+constexpr int CA_MIN_RANGE = 4 * CA_KEYS;
 __device__ __forceinline__ int64_t ca_chunk(int64_t T, int nsplit) {
     const int64_t c = (T + nsplit - 1) / nsplit;
-    return (c + CA_KEYS * CA_WARPS - 1) / (CA_KEYS * CA_WARPS) * (CA_KEYS * CA_WARPS);
+    return c < CA_MIN_RANGE ? CA_MIN_RANGE : (c + CA_KEYS - 1) / CA_KEYS * CA_KEYS;
 }
 
-template <int D, bool I8>
-struct CaSmem {
+// NT: groups of eight query rows.  Warps: what registers and shared memory allow; INT8 needs more of them, its conversions are latency.
+template <int D, bool I8, int NT>
+struct CaShape {
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int WARPS = !I8 ? 8 : NT == 1 ? 16 : NT == 2 ? 12 : 8;
+    static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROW = I8 ? D : 2 * D;                        // bytes of a vector
     static constexpr int BLOCK = CA_KEYS * ROW;                       // 16 keys or values
     static constexpr int STAGE = 2 * BLOCK + (I8 ? 128 : 0);          // keys, values, their scales
     static constexpr int STAGES = 3;
     static constexpr int RING = STAGE * STAGES;
-    static constexpr int STATE = CA_ROWS * (D + 2) * 4;               // a warp's state when the warps are joined
-    static constexpr int WARP = RING > STATE ? RING : STATE;
-    static constexpr int TOTAL = WARP * CA_WARPS;
+    static constexpr int STATE = ROWS * (D + 2) * 4;                  // a warp's state when the warps are joined
+    static constexpr int WARP = ((RING > STATE ? RING : STATE) + 127) / 128 * 128;
+    static constexpr bool QREGS = NT < 4;                             // queries in registers, or in shared memory
+    static constexpr int QBYTES = QREGS ? 0 : NT * (D / 16) * 32 * 8;
+    static constexpr int TOTAL = WARP * WARPS + QBYTES;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -77,180 +88,227 @@ __device__ __forceinline__ int ca_at(int r, int c) {
     if constexpr (ROW == 64) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
     return r * ROW + ((c ^ (r & 7)) << 4);
 }
-// Two INT8 codes in the low bytes of the halves of w (the other bytes are ignored) -> two bfloat16, exactly: a code below 128 is the low
-// bits of the significand of 128 + code; its sign bit falls on the exponent's low bit, so 128 or 256 is taken off.
-__device__ __forceinline__ uint32_t i8x2_bf16(uint32_t w) {
-    const uint32_t x = (w & 0x007F007Fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
+// An 8 x 8 matrix of 16-bit values, a row to four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
+__device__ __forceinline__ float ca_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
-template <int D, bool I8>
-__global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(const CaArgs a) {
-    using L = CaSmem<D, I8>;
-    constexpr int ROW = L::ROW, PIECES = ROW / 16, KSTEPS = D / 16, NT = D / 8;
+template <int D, bool I8, int NT>
+__global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_kernel(const __grid_constant__ CaArgs a) {
+    using L = CaShape<D, I8, NT>;
+    constexpr int ROW = L::ROW, PIECES = ROW / 16, KSTEPS = D / 16, MT = D / 16, WARPS = L::WARPS;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n;
+    const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * L::ROWS;
     const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit);
     const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
     if (t0 >= T) return;
-    const unsigned char* kb = static_cast<const unsigned char*>(a.k) + (int64_t)kvh * a.cap * ROW;
-    const unsigned char* vb = static_cast<const unsigned char*>(a.v) + (int64_t)kvh * a.cap * ROW;
+    const unsigned char* kb = static_cast<const unsigned char*>(a.k) + ((int64_t)kvh * a.cap + t0) * ROW;
+    const unsigned char* vb = static_cast<const unsigned char*>(a.v) + ((int64_t)kvh * a.cap + t0) * ROW;
     unsigned char* ring = smem_raw + warp * L::WARP;
     const uint32_t ring_s = smem_u32(ring);
+    const int nkeys = (int)(t1 - t0), nblocks = (nkeys + CA_KEYS - 1) / CA_KEYS, ntail = (int)(pos - t0 < nkeys ? pos - t0 : nkeys);      // keys from ntail on are new rows (negative: from before t0)
 
-    // query rows g and g + 8 of this tile, as the A operand
-    int row[2], tok[2];
-    uint64_t sees[2];
-    uint32_t qf[KSTEPS][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        row[h] = blockIdx.z * CA_ROWS + g + 8 * h;
-        const bool on = row[h] < R;
-        tok[h] = on ? row[h] / G : 0;
-        sees[h] = !on ? 0ull : a.mask ? (uint64_t)a.mask[tok[h]] : (2ull << tok[h]) - 1ull;
-        const uint16_t* qp = a.q + (int64_t)(kvh * G + (on ? row[h] - tok[h] * G : 0)) * a.q_hs + (int64_t)tok[h] * a.q_rs;
-#pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-            if constexpr (I8) {       // the four values that one word of codes holds
-                const uint2 w = *reinterpret_cast<const uint2*>(qp + 16 * s + 4 * t4);
-                qf[s][h] = on ? w.x : 0u;
-                qf[s][2 + h] = on ? w.y : 0u;
-            } else {
-                const uint32_t lo = *reinterpret_cast<const uint32_t*>(qp + 16 * s + 2 * t4), hi = *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8 + 2 * t4);
-                qf[s][h] = on ? lo : 0u;
-                qf[s][2 + h] = on ? hi : 0u;
-            }
-        }
-    }
-
-    const int64_t nblocks = (t1 - t0 + CA_KEYS - 1) / CA_KEYS;
-    auto load = [&](int64_t b, int stage) {
+    // copies of block b: pieces lane, lane + 32, .. of 16 bytes; a warp covers whole vectors with each
+    constexpr int COPIES = CA_KEYS * PIECES / 32, RSTEP = 32 / PIECES;
+    const int lr0 = lane / PIECES, lc0 = lane % PIECES;
+    auto load = [&](int b, int stage) {
         if (b < nblocks) {
-            const int64_t key0 = t0 + b * CA_KEYS;
             const uint32_t dst = ring_s + stage * L::STAGE;
+            const int left = nkeys - b * CA_KEYS;
+            const int64_t src = (int64_t)b * L::BLOCK + lane * 16;
 #pragma unroll
-            for (int p = 0; p < CA_KEYS * PIECES / 32; ++p) {
-                const int i = p * 32 + lane, r = i / PIECES, c = i % PIECES;
-                const bool on = key0 + r < t1;
-                const int64_t off = (on ? key0 + r : t0) * ROW + 16 * c;
-                cp_async16(dst + ca_at<ROW>(r, c), kb + off, on);
-                cp_async16(dst + L::BLOCK + ca_at<ROW>(r, c), vb + off, on);
+            for (int p = 0; p < COPIES; ++p) {
+                const int r = lr0 + p * RSTEP, at = ca_at<ROW>(r, lc0);
+                const bool on = r < left;
+                const int64_t off = on ? src + p * 512 : 0;
+                cp_async16(dst + at, kb + off, on);
+                cp_async16(dst + L::BLOCK + at, vb + off, on);
             }
             if constexpr (I8) {
-                const bool on = key0 + (lane & 15) < t1;
-                const float* s = (lane < 16 ? a.ks : a.vs) + (int64_t)kvh * a.cap + (on ? key0 + (lane & 15) : t0);
+                const bool on = (lane & 15) < left;
+                const float* s = (lane < 16 ? a.ks : a.vs) + (int64_t)kvh * a.cap + t0 + (on ? b * CA_KEYS + (lane & 15) : 0);
                 cp_async4(dst + 2 * L::BLOCK + 4 * lane, s, on);
             }
         }
         cp_commit();
     };
 #pragma unroll
-    for (int s = 0; s < L::STAGES - 1; ++s) load(warp + s * CA_WARPS, s);
+    for (int s = 0; s < L::STAGES - 1; ++s) load(warp + s * WARPS, s);
 
-    float o[NT][4], mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    // query rows, as the B operand: row g of each group of eight
+    auto query = [&](int nt, int s) -> uint2 {
+        const int r = row0 + 8 * nt + g, tok = r / G;
+        if (r >= R) return make_uint2(0, 0);
+        const uint16_t* qp = a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 16 * s;
+        if constexpr (I8) return *reinterpret_cast<const uint2*>(qp + 4 * t4);       // the four values that one word of codes holds
+        return make_uint2(*reinterpret_cast<const uint32_t*>(qp + 2 * t4), *reinterpret_cast<const uint32_t*>(qp + 8 + 2 * t4));
+    };
+    uint2 qf[L::QREGS ? NT : 1][L::QREGS ? KSTEPS : 1];
+    uint2* qs = reinterpret_cast<uint2*>(smem_raw + L::WARP * WARPS);
+    if constexpr (L::QREGS) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+            for (int s = 0; s < KSTEPS; ++s) qf[nt][s] = query(nt, s);
+    } else {
+        for (int i = warp; i < NT * KSTEPS; i += WARPS) qs[i * 32 + lane] = query(i / KSTEPS, i % KSTEPS);
+        __syncthreads();
+    }
 
+    // rows 2 t4 and 2 t4 + 1 of each group: maximum and sum; output: 16 values of the vectors times eight rows
+    float o[MT][NT][4], mx[NT][2], sum[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mx[nt][e] = -INFINITY;
+            sum[nt][e] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.0f;
+    }
+
+    const int lr = lane & 7, lm = lane >> 3;            // row of a matrix load, and which of its four matrices
     int stage = 0;
-    for (int64_t b = warp; b < nblocks; b += CA_WARPS) {
+    for (int b = warp; b < nblocks; b += WARPS) {
         cp_wait<L::STAGES - 2>();
         __syncwarp();
-        load(b + (L::STAGES - 1) * CA_WARPS, stage == 0 ? L::STAGES - 1 : stage - 1);
+        load(b + (L::STAGES - 1) * WARPS, stage == 0 ? L::STAGES - 1 : stage - 1);
         const unsigned char* blk = ring + stage * L::STAGE;
         const uint32_t kst = ring_s + stage * L::STAGE, vst = kst + L::BLOCK;
-        const float* scales = reinterpret_cast<const float*>(blk + 2 * L::BLOCK);
-        const int64_t key0 = t0 + b * CA_KEYS;
-        // scores of 16 rows and 2 x 8 keys
-        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-        const int lr = lane & 7, lm = lane >> 3;        // row of a matrix load, and which of its four matrices
+        // scores: keys g and g + 8, rows 2 t4 and 2 t4 + 1
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
+        auto scores = [&](int c, const uint32_t (&w)[4]) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint2 q = L::QREGS ? qf[L::QREGS ? nt : 0][L::QREGS ? c : 0] : qs[(nt * KSTEPS + c) * 32 + lane];
+                mma_bf16(s[nt], w, q.x, q.y);
+            }
+        };
         if constexpr (I8) {
 #pragma unroll
             for (int c = 0; c < KSTEPS; c += 2) {
-                uint32_t w[4];                          // keys 0-7 pieces c, c + 1, keys 8-15 pieces c, c + 1
-                ldsm4(kst + ca_at<ROW>(lr + 8 * (lm >> 1), c + (lm & 1)), w);
+                uint32_t w[4];                          // keys 0-7, keys 8-15 of piece c, the same of piece c + 1
+                ldsm4(kst + ca_at<ROW>(lr + 8 * (lm & 1), c + (lm >> 1)), w);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        mma_bf16(s[j], qf[c + e], i8x2_bf16(__byte_perm(w[2 * j + e], 0, 0x4140)), i8x2_bf16(__byte_perm(w[2 * j + e], 0, 0x4342)));
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t f[4] = {i8x2_bf16(__byte_perm(w[2 * e], 0, 0x4140)), i8x2_bf16(__byte_perm(w[2 * e + 1], 0, 0x4140)),
+                                           i8x2_bf16(__byte_perm(w[2 * e], 0, 0x4342)), i8x2_bf16(__byte_perm(w[2 * e + 1], 0, 0x4342))};
+                    scores(c + e, f);
+                }
             }
         } else {
 #pragma unroll
             for (int c = 0; c < KSTEPS; ++c) {
                 uint32_t w[4];
-                ldsm4(kst + ca_at<ROW>(lr + 8 * (lm >> 1), 2 * c + (lm & 1)), w);
-                mma_bf16(s[0], qf[c], w[0], w[1]);
-                mma_bf16(s[1], qf[c], w[2], w[3]);
+                ldsm4(kst + ca_at<ROW>(lr + 8 * (lm & 1), 2 * c + (lm >> 1)), w);
+                scores(c, w);
             }
         }
-        // the thread's keys: 2 t4, 2 t4 + 1 of each group of eight
-        float vsc[2][2];
-        bool vis[2][2][2];                              // row half, key group, key
-        const bool tail = key0 + CA_KEYS > pos;         // some keys are new rows, or past the end
+        float kf[2] = {a.scale, a.scale}, vf[2] = {1.0f, 1.0f};
+        if constexpr (I8) {
+            const float* scales = reinterpret_cast<const float*>(blk + 2 * L::BLOCK);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int kk = 8 * j + 2 * t4 + e;
-                float f = a.scale;
-                if constexpr (I8) {
-                    f *= scales[kk];
-                    vsc[j][e] = scales[16 + kk];
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    bool v = true;
-                    if (tail) {
-                        const int64_t d = key0 + kk - pos;
-                        v = row[h] < R && (d < 0 || (d < a.n && ((sees[h] >> d) & 1)));
-                    }
-                    vis[h][j][e] = v;
-                    s[j][2 * h + e] = v ? s[j][2 * h + e] * f : -INFINITY;
-                }
+            for (int h = 0; h < 2; ++h) {
+                kf[h] *= scales[g + 8 * h];
+                vf[h] = scales[16 + g + 8 * h];
             }
-        uint32_t pa[4];
-        float p[2][4];
+        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float m = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float mn = fmaxf(mx[h], m);
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            if (__any_sync(0xffffffffu, mn > mx[h])) {
-                const float f = exp2f(mx[h] - base);
-                sum[h] *= f;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    o[i][2 * h] *= f;
-                    o[i][2 * h + 1] *= f;
-                }
-                mx[h] = mn;
-            }
+            for (int j = 0; j < 4; ++j) s[nt][j] *= kf[j >> 1];
+        const int d0 = b * CA_KEYS - ntail;             // the block's first key, counted from the first new row
+        const bool tail = d0 + CA_KEYS > 0;             // some keys are new rows, or past the end
+        uint32_t seen = 0xFFFFFFFFu;                    // bit 4 nt + j
+        if (tail) {
+            seen = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float x = exp2f(s[j][2 * h + e] - base);
-                    sum[h] += x;
-                    p[j][2 * h + e] = I8 ? (vis[h][j][e] ? x * vsc[j][e] : 0.0f) : x;
+                    const int r = row0 + 8 * nt + 2 * t4 + e, tok = r / G;
+                    if (r < R) {
+                        const uint64_t bits = a.mask ? (uint64_t)a.mask[tok] : (2ull << tok) - 1ull;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int d = d0 + g + 8 * h;
+                            if (d < 0 || (d < a.n && (bits >> d & 1))) seen |= 1u << (4 * nt + 2 * h + e);
+                        }
+                    }
                 }
-            pa[h] = pack_bf16x2(p[0][2 * h], p[0][2 * h + 1]);
-            pa[2 + h] = pack_bf16x2(p[1][2 * h], p[1][2 * h + 1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!(seen >> (4 * nt + j) & 1)) s[nt][j] = -INFINITY;
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grow = grow || fmaxf(s[nt][e], s[nt][2 + e]) > mx[nt][e] + CA_GROWTH;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+                    m = fmaxf(m, mx[nt][e]);
+                    const float f = mx[nt][e] == -INFINITY ? 0.0f : ca_ex2(mx[nt][e] - m);      // nothing so far: sum and output are zero
+                    mx[nt][e] = m;
+                    sum[nt][e] *= f;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[i][nt][e] *= f;
+                        o[i][nt][2 + e] *= f;
+                    }
+                }
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float base = mx[nt][e] == -INFINITY ? 0.0f : mx[nt][e];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float& x = s[nt][2 * h + e];
+                    x = ca_ex2(x - base);
+                    sum[nt][e] += x;
+                    if constexpr (I8) {
+                        x *= vf[h];
+                        if (tail && !(seen >> (4 * nt + 2 * h + e) & 1)) x = 0.0f;      // its scale may be anything
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) pb[nt][h] = transpose8(pack_bf16x2(s[nt][2 * h], s[nt][2 * h + 1]));
         }
         // a value that is not finite must not reach rows that do not see it: such blocks, which only new rows can make, go key by key
         bool odd = false;
         if constexpr (!I8) {
             if (tail) {
 #pragma unroll
-                for (int i = 0; i < CA_KEYS * PIECES / 32; ++i) {
+                for (int i = 0; i < COPIES; ++i) {
                     const uint4 w = *reinterpret_cast<const uint4*>(blk + L::BLOCK + 16 * (32 * i + lane));
                     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -260,22 +318,26 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(const CaArgs a) 
             }
         }
         if (odd) {
-#pragma unroll
+#pragma unroll 1
             for (int kk = 0; kk < CA_KEYS; ++kk) {
-                const int j = kk >> 3, e = kk & 1, src = (lane & ~3) | ((kk & 7) >> 1);
+                const int src = 4 * (kk & 7) + t4;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float w = __shfl_sync(0xffffffffu, p[j][2 * h + e], src);
-                    const bool on = __shfl_sync(0xffffffffu, (int)vis[h][j][e], src) != 0;
-                    if (on) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < NT; ++i) {
-                            const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + L::BLOCK + ca_at<ROW>(kk, i) + 4 * t4);
-                            o[i][2 * h] = fmaf(w, bf16_lo(x), o[i][2 * h]);
-                            o[i][2 * h + 1] = fmaf(w, bf16_hi(x), o[i][2 * h + 1]);
+                    for (int e = 0; e < 2; ++e) {
+                        const float lo = __shfl_sync(0xffffffffu, s[nt][e], src), hi = __shfl_sync(0xffffffffu, s[nt][2 + e], src);
+                        const uint32_t bits = __shfl_sync(0xffffffffu, seen, src);
+                        const float w = kk < 8 ? lo : hi;
+                        if (bits >> (4 * nt + (kk < 8 ? 0 : 2) + e) & 1) {
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const float x = bf16_to_f32(*reinterpret_cast<const uint16_t*>(blk + L::BLOCK + ca_at<ROW>(kk, 2 * i + h) + 2 * g));
+                                    o[i][nt][2 * h + e] = fmaf(w, x, o[i][nt][2 * h + e]);
+                                }
                         }
                     }
-                }
             }
         } else if constexpr (I8) {
 #pragma unroll
@@ -285,16 +347,20 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(const CaArgs a) 
                 for (int r = 0; r < 4; ++r)
                     w[r] = *reinterpret_cast<const uint32_t*>(blk + L::BLOCK + ca_at<ROW>(2 * t4 + (r & 1) + 8 * (r >> 1), 2 * cg + (g >> 2)) + 4 * (g & 3));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    mma_bf16(o[4 * cg + j], pa, i8x2_bf16(__byte_perm(w[0], w[1], 0x4400 + j * 0x1111)), i8x2_bf16(__byte_perm(w[2], w[3], 0x4400 + j * 0x1111)));
+                for (int j = 0; j < 2; ++j) {           // operand rows g and g + 8: values 4 g + 2 j and 4 g + 2 j + 1
+                    const uint32_t f[4] = {i8x2_bf16(__byte_perm(w[0], w[1], 0x4400 + 2 * j * 0x1111)), i8x2_bf16(__byte_perm(w[0], w[1], 0x4400 + (2 * j + 1) * 0x1111)),
+                                           i8x2_bf16(__byte_perm(w[2], w[3], 0x4400 + 2 * j * 0x1111)), i8x2_bf16(__byte_perm(w[2], w[3], 0x4400 + (2 * j + 1) * 0x1111))};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[2 * cg + j][nt], f, pb[nt][0], pb[nt][1]);
+                }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NT; i += 2) {
-                uint32_t w[4];
-                ldsm4_t(vst + ca_at<ROW>(lr + 8 * (lm & 1), i + (lm >> 1)), w);
-                mma_bf16(o[i], pa, w[0], w[1]);
-                mma_bf16(o[i + 1], pa, w[2], w[3]);
+            for (int i = 0; i < MT; ++i) {
+                uint32_t w[4];                          // values 0-7, 8-15 of keys 0-7, the same of keys 8-15
+                ldsm4_t(vst + ca_at<ROW>(lr + 8 * (lm >> 1), 2 * i + (lm & 1)), w);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_bf16(o[i][nt], w, pb[nt][0], pb[nt][1]);
             }
         }
         stage = stage + 1 == L::STAGES ? 0 : stage + 1;
@@ -302,41 +368,41 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(const CaArgs a) 
     cp_wait<0>();
     __syncwarp();
 
-    // the warps' states, joined: output in the operand's order of values
+    // the warps' states, joined
     float* st = reinterpret_cast<float*>(ring);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        float* r = st + (g + 8 * h) * (D + 2);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int e = 0; e < 2; ++e) {
+            float l = sum[nt][e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = I8 ? 32 * (i >> 2) + 8 * t4 + 4 * e + (i & 3) : 8 * i + 2 * t4 + e;
-                r[d] = o[i][2 * h + e];
+            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            float* r = st + (8 * nt + 2 * t4 + e) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) r[I8 ? 32 * (i >> 1) + 4 * g + 2 * (i & 1) + h : 16 * i + 8 * h + g] = o[i][nt][2 * h + e];
+            if (g == 0) {
+                r[D] = mx[nt][e];
+                r[D + 1] = l;
             }
-        if (t4 == 0) {
-            r[D] = mx[h];
-            r[D + 1] = sum[h];
         }
-    }
     __syncthreads();
-    for (int i = threadIdx.x; i < CA_ROWS * D; i += CA_THREADS) {
-        const int r = i / D, d = i - r * D, rr = blockIdx.z * CA_ROWS + r;
+    const int live = nblocks < WARPS ? nblocks : WARPS;       // warps that had a block
+    for (int i = threadIdx.x; i < L::ROWS * D; i += L::THREADS) {
+        const int r = i / D, d = i - r * D, rr = row0 + r;
         if (rr >= R) break;
+        const float* x = reinterpret_cast<const float*>(smem_raw) + r * (D + 2);
+        constexpr int STRIDE = L::WARP / 4;
         float m = -INFINITY, l = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < CA_WARPS; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem_raw + w * L::WARP)[r * (D + 2) + D]);
-#pragma unroll
-        for (int w = 0; w < CA_WARPS; ++w) {
-            const float* x = reinterpret_cast<const float*>(smem_raw + w * L::WARP) + r * (D + 2);
-            const float f = x[D] == -INFINITY ? 0.0f : exp2f(x[D] - m);
-            l += x[D + 1] * f;
-            v += f == 0.0f ? 0.0f : x[d] * f;
+        for (int w = 0; w < live; ++w) m = fmaxf(m, x[w * STRIDE + D]);
+        for (int w = 0; w < live; ++w) {
+            const float f = x[w * STRIDE + D] == -INFINITY ? 0.0f : ca_ex2(x[w * STRIDE + D] - m);
+            l += x[w * STRIDE + D + 1] * f;
+            v += f == 0.0f ? 0.0f : x[w * STRIDE + d] * f;
         }
         if (a.part != nullptr) {
-            float* y = a.part + ((((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * CA_ROWS + r) * (D + 2);
+            float* y = a.part + ((((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * L::ROWS + r) * (D + 2);
             y[d] = v;
             if (d == 0) {
                 y[D] = m;
@@ -349,29 +415,47 @@ __global__ void __launch_bounds__(CA_THREADS) cache_attn_kernel(const CaArgs a) 
     }
 }
 
-// Joins the ranges: one warp per query row.
+// Joins the ranges: one warp per query row.  Lane s holds the maximum and sum of range s; the outputs are taken four ranges at a time.
 template <int D>
-__global__ void __launch_bounds__(128) cache_attn_join_kernel(const CaArgs a, int tiles) {
+__global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ CaArgs a, int tiles, int rows) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, G = a.hq / a.hk, R = G * a.n;
     const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (i >= a.hk * R) return;
-    const int kvh = i / R, r = i - kvh * R, tile = r / CA_ROWS;
+    const int kvh = i / R, r = i - kvh * R, tile = r / rows;
     const int64_t T = ca_pos(a.pos_dev, a.pos, a.cap, a.n) + a.n, chunk = ca_chunk(T, a.nsplit);
-    const int active = (int)((T + chunk - 1) / chunk);
-    const float* x = a.part + (((int64_t)kvh * tiles + tile) * a.nsplit * CA_ROWS + r % CA_ROWS) * (D + 2);
-    constexpr int STRIDE = CA_ROWS * (D + 2), E = D / 32;
-    float m = -INFINITY;
-    for (int s = 0; s < active; ++s) m = fmaxf(m, x[(int64_t)s * STRIDE + D]);
-    float l = 0.0f, v[E] = {};
-    for (int s = 0; s < active; ++s) {
-        const float* y = x + (int64_t)s * STRIDE;
-        const float f = y[D] == -INFINITY ? 0.0f : exp2f(y[D] - m);
-        if (f == 0.0f) continue;
-        l += y[D + 1] * f;
+    const int active = (int)((T + chunk - 1) / chunk), stride = rows * (D + 2);
+    const float* x = a.part + ((int64_t)kvh * tiles + tile) * a.nsplit * stride + (r - tile * rows) * (D + 2);
+    constexpr int E = D / 32;
+    float m = -INFINITY, l = 0.0f, v[E] = {};
+    for (int s0 = 0; s0 < active; s0 += 32) {
+        const bool on = s0 + lane < active;
+        const float* y = x + (int64_t)(s0 + lane) * stride;
+        const float ms = on ? y[D] : -INFINITY, ls = on ? y[D + 1] : 0.0f, mn = fmaxf(m, warp_max(ms));
+        const float f = ms == -INFINITY ? 0.0f : ca_ex2(ms - mn), old = m == -INFINITY ? 0.0f : ca_ex2(m - mn);
+        float lw = ls * f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] += y[lane * E + e] * f;
+        for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+        l = l * old + lw;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= old;
+        m = mn;
+        const int count = active - s0 < 32 ? active - s0 : 32;
+        for (int s = 0; s < count; s += 4) {
+            float z[4][E], w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = __shfl_sync(0xffffffffu, f, (s + j) & 31);
+#pragma unroll
+                for (int e = 0; e < E; ++e) z[j][e] = s + j < count ? x[(int64_t)(s0 + s + j) * stride + lane * E + e] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (s + j < count && w[j] != 0.0f)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] += z[j][e] * w[j];
+        }
     }
     const int tk = r / G, hd = kvh * G + r - tk * G;
     uint16_t* o = a.out + (int64_t)tk * a.hq * D + hd * D + lane * E;
@@ -379,29 +463,39 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const CaArgs a, in
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(o + e) = l == 0.0f ? 0u : pack_bf16x2(v[e] / l, v[e + 1] / l);
 }
 
-// Ranges of positions: as many CTAs as multiprocessors, none shorter than one block for every warp.
-static int ca_splits(int64_t positions, int hk, int tiles) {
-    const int64_t most = (positions + CA_KEYS * CA_WARPS - 1) / (CA_KEYS * CA_WARPS), want = sm_count() / ((int64_t)hk * tiles);
+// How a call is cut: groups of eight query rows in a CTA, tiles of them, ranges of positions (as many CTAs as multiprocessors).
+struct CaPlan { int nt, tiles, nsplit; };
+static CaPlan ca_plan(int64_t positions, int R, int hk) {
+    CaPlan p;
+    p.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+    p.tiles = (R + 8 * p.nt - 1) / (8 * p.nt);
+    const int64_t most = (positions + CA_MIN_RANGE - 1) / CA_MIN_RANGE, want = sm_count() / ((int64_t)hk * p.tiles);
     const int64_t s = want < most ? want : most;
-    return s < 1 ? 1 : (int)s;
+    p.nsplit = s < 1 ? 1 : (int)s;
+    return p;
 }
 
-template <int D, bool I8>
-static int launch_ca(const CaArgs& a, int tiles, cudaStream_t st) {
-    using L = CaSmem<D, I8>;
+template <int D, bool I8, int NT>
+static int launch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
+    using L = CaShape<D, I8, NT>;
     static bool configured[64] = {};
     const int dev = current_device();
     SCMX_REQUIRE(dev >= 0, SCMX_ECUDA, "no current CUDA device (ordinal 0..63)");
     if (!configured[dev]) {
-        SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+        SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<D, I8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
         configured[dev] = true;
     }
-    SCMX_PDL_OK("cache_attn_kernel", launch_pdl(cache_attn_kernel<D, I8>, dim3((unsigned)a.hk, (unsigned)a.nsplit, (unsigned)tiles), dim3(CA_THREADS),
+    SCMX_PDL_OK("cache_attn_kernel", launch_pdl(cache_attn_kernel<D, I8, NT>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles), dim3(L::THREADS),
                                                 (size_t)L::TOTAL, st, a));
     if (a.part != nullptr)
-        SCMX_PDL_OK("cache_attn_join_kernel", launch_pdl(cache_attn_join_kernel<D>, dim3((unsigned)((a.hq * a.n + 3) / 4)), dim3(128), 0, st, a, tiles));
+        SCMX_PDL_OK("cache_attn_join_kernel", launch_pdl(cache_attn_join_kernel<D>, dim3((unsigned)((a.hq * a.n + 3) / 4)), dim3(128), 0, st, a, p.tiles, L::ROWS));
     return SCMX_OK;
 }
+template <int D, bool I8>
+static int dispatch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
+    return p.nt == 1 ? launch_ca<D, I8, 1>(a, p, st) : p.nt == 2 ? launch_ca<D, I8, 2>(a, p, st) : launch_ca<D, I8, 4>(a, p, st);
+}
+static int64_t ca_scratch(const CaPlan& p, int hk, int d) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * 8 * p.nt * (d + 2) * 4; }
 
 }  // namespace scmx
 
@@ -409,8 +503,7 @@ using namespace scmx;
 
 extern "C" int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int hk, int d) {
     if (positions < 1 || n < 1 || n > CA_MAX_ROWS || hk < 1 || hq < hk || hq % hk || (d != 64 && d != 128)) return 0;
-    const int tiles = (hq / hk * n + CA_ROWS - 1) / CA_ROWS, ns = ca_splits(positions, hk, tiles);
-    return ns == 1 ? 0 : (int64_t)hk * tiles * ns * CA_ROWS * (d + 2) * 4;
+    return ca_scratch(ca_plan(positions, hq / hk * n, hk), hk, d);
 }
 
 extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,
@@ -425,14 +518,14 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
     SCMX_REQUIRE(q_head_stride % 4 == 0 && q_row_stride % 4 == 0 && ((uintptr_t)q & 7) == 0 && ((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 &&
                      ((uintptr_t)out & 3) == 0, SCMX_EINVAL, "cache_attn: query rows must be 8-byte and caches 16-byte aligned");
     CaArgs a;
-    const int tiles = (hq / hk * n + CA_ROWS - 1) / CA_ROWS;
-    a.nsplit = ca_splits(pos_dev ? capacity : pos + n, hk, tiles);
-    const int64_t need = scmx_cache_attn_scratch(pos_dev ? capacity : pos + n, n, hq, hk, d);
+    const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk);
+    a.nsplit = p.nsplit;
+    const int64_t need = ca_scratch(p, hk, d);
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",
                  (long long)scratch_bytes, (long long)need);
     a.q = q; a.q_hs = q_head_stride; a.q_rs = q_row_stride; a.k = k; a.v = v; a.ks = k_scales; a.vs = v_scales; a.mask = mask; a.pos_dev = pos_dev; a.pos = pos;
     a.part = need ? static_cast<float*>(scratch) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.scale = scale * CA_LOG2E;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (d == 128) return int8 ? launch_ca<128, true>(a, tiles, st) : launch_ca<128, false>(a, tiles, st);
-    return int8 ? launch_ca<64, true>(a, tiles, st) : launch_ca<64, false>(a, tiles, st);
+    if (d == 128) return int8 ? dispatch_ca<128, true>(a, p, st) : dispatch_ca<128, false>(a, p, st);
+    return int8 ? dispatch_ca<64, true>(a, p, st) : dispatch_ca<64, false>(a, p, st);
 }

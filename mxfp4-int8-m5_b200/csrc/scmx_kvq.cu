@@ -5,76 +5,112 @@
 
 namespace scmx {
 
-constexpr int KV_THREADS = 256;
+constexpr int KV_THREADS = 256, KV_TURNS = 4;      // vectors of a thread whose loads are in flight together
 
 struct KvWriteArgs {
-    const uint16_t *src[2];          // bf16 keys, values
-    int64_t hs[2], rs[2];            // their head and row strides in elements
-    int8_t* codes[2];                // [hk, cap, d]
-    float* scales[2];                // [hk, cap]
+    const uint16_t *k, *v;           // bf16 [hk, L, d]
+    int64_t k_hs, k_rs, v_hs, v_rs;  // head and row strides in elements
+    int8_t *kc, *vc;                 // [hk, cap, d]
+    float *ks, *vs;                  // [hk, cap]
     const int32_t* pos_dev;
-    int64_t pos, cap, vectors;       // vectors: hk * L
-    int L, d;
+    int64_t pos, cap;
+    int L, hk, d;
 };
 
-// A vector belongs to G lanes of 8 values each (G the power of two from d / 8 on); blockIdx.y: 0 keys, 1 values.
+// A vector belongs to G lanes of 8 values each (G the power of two from d / 8 on).  blockIdx: rows, heads, keys or values.
 template <int G>
-__global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const KvWriteArgs a) {
+__global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_constant__ KvWriteArgs a) {
+    constexpr int ROWS = KV_THREADS / G;
     pdl_launch_dependents();
     pdl_wait();
-    const int which = blockIdx.y, l = threadIdx.x % G;
-    const int64_t i = (int64_t)blockIdx.x * (KV_THREADS / G) + threadIdx.x / G;
-    const int64_t pos = a.pos_dev ? (int64_t)a.pos_dev[0] : a.pos;
-    const int64_t head = i / a.L, row = i - head * a.L, at = pos + row;
-    const bool on = i < a.vectors && 8 * l < a.d;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (on) w = *reinterpret_cast<const uint4*>(a.src[which] + head * a.hs[which] + row * a.rs[which] + 8 * l);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    uint32_t top = 0;                // magnitudes of bfloat16 order like their bits, infinities and NaN last
+    const bool val = blockIdx.z != 0;
+    const int l = threadIdx.x % G, first = blockIdx.x * (ROWS * KV_TURNS) + threadIdx.x / G;
+    const int64_t pos = a.pos_dev ? (int64_t)a.pos_dev[0] : a.pos, rs = val ? a.v_rs : a.k_rs;
+    for (int head = blockIdx.y; head < a.hk; head += gridDim.y) {
+        const uint16_t* src = (val ? a.v + head * a.v_hs : a.k + head * a.k_hs) + 8 * l;
+        uint4 w[KV_TURNS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+        for (int i = 0; i < KV_TURNS; ++i) {
+            const int row = first + i * ROWS;
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (row < a.L && 8 * l < a.d) w[i] = *reinterpret_cast<const uint4*>(src + row * rs);
+        }
+        int8_t* codes = (val ? a.vc : a.kc) + head * a.cap * a.d + 8 * l;
+        float* scales = (val ? a.vs : a.ks) + head * a.cap;
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float s, qi;
-    quant_scale(__uint_as_float(top << 16), s, qi);
-    if (s < 1.17549435e-38f) s = qi = 0.0f;                  // 1 / s would overflow: such a vector is stored as zero
-    if (top >= 0x7F80u) { s = __uint_as_float(0x7FC00000u); qi = 0.0f; }      // a value that is not finite: the vector reads back as NaN
-    if (!on || at < 0 || at >= a.cap) return;                // a device-side position beyond the cache: the row is dropped
-    uint32_t q[2] = {0, 0};
-    if (qi > 0.0f) {
-        q[0] = quant4(bf16_lo(u[0]), bf16_hi(u[0]), bf16_lo(u[1]), bf16_hi(u[1]), qi);
-        q[1] = quant4(bf16_lo(u[2]), bf16_hi(u[2]), bf16_lo(u[3]), bf16_hi(u[3]), qi);
+        for (int i = 0; i < KV_TURNS; ++i) {
+            if (blockIdx.x * (ROWS * KV_TURNS) + i * ROWS >= a.L) break;
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t top = 0;                // magnitudes of bfloat16 order like their bits, infinities and NaN last
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float s, qi;
+            quant_scale(__uint_as_float(top << 16), s, qi);
+            if (s < 1.17549435e-38f) s = qi = 0.0f;                  // 1 / s would overflow: such a vector is stored as zero
+            if (top >= 0x7F80u) { s = __uint_as_float(0x7FC00000u); qi = 0.0f; }      // a value that is not finite: the vector reads back as NaN
+            const int row = first + i * ROWS;
+            const int64_t at = pos + row;
+            if (row >= a.L || 8 * l >= a.d || at < 0 || at >= a.cap) continue;      // a device-side position beyond the cache: the row is dropped
+            uint32_t q[2] = {0, 0};
+            if (qi > 0.0f) {
+                q[0] = quant4(bf16_lo(u[0]), bf16_hi(u[0]), bf16_lo(u[1]), bf16_hi(u[1]), qi);
+                q[1] = quant4(bf16_lo(u[2]), bf16_hi(u[2]), bf16_lo(u[3]), bf16_hi(u[3]), qi);
+            }
+            *reinterpret_cast<uint2*>(codes + at * a.d) = make_uint2(q[0], q[1]);
+            if (l == 0) scales[at] = s;
+        }
     }
-    *reinterpret_cast<uint2*>(a.codes[which] + (head * a.cap + at) * a.d + 8 * l) = make_uint2(q[0], q[1]);
-    if (l == 0) a.scales[which][head * a.cap + at] = s;
 }
 
 struct KvReadArgs {
-    const int8_t* codes[2];
-    const float* scales[2];
-    uint16_t* out[2];                // bf16 [hk, n, d]
-    int64_t start, cap, n, pieces;   // pieces of 8 values: hk * n * d / 8
-    int per;                         // d / 8
+    const int8_t *kc, *vc;
+    const float *ks, *vs;
+    uint16_t *k, *v;                 // bf16 [hk, n, d]
+    int64_t start, cap, n;
+    int hk, d, pieces, rows;         // pieces of 16 values of a vector; vectors that a CTA takes in a turn
 };
 
-__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvReadArgs a) {
+// A lane takes 16 codes; codes become bfloat16 exactly, and their product with the scale is rounded once.
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvReadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int which = blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * KV_THREADS + threadIdx.x;
-    if (i >= a.pieces) return;
-    const int64_t vec = i / a.per, head = vec / a.n, row = a.start + vec - head * a.n;
-    const int l = (int)(i - vec * a.per);
-    const uint2 c = *reinterpret_cast<const uint2*>(a.codes[which] + (head * a.cap + row) * (8 * a.per) + 8 * l);
-    const float s = a.scales[which][head * a.cap + row];
-    const uint32_t u[2] = {c.x, c.y};
-    uint32_t o[4];
+    const bool val = blockIdx.z != 0;
+    const int r = threadIdx.x / a.pieces, l = threadIdx.x - r * a.pieces;
+    if (r >= a.rows) return;
+    for (int head = blockIdx.y; head < a.hk; head += gridDim.y) {
+        const int8_t* codes = (val ? a.vc : a.kc) + (head * a.cap + a.start) * a.d + 16 * l;
+        const float* scales = (val ? a.vs : a.ks) + head * a.cap + a.start;
+        uint16_t* out = (val ? a.v : a.k) + head * a.n * a.d + 16 * l;
+        const int64_t first = (int64_t)blockIdx.x * a.rows * KV_TURNS + r;
+        uint4 c[KV_TURNS];
+        float s[KV_TURNS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int lo = (int8_t)(u[j / 2] >> (16 * (j & 1))), hi = (int8_t)(u[j / 2] >> (16 * (j & 1) + 8));
-        o[j] = pack_bf16x2(__fmul_rn((float)lo, s), __fmul_rn((float)hi, s));
+        for (int i = 0; i < KV_TURNS; ++i) {
+            const int64_t row = first + i * a.rows;
+            if (row < a.n) {
+                c[i] = *reinterpret_cast<const uint4*>(codes + row * a.d);
+                s[i] = scales[row];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < KV_TURNS; ++i) {
+            const int64_t row = first + i * a.rows;
+            if (row >= a.n) continue;
+            const uint32_t u[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = i8x2_bf16(__byte_perm(u[j], 0, 0x4140)), hi = i8x2_bf16(__byte_perm(u[j], 0, 0x4342));
+                o[2 * j] = pack_bf16x2(__fmul_rn(bf16_lo(lo), s[i]), __fmul_rn(bf16_hi(lo), s[i]));
+                o[2 * j + 1] = pack_bf16x2(__fmul_rn(bf16_lo(hi), s[i]), __fmul_rn(bf16_hi(hi), s[i]));
+            }
+            uint4* p = reinterpret_cast<uint4*>(out + row * a.d);
+            p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
     }
-    *reinterpret_cast<uint4*>(a.out[which] + 8 * i) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 constexpr int KEEP_LAYERS = 64, KEEP_ROWS = 64, KEEP_THREADS = 128;
@@ -142,15 +178,15 @@ extern "C" int scmx_kv_append(const uint16_t* k, int64_t k_head_stride, int64_t 
                      aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_append: vectors must start on 16-byte boundaries");
     if (L == 0) return SCMX_OK;
     KvWriteArgs a;
-    a.src[0] = k; a.src[1] = v; a.hs[0] = k_head_stride; a.hs[1] = v_head_stride; a.rs[0] = k_row_stride; a.rs[1] = v_row_stride;
-    a.codes[0] = k_codes; a.codes[1] = v_codes; a.scales[0] = k_scales; a.scales[1] = v_scales;
-    a.pos_dev = pos_dev; a.pos = pos; a.cap = capacity; a.vectors = (int64_t)hk * L; a.L = (int)L; a.d = d;
+    a.k = k; a.v = v; a.k_hs = k_head_stride; a.v_hs = v_head_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride;
+    a.kc = k_codes; a.vc = v_codes; a.ks = k_scales; a.vs = v_scales;
+    a.pos_dev = pos_dev; a.pos = pos; a.cap = capacity; a.L = (int)L; a.hk = hk; a.d = d;
     const int G = d <= 16 ? 2 : d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
     void (*kern)(KvWriteArgs) = G == 2 ? kv_append_kernel<2> : G == 4 ? kv_append_kernel<4> : G == 8 ? kv_append_kernel<8> : G == 16 ? kv_append_kernel<16>
                                                                                                                                : kv_append_kernel<32>;
-    const int64_t blocks = (a.vectors * G + KV_THREADS - 1) / KV_THREADS;
-    SCMX_REQUIRE(blocks < (1ll << 31), SCMX_ELIMIT, "kv_append: %lld vectors", (long long)a.vectors);
-    SCMX_PDL_OK("kv_append_kernel", launch_pdl(kern, dim3((unsigned)blocks, 2), dim3(KV_THREADS), 0, (cudaStream_t)stream, a));
+    const int per = KV_THREADS / G * KV_TURNS;
+    SCMX_PDL_OK("kv_append_kernel", launch_pdl(kern, dim3((unsigned)((L + per - 1) / per), (unsigned)(hk < 65535 ? hk : 65535), 2), dim3(KV_THREADS), 0,
+                                               (cudaStream_t)stream, a));
     return SCMX_OK;
 }
 
@@ -163,11 +199,12 @@ extern "C" int scmx_kv_read(const int8_t* k_codes, const float* k_scales, const 
     SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_read: null buffer");
     SCMX_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_read: buffers must be 16-byte aligned");
     KvReadArgs a;
-    a.codes[0] = k_codes; a.codes[1] = v_codes; a.scales[0] = k_scales; a.scales[1] = v_scales; a.out[0] = k; a.out[1] = v;
-    a.start = start; a.cap = capacity; a.n = n; a.per = d / 8; a.pieces = (int64_t)hk * n * a.per;
-    const int64_t blocks = (a.pieces + KV_THREADS - 1) / KV_THREADS;
-    SCMX_REQUIRE(blocks < (1ll << 31), SCMX_ELIMIT, "kv_read: %lld rows of %d heads", (long long)n, hk);
-    SCMX_PDL_OK("kv_read_kernel", launch_pdl(kv_read_kernel, dim3((unsigned)blocks, 2), dim3(KV_THREADS), 0, (cudaStream_t)stream, a));
+    a.kc = k_codes; a.vc = v_codes; a.ks = k_scales; a.vs = v_scales; a.k = k; a.v = v;
+    a.start = start; a.cap = capacity; a.n = n; a.hk = hk; a.d = d; a.pieces = d / 16; a.rows = KV_THREADS / a.pieces;
+    const int64_t blocks = (n + a.rows * KV_TURNS - 1) / (a.rows * KV_TURNS);
+    SCMX_REQUIRE(blocks < (1ll << 31), SCMX_ELIMIT, "kv_read: %lld rows", (long long)n);
+    SCMX_PDL_OK("kv_read_kernel", launch_pdl(kv_read_kernel, dim3((unsigned)blocks, (unsigned)(hk < 65535 ? hk : 65535), 2), dim3(KV_THREADS), 0,
+                                             (cudaStream_t)stream, a));
     return SCMX_OK;
 }
 

@@ -118,21 +118,32 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     const uint32_t ring_s = smem_u32(ring);
     const int nkeys = (int)(t1 - t0), nblocks = (nkeys + CA_KEYS - 1) / CA_KEYS, ntail = (int)(pos - t0 < nkeys ? pos - t0 : nkeys);      // keys from ntail on are new rows (negative: from before t0)
 
-    // copies of block b: pieces lane, lane + 32, .. of 16 bytes; a warp covers whole vectors with each
-    constexpr int COPIES = CA_KEYS * PIECES / 32, RSTEP = 32 / PIECES;
-    const int lr0 = lane / PIECES, lc0 = lane % PIECES;
+    // copies of block b: pieces lane, lane + 32, .. of 16 bytes; a warp covers whole vectors with each, whose places repeat after DIST
+    constexpr int COPIES = CA_KEYS * PIECES / 32, RSTEP = 32 / PIECES, DIST = RSTEP >= 8 ? 1 : 8 / RSTEP;
+    const int lr0 = lane / PIECES;
+    int at[DIST];
+#pragma unroll
+    for (int p = 0; p < DIST; ++p) at[p] = ca_at<ROW>(lr0 + p * RSTEP, lane % PIECES);
     auto load = [&](int b, int stage) {
         if (b < nblocks) {
             const uint32_t dst = ring_s + stage * L::STAGE;
             const int left = nkeys - b * CA_KEYS;
-            const int64_t src = (int64_t)b * L::BLOCK + lane * 16;
+            const unsigned char *ksrc = kb + (int64_t)b * L::BLOCK + lane * 16, *vsrc = vb + (int64_t)b * L::BLOCK + lane * 16;
+            if (left >= CA_KEYS) {
 #pragma unroll
-            for (int p = 0; p < COPIES; ++p) {
-                const int r = lr0 + p * RSTEP, at = ca_at<ROW>(r, lc0);
-                const bool on = r < left;
-                const int64_t off = on ? src + p * 512 : 0;
-                cp_async16(dst + at, kb + off, on);
-                cp_async16(dst + L::BLOCK + at, vb + off, on);
+                for (int p = 0; p < COPIES; ++p) {
+                    const uint32_t to = dst + at[p % DIST] + p / DIST * (DIST * RSTEP * ROW);
+                    cp_async16(to, ksrc + p * 512, true);
+                    cp_async16(to + L::BLOCK, vsrc + p * 512, true);
+                }
+            } else {
+#pragma unroll
+                for (int p = 0; p < COPIES; ++p) {
+                    const uint32_t to = dst + at[p % DIST] + p / DIST * (DIST * RSTEP * ROW);
+                    const bool on = lr0 + p * RSTEP < left;
+                    cp_async16(to, on ? ksrc + p * 512 : kb, on);
+                    cp_async16(to + L::BLOCK, on ? vsrc + p * 512 : vb, on);
+                }
             }
             if constexpr (I8) {
                 const bool on = (lane & 15) < left;
@@ -150,7 +161,10 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
         const int r = row0 + 8 * nt + g, tok = r / G;
         if (r >= R) return make_uint2(0, 0);
         const uint16_t* qp = a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 16 * s;
-        if constexpr (I8) return *reinterpret_cast<const uint2*>(qp + 4 * t4);       // the four values that one word of codes holds
+        if constexpr (I8) {      // the four values that one word of codes holds: 0 and 2, 1 and 3
+            const uint2 w = *reinterpret_cast<const uint2*>(qp + 4 * t4);
+            return make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632));
+        }
         return make_uint2(*reinterpret_cast<const uint32_t*>(qp + 2 * t4), *reinterpret_cast<const uint32_t*>(qp + 8 + 2 * t4));
     };
     uint2 qf[L::QREGS ? NT : 1][L::QREGS ? KSTEPS : 1];
@@ -180,6 +194,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.0f;
     }
 
+    const I8Pairs i8;
     const int lr = lane & 7, lm = lane >> 3;            // row of a matrix load, and which of its four matrices
     int stage = 0;
     for (int b = warp; b < nblocks; b += WARPS) {
@@ -208,8 +223,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
                 ldsm4(kst + ca_at<ROW>(lr + 8 * (lm & 1), c + (lm >> 1)), w);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t f[4] = {i8x2_bf16(__byte_perm(w[2 * e], 0, 0x4140)), i8x2_bf16(__byte_perm(w[2 * e + 1], 0, 0x4140)),
-                                           i8x2_bf16(__byte_perm(w[2 * e], 0, 0x4342)), i8x2_bf16(__byte_perm(w[2 * e + 1], 0, 0x4342))};
+                    const uint32_t f[4] = {i8.even(w[2 * e]), i8.even(w[2 * e + 1]), i8.odd(w[2 * e]), i8.odd(w[2 * e + 1])};
                     scores(c + e, f);
                 }
             }
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) grow = grow || fmaxf(s[nt][e], s[nt][2 + e]) > mx[nt][e] + CA_GROWTH;
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[nt][e], s[nt][2 + e]) > mx[nt][e] + CA_GROWTH;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -341,17 +355,14 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             }
         } else if constexpr (I8) {
 #pragma unroll
-            for (int cg = 0; cg < D / 32; ++cg) {       // 32 values: a thread's word holds values 4 g .. of its four keys
+            for (int i = 0; i < MT; i += 2) {           // pairs of values as 16-bit units: keys 0-7, 8-15 of piece i, the same of piece i + 1
                 uint32_t w[4];
+                ldsm4_t(vst + ca_at<ROW>(lr + 8 * (lm & 1), i + (lm >> 1)), w);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    w[r] = *reinterpret_cast<const uint32_t*>(blk + L::BLOCK + ca_at<ROW>(2 * t4 + (r & 1) + 8 * (r >> 1), 2 * cg + (g >> 2)) + 4 * (g & 3));
+                for (int e = 0; e < 2; ++e) {           // operand rows g and g + 8: values 2 g and 2 g + 1 of the piece
+                    const uint32_t f[4] = {i8.even(w[2 * e]), i8.odd(w[2 * e]), i8.even(w[2 * e + 1]), i8.odd(w[2 * e + 1])};
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {           // operand rows g and g + 8: values 4 g + 2 j and 4 g + 2 j + 1
-                    const uint32_t f[4] = {i8x2_bf16(__byte_perm(w[0], w[1], 0x4400 + 2 * j * 0x1111)), i8x2_bf16(__byte_perm(w[0], w[1], 0x4400 + (2 * j + 1) * 0x1111)),
-                                           i8x2_bf16(__byte_perm(w[2], w[3], 0x4400 + 2 * j * 0x1111)), i8x2_bf16(__byte_perm(w[2], w[3], 0x4400 + (2 * j + 1) * 0x1111))};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[2 * cg + j][nt], f, pb[nt][0], pb[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[i + e][nt], f, pb[nt][0], pb[nt][1]);
                 }
             }
         } else {
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) r[I8 ? 32 * (i >> 1) + 4 * g + 2 * (i & 1) + h : 16 * i + 8 * h + g] = o[i][nt][2 * h + e];
+                for (int h = 0; h < 2; ++h) r[I8 ? 16 * i + 2 * g + h : 16 * i + 8 * h + g] = o[i][nt][2 * h + e];
             if (g == 0) {
                 r[D] = mx[nt][e];
                 r[D + 1] = l;

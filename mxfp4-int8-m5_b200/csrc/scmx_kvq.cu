@@ -76,6 +76,7 @@ struct KvReadArgs {
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvReadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
+    const I8Pairs i8;
     const bool val = blockIdx.z != 0;
     const int r = threadIdx.x / a.pieces, l = threadIdx.x - r * a.pieces;
     if (r >= a.rows) return;
@@ -102,9 +103,9 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
             uint32_t o[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t lo = i8x2_bf16(__byte_perm(u[j], 0, 0x4140)), hi = i8x2_bf16(__byte_perm(u[j], 0, 0x4342));
-                o[2 * j] = pack_bf16x2(__fmul_rn(bf16_lo(lo), s[i]), __fmul_rn(bf16_hi(lo), s[i]));
-                o[2 * j + 1] = pack_bf16x2(__fmul_rn(bf16_lo(hi), s[i]), __fmul_rn(bf16_hi(hi), s[i]));
+                const uint32_t even = i8.even(u[j]), odd = i8.odd(u[j]);
+                o[2 * j] = pack_bf16x2(__fmul_rn(bf16_lo(even), s[i]), __fmul_rn(bf16_lo(odd), s[i]));
+                o[2 * j + 1] = pack_bf16x2(__fmul_rn(bf16_hi(even), s[i]), __fmul_rn(bf16_hi(odd), s[i]));
             }
             uint4* p = reinterpret_cast<uint4*>(out + row * a.d);
             p[0] = make_uint4(o[0], o[1], o[2], o[3]);

@@ -126,7 +126,7 @@ SIGNATURES = {
     "scmx_kv_keep": [ctypes.POINTER(ScmxKvLayer), c_int, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp],
     "scmx_cache_attn_scratch": [c_i64, c_int, c_int, c_int, c_int],
     "scmx_cache_attn": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_float, c_vp, c_vp, c_i64,
-                        c_vp],
+                        c_vp, c_vp],
     "scmx_verify_scratch": [c_int, c_i64],
     "scmx_verify": [c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_float, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
     "scmx_gemv_pro": [c_vp, c_int, c_vp, c_float, c_vp, c_vp, c_vp, c_i64, c_i64, _FMT_P, c_int, c_vp, c_vp, c_int, c_int, c_int,
@@ -340,6 +340,9 @@ def _raise_status(st):
 _GEMM_ROLES = {51: "latent attention producer waiting for a free key tile", 52: "latent attention producer waiting for a free value tile",
                53: "latent attention MMA thread waiting for operands", 54: "latent attention MMA thread waiting for softmax weights",
                55: "latent attention softmax warp waiting for scores", 56: "latent attention softmax warp waiting for the last product",
+               71: "cache attention producer waiting for a free tile", 72: "cache attention MMA warp waiting for operands",
+               73: "cache attention MMA warp waiting for weights", 74: "cache attention softmax warp waiting for scores or values",
+               75: "cache attention softmax warp waiting for the last product", 76: "cache attention converting warp waiting for a tile",
                61: "delta producer waiting for a free stage", 62: "delta MMA thread waiting for operands",
                63: "delta MMA thread waiting for states or corrections", 64: "delta warp waiting for a product",
                41: "retention chunk product waiting for operands", 42: "retention chunk kernel waiting for the product",
@@ -357,7 +360,7 @@ _STEP_ROWS = ("input row", "q|k|v row", "attention output", "residual row after 
 
 
 def describe_status(code):
-    """Text for a status-word code: 1..6 GEMM roles, 11 / 12 streaming GEMV, 20 peer barrier, 31..64 kernels of the sequence mixers,
+    """Text for a status-word code: 1..6 GEMM roles, 11 / 12 streaming GEMV, 20 peer barrier, 31..64 kernels of the sequence mixers, 71..76 attention to a cache,
     1000 + 5 layer + k row k of a layer of the one-kernel decode step."""
     if code >= 1000:
         return f"decode step: layer {(code - 1000) // 5} waiting for its {_STEP_ROWS[(code - 1000) % 5]}"

@@ -2,53 +2,23 @@
 // keys and values:  o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max),  j over the positions before `pos` and those
 // of the new rows that row i's mask names.
 //
-// The G query heads of a key/value head and the n rows are G n query rows that read the same keys: they meet the cache in one pass, up to 32 of
-// them in a CTA.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16, bfloat16, float32 sums): keys
+// The G query heads of a key/value head and the n rows are G n query rows that read the same keys: they meet the cache in one pass.  Up to
+// 16 of them run here, more on tcgen05 (scmx_cache_attn_tc.cu).  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16, bfloat16, float32 sums): keys
 // and values are the 16-row operand, query rows come eight at a time, so one row costs eight and an INT8 code is converted once for
 // all rows.  The positions are cut into ranges, one CTA each; in a CTA every warp takes blocks of 16 positions of its own, brought into its own ring
 // in shared memory by asynchronous copies, and keeps a running maximum, sum and output in registers.  The maximum is only raised when a
 // score exceeds it by 2^8, so that most blocks neither exchange nor rescale anything.  The warps' states are joined in shared memory, the
 // ranges' by a second launch.
 // INT8 codes become bfloat16 exactly (8 significant bits); a position's key scale multiplies its scores, its value scale its weights.
-#include "scmx_common.cuh"
-#include "scmx_ptx.cuh"
+#include "scmx_cache_attn.cuh"
 
 namespace scmx {
-
-constexpr int CA_KEYS = 16;             // positions of a block
-constexpr int CA_MAX_ROWS = 64;
-constexpr float CA_LOG2E = 1.4426950408889634f;
-constexpr float CA_GROWTH = 8.0f;      // log2 of how far a weight may exceed one before the maximum is raised
-
-struct CaArgs {
-    const uint16_t* q;               // bf16, heads q_hs and rows q_rs elements apart
-    const void *k, *v;               // [hk, cap, d] bf16 or int8
-    const float *ks, *vs;            // [hk, cap] (INT8)
-    const int64_t* mask;             // [n] or null: row i sees rows 0 .. i
-    const int32_t* pos_dev;
-    float* part;                     // [hk, tiles, nsplit, rows of a tile, D + 2] or null (nsplit 1)
-    uint16_t* out;                   // bf16 [n, hq d]
-    int64_t q_hs, q_rs, pos, cap;
-    int n, hq, hk, nsplit;
-    float scale;                     // times log2(e)
-};
-
-// Positions of a call and of one range: ranges are whole blocks and no shorter than four, so a short cache uses the first few only.
-__device__ __forceinline__ int64_t ca_pos(const int32_t* pos_dev, int64_t pos, int64_t cap, int n) {
-    int64_t p = pos_dev ? (int64_t)pos_dev[0] : pos;
-    return p < 0 ? 0 : p > cap - n ? cap - n : p;
-}
-constexpr int CA_MIN_RANGE = 4 * CA_KEYS;
-__device__ __forceinline__ int64_t ca_chunk(int64_t T, int nsplit) {
-    const int64_t c = (T + nsplit - 1) / nsplit;
-    return c < CA_MIN_RANGE ? CA_MIN_RANGE : (c + CA_KEYS - 1) / CA_KEYS * CA_KEYS;
-}
 
 // NT: groups of eight query rows.  Warps: what registers and shared memory allow; INT8 needs more of them, its conversions are latency.
 template <int D, bool I8, int NT>
 struct CaShape {
     static constexpr int ROWS = 8 * NT;
-    static constexpr int WARPS = !I8 ? 8 : NT == 1 ? 16 : NT == 2 ? 12 : 8;
+    static constexpr int WARPS = !I8 ? 8 : NT == 1 ? 16 : 12;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROW = I8 ? D : 2 * D;                        // bytes of a vector
     static constexpr int BLOCK = CA_KEYS * ROW;                       // 16 keys or values
@@ -57,9 +27,7 @@ struct CaShape {
     static constexpr int RING = STAGE * STAGES;
     static constexpr int STATE = ROWS * (D + 2) * 4;                  // a warp's state when the warps are joined
     static constexpr int WARP = ((RING > STATE ? RING : STATE) + 127) / 128 * 128;
-    static constexpr bool QREGS = NT < 4;                             // queries in registers, or in shared memory
-    static constexpr int QBYTES = QREGS ? 0 : NT * (D / 16) * 32 * 8;
-    static constexpr int TOTAL = WARP * WARPS + QBYTES;
+    static constexpr int TOTAL = WARP * WARPS;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -109,7 +77,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * L::ROWS;
-    const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit);
+    const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
     const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
     if (t0 >= T) return;
     const unsigned char* kb = static_cast<const unsigned char*>(a.k) + ((int64_t)kvh * a.cap + t0) * ROW;
@@ -167,17 +135,11 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
         }
         return make_uint2(*reinterpret_cast<const uint32_t*>(qp + 2 * t4), *reinterpret_cast<const uint32_t*>(qp + 8 + 2 * t4));
     };
-    uint2 qf[L::QREGS ? NT : 1][L::QREGS ? KSTEPS : 1];
-    uint2* qs = reinterpret_cast<uint2*>(smem_raw + L::WARP * WARPS);
-    if constexpr (L::QREGS) {
+    uint2 qf[NT][KSTEPS];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int s = 0; s < KSTEPS; ++s) qf[nt][s] = query(nt, s);
-    } else {
-        for (int i = warp; i < NT * KSTEPS; i += WARPS) qs[i * 32 + lane] = query(i / KSTEPS, i % KSTEPS);
-        __syncthreads();
-    }
+        for (int s = 0; s < KSTEPS; ++s) qf[nt][s] = query(nt, s);
 
     // rows 2 t4 and 2 t4 + 1 of each group: maximum and sum; output: 16 values of the vectors times eight rows
     float o[MT][NT][4], mx[NT][2], sum[NT][2];
@@ -211,10 +173,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             for (int j = 0; j < 4; ++j) s[nt][j] = 0.0f;
         auto scores = [&](int c, const uint32_t (&w)[4]) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint2 q = L::QREGS ? qf[L::QREGS ? nt : 0][L::QREGS ? c : 0] : qs[(nt * KSTEPS + c) * 32 + lane];
-                mma_bf16(s[nt], w, q.x, q.y);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma_bf16(s[nt], w, qf[nt][c].x, qf[nt][c].y);
         };
         if constexpr (I8) {
 #pragma unroll
@@ -435,7 +394,7 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
     const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (i >= a.hk * R) return;
     const int kvh = i / R, r = i - kvh * R, tile = r / rows;
-    const int64_t T = ca_pos(a.pos_dev, a.pos, a.cap, a.n) + a.n, chunk = ca_chunk(T, a.nsplit);
+    const int64_t T = ca_pos(a.pos_dev, a.pos, a.cap, a.n) + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
     const int active = (int)((T + chunk - 1) / chunk), stride = rows * (D + 2);
     const float* x = a.part + ((int64_t)kvh * tiles + tile) * a.nsplit * stride + (r - tile * rows) * (D + 2);
     constexpr int E = D / 32;
@@ -474,15 +433,25 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(o + e) = l == 0.0f ? 0u : pack_bf16x2(v[e] / l, v[e + 1] / l);
 }
 
-// How a call is cut: groups of eight query rows in a CTA, tiles of them, ranges of positions (as many CTAs as multiprocessors).
-struct CaPlan { int nt, tiles, nsplit; };
 static CaPlan ca_plan(int64_t positions, int R, int hk) {
     CaPlan p;
-    p.nt = R <= 8 ? 1 : R <= 16 ? 2 : 4;
-    p.tiles = (R + 8 * p.nt - 1) / (8 * p.nt);
-    const int64_t most = (positions + CA_MIN_RANGE - 1) / CA_MIN_RANGE, want = sm_count() / ((int64_t)hk * p.tiles);
+    p.tc = R > 16;
+    if (p.tc) {
+        p.nt = R > 128 ? 2 : 1;
+        p.copies = R <= 32 ? 4 : R <= 64 ? 2 : 1;
+        p.rows = 128 * p.nt / p.copies;
+        p.unit = 128;
+    } else {
+        p.nt = R <= 8 ? 1 : 2;
+        p.copies = 1;
+        p.rows = 8 * p.nt;
+        p.unit = 4 * CA_KEYS;
+    }
+    p.tiles = (R + p.rows - 1) / p.rows;
+    const int64_t most = (positions + p.unit - 1) / p.unit, want = sm_count() / ((int64_t)hk * p.tiles);
     const int64_t s = want < most ? want : most;
     p.nsplit = s < 1 ? 1 : (int)s;
+    if (!p.tc && positions > (int64_t)p.nsplit * p.unit) p.unit = CA_KEYS;      // long enough: ranges end at any block
     return p;
 }
 
@@ -498,15 +467,11 @@ static int launch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
     }
     SCMX_PDL_OK("cache_attn_kernel", launch_pdl(cache_attn_kernel<D, I8, NT>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles), dim3(L::THREADS),
                                                 (size_t)L::TOTAL, st, a));
-    if (a.part != nullptr)
-        SCMX_PDL_OK("cache_attn_join_kernel", launch_pdl(cache_attn_join_kernel<D>, dim3((unsigned)((a.hq * a.n + 3) / 4)), dim3(128), 0, st, a, p.tiles, L::ROWS));
     return SCMX_OK;
 }
 template <int D, bool I8>
-static int dispatch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
-    return p.nt == 1 ? launch_ca<D, I8, 1>(a, p, st) : p.nt == 2 ? launch_ca<D, I8, 2>(a, p, st) : launch_ca<D, I8, 4>(a, p, st);
-}
-static int64_t ca_scratch(const CaPlan& p, int hk, int d) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * 8 * p.nt * (d + 2) * 4; }
+static int dispatch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) { return p.nt == 1 ? launch_ca<D, I8, 1>(a, p, st) : launch_ca<D, I8, 2>(a, p, st); }
+static int64_t ca_scratch(const CaPlan& p, int hk, int d) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * p.rows * (d + 2) * 4; }
 
 }  // namespace scmx
 
@@ -519,24 +484,29 @@ extern "C" int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int
 
 extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,
                                const float* v_scales, int int8, const int64_t* mask, int n, int64_t pos, const int32_t* pos_dev, int64_t capacity, int hq, int hk,
-                               int d, float scale, uint16_t* out, void* scratch, int64_t scratch_bytes, void* stream) {
-    SCMX_REQUIRE(q && k && v && out && (!int8 || (k_scales && v_scales)), SCMX_EINVAL, "cache_attn: null buffer");
+                               int d, float scale, uint16_t* out, void* scratch, int64_t scratch_bytes, int32_t* status, void* stream) {
+    SCMX_REQUIRE(q && k && v && out && status && (!int8 || (k_scales && v_scales)), SCMX_EINVAL, "cache_attn: null buffer");
     SCMX_REQUIRE(n >= 1 && n <= CA_MAX_ROWS, SCMX_ELIMIT, "cache_attn: %d rows (1 .. %d)", n, CA_MAX_ROWS);
     SCMX_REQUIRE(d == 64 || d == 128, SCMX_EINVAL, "cache_attn: head size %d (64 or 128)", d);
     SCMX_REQUIRE(hk > 0 && hq > 0 && hq % hk == 0, SCMX_EINVAL, "cache_attn: hq=%d hk=%d", hq, hk);
     SCMX_REQUIRE(capacity >= n && (pos_dev != nullptr || (pos >= 0 && pos + n <= capacity)), SCMX_EINVAL, "cache_attn: rows %lld .. %lld of a cache of %lld",
                  (long long)pos, (long long)(pos + n), (long long)capacity);
     SCMX_REQUIRE(q_head_stride % 4 == 0 && q_row_stride % 4 == 0 && ((uintptr_t)q & 7) == 0 && ((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 &&
-                     ((uintptr_t)out & 3) == 0, SCMX_EINVAL, "cache_attn: query rows must be 8-byte and caches 16-byte aligned");
+                     ((uintptr_t)out & 15) == 0, SCMX_EINVAL, "cache_attn: query rows must be 8-byte, caches and the output 16-byte aligned");
     CaArgs a;
     const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk);
-    a.nsplit = p.nsplit;
+    a.nsplit = p.nsplit; a.unit = p.unit;
     const int64_t need = ca_scratch(p, hk, d);
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",
                  (long long)scratch_bytes, (long long)need);
     a.q = q; a.q_hs = q_head_stride; a.q_rs = q_row_stride; a.k = k; a.v = v; a.ks = k_scales; a.vs = v_scales; a.mask = mask; a.pos_dev = pos_dev; a.pos = pos;
     a.part = need ? static_cast<float*>(scratch) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.scale = scale * CA_LOG2E;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (d == 128) return int8 ? dispatch_ca<128, true>(a, p, st) : dispatch_ca<128, false>(a, p, st);
-    return int8 ? dispatch_ca<64, true>(a, p, st) : dispatch_ca<64, false>(a, p, st);
+    int rc = p.tc ? cache_attn_tc(a, p, d, int8, status, st)
+             : d == 128 ? (int8 ? dispatch_ca<128, true>(a, p, st) : dispatch_ca<128, false>(a, p, st))
+                        : (int8 ? dispatch_ca<64, true>(a, p, st) : dispatch_ca<64, false>(a, p, st));
+    if (rc != SCMX_OK || a.part == nullptr) return rc;
+    void (*join)(CaArgs, int, int) = d == 128 ? cache_attn_join_kernel<128> : cache_attn_join_kernel<64>;
+    SCMX_PDL_OK("cache_attn_join_kernel", launch_pdl(join, dim3((unsigned)((hq * n + 3) / 4)), dim3(128), 0, st, a, p.tiles, p.rows));
+    return SCMX_OK;
 }

@@ -1,0 +1,531 @@
+// Attention of more than 16 query rows (drafted rows times the query heads of a key/value head) to a cache, on tcgen05.  The formula, the cut into
+// ranges of positions and the join of the ranges are those of scmx_cache_attn.cu; here a CTA takes 128 or 256 query rows.
+//
+// Two streams share the tensor core: while it works for one, the other's softmax runs.  With one query tile of 128 rows the streams take the
+// key tiles (128 positions) in turn and are joined at the end; with two, each stream has a query tile of its own.  A `unit` is a stream's work
+// on one key tile: S = Q K^T (128 x 128, float32 in tensor memory), softmax, O += P V with P (bfloat16) read from tensor memory, where it
+// overwrites S.
+//   warp 0        TMA producer of key and value tiles
+//   warp 1        all MMAs (the warp stays converged, one lane issues)
+//   warps 2-9     two softmax warpgroups, one per stream, a thread per lane of tensor memory.  The maximum is raised when it has grown by
+//                 more than 2^8
+//   warps 10-13   (INT8) codes of a tile to bfloat16 operands, exactly; a position's key scale multiplies its scores, its value scale its
+//                 weights.  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are laid
+//                 out alike, and outputs put back
+// Up to 64 query rows leave lanes idle: a tile then holds two or four copies of them, each copy's threads take a half or a quarter of a tile's
+// keys, and their weights for the other keys are zero.  The copies are joined like the streams.  So the softmax of few rows is spread over all
+// threads, and the products, which a memory-bound call has time for, stay whole tiles.
+// New rows' values that are not finite must not reach rows that do not see them (0 x inf): the threads of a tile that holds new rows clear them
+// in shared memory, with the rows behind the last position, and add them at the end to the rows that see them.
+// Every mbarrier wait is bounded (status word codes 71..76).
+#include "mixers/mix_tc.cuh"
+#include "scmx_cache_attn.cuh"
+
+namespace scmx {
+
+constexpr int CT_TILE = 128 * 128;        // bytes of a [128 rows x 64 bfloat16] or [128 x 128 INT8] block
+constexpr int CT_SCALES = 4;              // tiles whose scales are held
+
+template <int D, bool I8, int MQ>
+struct CtSmem {
+    static constexpr int KB = D / 64;
+    static constexpr int KS = D == 64 ? (I8 ? 2 : 4) : I8 ? (MQ == 2 ? 1 : 2) : (MQ == 2 ? 2 : 3);       // stages of key operands
+    static constexpr int VS = KS;
+    static constexpr int NS = !I8 ? 0 : D == 64 ? 6 : MQ == 2 ? 5 : 3;                                    // stages of INT8 tiles
+    static constexpr int Q_OFF = 0;
+    static constexpr int K_OFF = Q_OFF + MQ * KB * CT_TILE;
+    static constexpr int V_OFF = K_OFF + KS * KB * CT_TILE;
+    static constexpr int C_OFF = V_OFF + VS * KB * CT_TILE;
+    static constexpr int SC_OFF = C_OFF + NS * CT_TILE;                       // scales: [CT_SCALES][keys, values][128] float
+    static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
+    // kfull, kempty [KS], vfull, vempty [VS], codes full, empty [NS], scales [CT_SCALES], S, P, O [2]
+    static constexpr int NBAR = 2 * KS + 2 * VS + 2 * NS + (I8 ? CT_SCALES : 0) + 6;
+    static constexpr int MISC_OFF = BAR_OFF + 8 * NBAR;
+    static constexpr int TOTAL = MISC_OFF + 32 + 1024;
+    static constexpr int ML_OFF = K_OFF + 256 * (D + 1) * 4;                  // outputs of 256 lanes from K_OFF on, then their maxima and sums, in place of operands
+    static_assert(MQ == 2 || ML_OFF + 2048 <= SC_OFF, "joined outputs fit the operands' memory");
+    static_assert(TOTAL <= 232448, "shared memory of an SM");
+};
+
+// 16 registers of a thread -> 16 consecutive 32-bit columns of its lane.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Bits of 32 keys, the first `b` positions after the first new row (negative: before it), that a row with these bits sees.
+__device__ __forceinline__ uint32_t ct_seen(uint64_t bits, int b) {
+    if (b <= -32) return 0xFFFFFFFFu;
+    if (b < 0) return (uint32_t)(bits << -b) | ((1u << -b) - 1u);
+    return b < 64 ? (uint32_t)(bits >> b) : 0u;
+}
+
+// MQ: query tiles; COPIES of the rows in a tile (1 with two tiles).
+template <int D, bool I8, int MQ, int COPIES>
+__global__ void __launch_bounds__(I8 ? 448 : 320, 1)
+    cache_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CaArgs a, int32_t* status,
+                         uint64_t wait_ns) {
+    using L = CtSmem<D, I8, MQ>;
+    constexpr int KB = L::KB, KS = L::KS, VS = L::VS, NS = L::NS, THREADS = I8 ? 448 : 320;
+    constexpr int RP = 128 / COPIES, ROWS = MQ * RP, NCH = 4 / COPIES;      // rows of a tile, of the CTA; 32-key pieces of a thread
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem), bars = sbase + L::BAR_OFF;
+    const uint32_t b_kf = bars, b_ke = b_kf + 8 * KS, b_vf = b_ke + 8 * KS, b_ve = b_vf + 8 * VS, b_cf = b_ve + 8 * VS, b_ce = b_cf + 8 * NS, b_sc = b_ce + 8 * NS,
+                   b_s = b_sc + (I8 ? 8 * CT_SCALES : 0), b_p = b_s + 16, b_o = b_p + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
+    uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF + 8);      // new rows with values that are not finite
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, tid = threadIdx.x;
+
+    if (tid == 0) {
+        prefetch_map(&tmK);
+        prefetch_map(&tmV);
+        for (int i = 0; i < L::NBAR; ++i) {
+            const uint32_t b = bars + 8 * i;
+            const bool weights = b == b_p || b == b_p + 8;                                                        // one arrival per softmax warp
+            const bool converted = I8 && ((b >= b_kf && b < b_ke) || (b >= b_vf && b < b_ve) || (b >= b_ce && b < b_s));      // one per converting warp
+            mbar_init(b, weights || converted ? 4 : 1);
+        }
+        *abort_flag = 0;
+        bad[0] = bad[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * ROWS;
+    const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
+    const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
+    const int nkeys = t1 > t0 ? (int)(t1 - t0) : 0, ntiles = (nkeys + 127) / 128, units = ntiles * MQ;
+    const int dnew = (int)(t0 - pos > -(int64_t)nkeys - 64 ? t0 - pos : -(int64_t)nkeys - 64);      // the range's first key, counted from the first new row
+
+    // queries: K-major tiles with the 128-byte swizzle; a negative scale is taken by the queries
+    if (ntiles) {
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        for (int i = tid; i < MQ * 128 * (D / 8); i += THREADS) {
+            const int c = i % (D / 8), l = i / (D / 8), r = row0 + l / 128 * RP + l % 128 % RP, tok = r / G;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (r < R) {
+                const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 8 * c);
+                const uint2 x = p[0], y = p[1];
+                if constexpr (I8) w = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x5410), __byte_perm(y.x, y.y, 0x7632));
+                else w = make_uint4(x.x, x.y, y.x, y.y);
+                w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+            }
+            *reinterpret_cast<uint4*>(smem + L::Q_OFF + (l / 128 * KB + c / 8) * CT_TILE + l % 128 * 128 + (((c & 7) ^ (l & 7)) << 4)) = w;
+        }
+        proxy_fence();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    int fail = 0;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int j = 0; j < ntiles; ++j) {
+                const int key = (int)t0 + 128 * j;
+                if constexpr (I8) {
+                    bool ok = true;
+                    for (int h = 0; h < 2 && ok; ++h) {
+                        const int i = 2 * j + h, s = i % NS;
+                        if (int w = mbar_wait(b_ce + 8 * s, ((i / NS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; ok = false; break; }
+                        mbar_expect_tx(b_cf + 8 * s, CT_TILE);
+                        tma_load_3d(sbase + L::C_OFF + s * CT_TILE, h ? &tmV : &tmK, 0, key, kvh, b_cf + 8 * s);
+                    }
+                    if (!ok) break;
+                } else {
+                    const int ks = j % KS, vs = j % VS;
+                    if (int w = mbar_wait(b_ke + 8 * ks, ((j / KS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
+                    mbar_expect_tx(b_kf + 8 * ks, KB * CT_TILE);
+                    for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::K_OFF + (ks * KB + c) * CT_TILE, &tmK, c * 128, key, kvh, b_kf + 8 * ks);
+                    if (int w = mbar_wait(b_ve + 8 * vs, ((j / VS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
+                    mbar_expect_tx(b_vf + 8 * vs, KB * CT_TILE);
+                    for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::V_OFF + (vs * KB + c) * CT_TILE, &tmV, c * 128, key, kvh, b_vf + 8 * vs);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t on = elect_lane();
+        const uint32_t idesc_s = umma_idesc_bf16(128, 128), idesc_o = umma_idesc_bf16(128, D) | IDESC_B_MN;
+        int kt = -1, vt = -1;            // last tiles that were waited for
+        auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+            if (!wait_warp(bar, parity, abort_flag, wait_ns, code, fail)) return false;
+            tc_fence_after();
+            return true;
+        };
+        auto scores = [&](int u) -> bool {
+            const int m = u & 1, j = MQ == 2 ? u >> 1 : u, ks = j % KS;
+            if (j != kt && !wait(b_kf + 8 * ks, (j / KS) & 1, 72)) return false;
+            kt = j;
+            const uint32_t q = sbase + L::Q_OFF + (MQ == 2 ? m * KB : 0) * CT_TILE;
+#pragma unroll
+            for (int c = 0; c < KB; ++c) {
+                const uint64_t da = umma_desc(q + c * CT_TILE), db = umma_desc(sbase + L::K_OFF + (ks * KB + c) * CT_TILE);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_bf16(on, tmem + 128 * m, da + 2 * k, db + 2 * k, idesc_s, c + k > 0);
+            }
+            umma_commit(on, b_s + 8 * m);
+            if (MQ == 1 || m == 1) umma_commit(on, b_ke + 8 * ks);
+            return true;
+        };
+        bool ok = units == 0 || scores(0);
+        if (ok && units > 1) ok = scores(1);
+        for (int u = 0; u < units && ok; ++u) {
+            const int m = u & 1, j = MQ == 2 ? u >> 1 : u, vs = j % VS;
+            if (!(ok = wait(b_p + 8 * m, (u >> 1) & 1, 73))) break;
+            if (j != vt && !(ok = wait(b_vf + 8 * vs, (j / VS) & 1, 72))) break;
+            vt = j;
+            const uint64_t dv = umma_desc_mn(sbase + L::V_OFF + vs * KB * CT_TILE, CT_TILE);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) umma_bf16_ts(on, tmem + 256 + 128 * m, tmem + 128 * m + 8 * k, dv + 128 * k, idesc_o, k > 0 ? 1u : (uint32_t)(u > 1));
+            if (MQ == 1 || m == 1) umma_commit(on, b_ve + 8 * vs);
+            if (u + 2 >= units) umma_commit(on, b_o + 8 * m);
+            else ok = scores(u + 2);
+        }
+        if (!on) fail = fail > 0 ? -1 : fail;      // one lane reports
+    } else if (warp < 10) {
+        const int m = (warp - 2) >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = row / G;
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
+        const int c0 = copy * (128 / COPIES);                   // the thread's first key of a tile
+        uint64_t bits = 0;
+        if (row < R) {
+            bits = a.mask ? (uint64_t)a.mask[tok] : (2ull << tok) - 1ull;
+            if (a.n < 64) bits &= (1ull << a.n) - 1ull;
+        }
+        const float sl = I8 ? 1.0f : fabsf(a.scale);            // scores times this are exponents of 2 (INT8: the key scales have it)
+        float mx = -1e30f, sum = 0.0f;
+        for (int u = m; u < units; u += 2) {
+            const int j = MQ == 2 ? u >> 1 : u, d0 = dnew + 128 * j;
+            const bool tail = d0 + 128 > 0;                     // some keys are new rows, or past the end
+            const float* scales = reinterpret_cast<const float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 256 + c0;
+            int w = mbar_wait(b_s + 8 * m, (u >> 1) & 1, abort_flag, wait_ns);
+            if (I8 && !w) w = mbar_wait(b_sc + 8 * (j & (CT_SCALES - 1)), (j / CT_SCALES) & 1, abort_flag, wait_ns);
+            if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 74 : -1; break; }
+            tc_fence_after();
+            // scores of piece c: 32 keys, as exponents of 2 once multiplied by sl; unseen ones -inf
+            auto finish = [&](uint32_t (&v)[32], int c) {
+                if constexpr (I8) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(scales + 32 * c + i);
+                        v[i] = __float_as_uint(__uint_as_float(v[i]) * f.x);
+                        v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * f.y);
+                        v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) * f.z);
+                        v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) * f.w);
+                    }
+                }
+                if (tail) {
+                    const uint32_t seen = ct_seen(bits, d0 + c0 + 32 * c);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1)) v[i] = 0xFF800000u;
+                }
+            };
+            uint32_t r[2][32];
+            float tm = -INFINITY;
+            tmem_ld32(ts + c0, r[0]);
+            tmem_ld_fence(r[0]);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                uint32_t(&v)[32] = r[c & 1];
+                if (c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
+                finish(v, c);
+                float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    m0 = fmaxf(m0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+                    m1 = fmaxf(m1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
+                }
+                tm = fmaxf(tm, fmaxf(m0, m1));
+                if (c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
+            }
+            const bool first = u == m, grow = first || (tm - mx) * sl > CA_GROWTH;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float mn = grow ? fmaxf(mx, tm) : mx, f = ex2_approx((mx - mn) * sl);
+                mx = mn;
+                if (!first) {      // S complete implies the stream's last product complete: MMAs of one thread finish in order
+                    sum *= f;
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * c, v);
+                        tmem_ld_fence(v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st32(to + 32 * c, v);
+                    }
+                }
+            }
+            const float off = -mx * sl;
+            float s0 = 0.0f, s1 = 0.0f;
+            if (NCH > 2) {
+                tmem_ld32(ts + c0, r[0]);
+                tmem_ld_fence(r[0]);
+            }
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                uint32_t(&v)[32] = r[c & 1];
+                if (NCH > 2) {
+                    if (c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
+                    finish(v, c);
+                }
+                const uint32_t seen = tail ? ct_seen(bits, d0 + c0 + 32 * c) : 0xFFFFFFFFu;
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(__uint_as_float(v[i + e]), sl, off));
+                    s0 += x[0] + x[1];
+                    s1 += x[2] + x[3];
+                    if constexpr (I8) {
+                        const float4 f = *reinterpret_cast<const float4*>(scales + 128 + 32 * c + i);
+                        x[0] *= f.x; x[1] *= f.y; x[2] *= f.z; x[3] *= f.w;
+                        if (tail)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (!(seen >> (i + e) & 1)) x[e] = 0.0f;      // its scale may be anything
+                    }
+                    pk[i / 2] = pack_bf16x2(x[0], x[1]);
+                    pk[i / 2 + 1] = pack_bf16x2(x[2], x[3]);
+                }
+                if (NCH > 2 && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
+                tmem_st16(ts + c0 / 2 + 16 * c, pk);
+            }
+            if (COPIES > 1) {            // weights of the other copies' keys
+                uint32_t z[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = 0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c / NCH != copy) tmem_st16(ts + 16 * c, z);
+            }
+            sum += s0 + s1;
+            tmem_st_wait();
+            tc_fence_before();
+            if (!I8 && tail && (MQ == 1 || m == 0)) {      // a thread per position
+                w = mbar_wait(b_vf + 8 * (j % VS), (j / VS) & 1, abort_flag, wait_ns);
+                if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 74 : -1; break; }
+                const int d = d0 + l;
+                if (d >= 0) {
+                    bool odd = false;
+#pragma unroll
+                    for (int c = 0; c < KB; ++c) {
+                        uint4* p = reinterpret_cast<uint4*>(smem + L::V_OFF + (j % VS * KB + c) * CT_TILE + l * 128);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 x = p[i];
+                            uint32_t v[4] = {x.x, x.y, x.z, x.w};
+                            bool any = d >= a.n;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const bool lo = (v[e] & 0x7F80u) == 0x7F80u, hi = (v[e] & 0x7F800000u) == 0x7F800000u;
+                                if (lo || d >= a.n) v[e] &= 0xFFFF0000u;
+                                if (hi || d >= a.n) v[e] &= 0x0000FFFFu;
+                                any |= lo || hi;
+                            }
+                            odd |= any;
+                            if (any) p[i] = make_uint4(v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                    if (odd && d < a.n) atomicOr(bad + (d >> 5), 1u << (d & 31));
+                }
+                proxy_fence();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_p + 8 * m);
+        }
+        // both streams' products are complete before the operands' memory is used again
+        if (fail == 0) {
+            int w = units > 0 ? mbar_wait(b_o, 0, abort_flag, wait_ns) : 0;
+            if (!w && units > 1) w = mbar_wait(b_o + 8, 0, abort_flag, wait_ns);
+            if (__any_sync(0xffffffffu, w)) fail = w == 1 ? 75 : -1;
+            tc_fence_after();
+        }
+        const bool mine = fail == 0 && units > m;
+        float* out = reinterpret_cast<float*>(smem + L::K_OFF);
+        float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
+        // what a value that is not finite adds to a row that sees it
+        auto odd_values = [&](uint64_t see, int d) {
+            float x = 0.0f;
+            for (uint64_t b = see; b; b &= b - 1) {
+                const float v = bf16_to_f32(static_cast<const uint16_t*>(a.v)[((int64_t)kvh * a.cap + pos + (__ffsll((long long)b) - 1)) * D + d]);
+                if ((__float_as_uint(v) & 0x7F800000u) == 0x7F800000u) x += v;
+            }
+            return x;
+        };
+        // a result: value d of a query row, with the maximum and sum of its positions in this range
+        auto put = [&](int rr, int d, float v, float mxl, float total) {
+            if (a.part != nullptr) {
+                float* y = a.part + ((((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS + (rr - row0)) * (D + 2);
+                y[d] = v;
+                if (d == 0) {
+                    y[D] = mxl;
+                    y[D + 1] = total;
+                }
+            } else {
+                const int tk = rr / G;
+                a.out[(int64_t)tk * a.hq * D + (kvh * G + rr - tk * G) * D + d] = f32_to_bf16(total == 0.0f ? 0.0f : v / total);
+            }
+        };
+        auto place = [](int c) { return I8 ? (c & ~3) | ((c & 1) << 1) | ((c >> 1) & 1) : c; };      // the value that a column holds
+        const float mxl = sum == 0.0f ? -INFINITY : mx * sl;
+        if constexpr (MQ == 2) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const uint64_t see = bits & ((uint64_t)bad[1] << 32 | bad[0]);
+            for (int c = 0; c < D / 32 && mine; ++c) {      // a tensor-memory load is the whole warp's
+                uint32_t v[32];
+                tmem_ld32(to + 32 * c, v);
+                tmem_ld_fence(v);
+                if (row < R)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int d = place(32 * c + i);
+                        put(row, d, __uint_as_float(v[i]) + (see ? odd_values(see, d) : 0.0f), mxl, sum);
+                    }
+            }
+        } else {
+            const int slot = 128 * m + l;
+            ml[slot] = mine ? make_float2(mxl, sum) : make_float2(-INFINITY, 0.0f);
+            if (mine)
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(to + 32 * c, v);
+                    tmem_ld_fence(v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) out[slot * (D + 1) + place(32 * c + i)] = __uint_as_float(v[i]);
+                }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
+            for (int i = 128 * m + l; i < RP * D; i += 256) {
+                const int r = i / D, d = i - r * D, rr = row0 + r;
+                if (rr >= R || units == 0) break;
+                float top = -INFINITY, total = 0.0f, v = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 2 * COPIES; ++s) top = fmaxf(top, ml[(s & 1) * 128 + (s >> 1) * RP + r].x);
+#pragma unroll
+                for (int s = 0; s < 2 * COPIES; ++s) {
+                    const int at = (s & 1) * 128 + (s >> 1) * RP + r;
+                    const float2 z = ml[at];
+                    const float f = z.x == -INFINITY ? 0.0f : ex2_approx(z.x - top);
+                    total += z.y * f;
+                    if (f != 0.0f) v += out[at * (D + 1) + d] * f;
+                }
+                if (odd) {
+                    const int tk = rr / G;
+                    const uint64_t b = a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull;
+                    v += odd_values(b & odd, d);
+                }
+                put(rr, d, v, top, total);
+            }
+        }
+    } else if (I8) {
+        // codes to operands: a thread to a position
+        const int r = tid - 320;
+        const I8Pairs i8;
+        const float factor = fabsf(a.scale);
+        constexpr int N = NS ? NS : 1;
+        for (int i = 0; i < 2 * ntiles; ++i) {
+            const int j = i >> 1, s = i % N, st = j % KS;
+            const bool val = i & 1;
+            float ksc = 0.0f, vsc = 0.0f;
+            if (!val && t0 + 128 * j + r < t1) {
+                const int64_t at = (int64_t)kvh * a.cap + t0 + 128 * j + r;
+                ksc = a.ks[at] * factor;
+                vsc = a.vs[at];
+            }
+            int w = mbar_wait(b_cf + 8 * s, (i / N) & 1, abort_flag, wait_ns);
+            if (!w) w = mbar_wait((val ? b_ve : b_ke) + 8 * st, ((j / KS) & 1) ^ 1, abort_flag, wait_ns);
+            if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 76 : -1; break; }
+            const uint8_t* src = smem + L::C_OFF + s * CT_TILE + r * 128;
+            uint8_t* dst = smem + (val ? L::V_OFF : L::K_OFF) + st * KB * CT_TILE + r * 128;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                const uint4 c = *reinterpret_cast<const uint4*>(src + ((x ^ (r & 7)) << 4));
+                const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+                uint32_t o[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[2 * e] = i8.even(u[e]);
+                    o[2 * e + 1] = i8.odd(u[e]);
+                }
+                uint8_t* p = dst + x / 4 * CT_TILE;
+                const int e = 2 * (x & 3);
+                *reinterpret_cast<uint4*>(p + ((e ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(p + (((e + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            if (!val) {
+                float* sc = reinterpret_cast<float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 256 + r;
+                sc[0] = ksc;
+                sc[128] = vsc;
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(b_ce + 8 * s);
+                mbar_arrive((val ? b_vf : b_kf) + 8 * st);
+                if (!val) mbar_arrive(b_sc + 8 * (j & (CT_SCALES - 1)));
+            }
+        }
+    }
+
+    if (fail > 0) {
+        if (atomicCAS(status, 0, fail) == 0) {
+            status[1] = blockIdx.x;
+            status[2] = threadIdx.x;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*abort_flag) {
+        const uint64_t begin = globaltimer_ns();
+        while (globaltimer_ns() - begin < 200000ull) __nanosleep(1000);   // 0.2 ms for outstanding TMA writes
+        __syncthreads();
+    }
+    if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+template <int D, bool I8, int MQ, int COPIES>
+static int launch_ct(const CUtensorMap& k, const CUtensorMap& v, const CaArgs& a, const CaPlan& p, int32_t* status, cudaStream_t st) {
+    using L = CtSmem<D, I8, MQ>;
+    static bool configured[64] = {};
+    const int dev = current_device();
+    SCMX_REQUIRE(dev >= 0, SCMX_ECUDA, "no current CUDA device (ordinal 0..63)");
+    if (!configured[dev]) {
+        SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_tc_kernel<D, I8, MQ, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+        configured[dev] = true;
+    }
+    SCMX_PDL_OK("cache_attn_tc_kernel", launch_pdl(cache_attn_tc_kernel<D, I8, MQ, COPIES>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles),
+                                                   dim3(I8 ? 448 : 320), (size_t)L::TOTAL, st, k, v, a, status, g_wait_limit_ns));
+    return SCMX_OK;
+}
+template <int D, bool I8>
+static int dispatch_ct(const CUtensorMap& k, const CUtensorMap& v, const CaArgs& a, const CaPlan& p, int32_t* status, cudaStream_t st) {
+    if (p.nt == 2) return launch_ct<D, I8, 2, 1>(k, v, a, p, status, st);
+    return p.copies == 4 ? launch_ct<D, I8, 1, 4>(k, v, a, p, status, st) : p.copies == 2 ? launch_ct<D, I8, 1, 2>(k, v, a, p, status, st)
+                                                                                         : launch_ct<D, I8, 1, 1>(k, v, a, p, status, st);
+}
+
+int cache_attn_tc(const CaArgs& a, const CaPlan& p, int d, int int8, int32_t* status, cudaStream_t st) {
+    SCMX_REQUIRE(a.cap < (1ll << 31) - 128, SCMX_ELIMIT, "cache_attn: a cache of %lld positions", (long long)a.cap);
+    CUtensorMap k, v;
+    const int64_t row = int8 ? d : 2 * d;
+    int rc = make_map_planes(&k, a.k, a.hk, a.cap, row, row, row * a.cap, 128);
+    if (!rc) rc = make_map_planes(&v, a.v, a.hk, a.cap, row, row, row * a.cap, 128);
+    if (rc) return rc;
+    if (d == 128) return int8 ? dispatch_ct<128, true>(k, v, a, p, status, st) : dispatch_ct<128, false>(k, v, a, p, status, st);
+    return int8 ? dispatch_ct<64, true>(k, v, a, p, status, st) : dispatch_ct<64, false>(k, v, a, p, status, st);
+}
+
+}  // namespace scmx

@@ -128,5 +128,5 @@ def cache_attention(q, cache, scale, mask=None, pos_dev=None):
     scratch = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None       # this call's own: graphs may be replayed side by side
     _lib.call("scmx_cache_attn", q.data_ptr(), qhs, qrs, cache.k.data_ptr(), cache.v.data_ptr(), cache.ks.data_ptr() if int8 else None,
               cache.vs.data_ptr() if int8 else None, int(int8), _lib.ptr(mask), n, pos, _pos_dev(pos_dev), cap, hq, hk, d, float(scale), out.data_ptr(),
-              _lib.ptr(scratch), size, _lib.stream())
+              _lib.ptr(scratch), size, _lib.status_buffer().data_ptr(), _lib.stream())
     return out

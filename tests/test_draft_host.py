@@ -55,7 +55,7 @@ def test_entry_points_refuse(scmx):
         _refused(scmx, "scmx_kv_keep", (layers, 2, P, n, pos, None, 2, d, 16, 0, None), text)
 
     def attn(q=P, qhs=64, qrs=64, int8=0, ks=None, n=3, pos=0, cap=100, hq=4, hk=2, d=64, scratch=P, size=1 << 20):
-        return (q, qhs, qrs, P, P, ks, ks, int8, None, n, pos, None, cap, hq, hk, d, 1.0, P, scratch, size, None)
+        return (q, qhs, qrs, P, P, ks, ks, int8, None, n, pos, None, cap, hq, hk, d, 1.0, P, scratch, size, P, None)
     for kw, text in ((dict(q=None), "null"), (dict(int8=1), "null"), (dict(n=0), "0 rows"), (dict(n=65), "65 rows"), (dict(d=96), "head size"), (dict(hq=5), "hq=5"),
                      (dict(hk=0), "hk=0"), (dict(pos=98), "rows 98"), (dict(pos=-1), "rows -1"), (dict(cap=2), "rows"), (dict(qhs=66), "aligned"),
                      (dict(q=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(pos=5000, cap=9000, size=8), "scratch"), (dict(pos=5000, cap=9000, scratch=None), "scratch")):

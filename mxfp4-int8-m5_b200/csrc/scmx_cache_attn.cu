@@ -25,7 +25,8 @@ struct CaShape {
     static constexpr int STAGE = 2 * BLOCK + (I8 ? 128 : 0);          // keys, values, their scales
     static constexpr int STAGES = 3;
     static constexpr int RING = STAGE * STAGES;
-    static constexpr int STATE = ROWS * (D + 2) * 4;                  // a warp's state when the warps are joined
+    static constexpr int PITCH = D + 4;                               // a warp's state when the warps are joined: rows of values, then maxima and sums
+    static constexpr int STATE = ROWS * (PITCH + 2) * 4;
     static constexpr int WARP = ((RING > STATE ? RING : STATE) + 127) / 128 * 128;
     static constexpr int TOTAL = WARP * WARPS;
 };
@@ -62,12 +63,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
-__device__ __forceinline__ float ca_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <int D, bool I8, int NT>
 __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_kernel(const __grid_constant__ CaArgs a) {
     using L = CaShape<D, I8, NT>;
@@ -338,7 +333,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     cp_wait<0>();
     __syncwarp();
 
-    // the warps' states, joined
+    // the warps' states, joined: a warp to a row
     float* st = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -347,90 +342,56 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             float l = sum[nt][e];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-            float* r = st + (8 * nt + 2 * t4 + e) * (D + 2);
+            const int r = 8 * nt + 2 * t4 + e;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) r[I8 ? 16 * i + 2 * g + h : 16 * i + 8 * h + g] = o[i][nt][2 * h + e];
-            if (g == 0) {
-                r[D] = mx[nt][e];
-                r[D + 1] = l;
-            }
+                for (int h = 0; h < 2; ++h) st[r * L::PITCH + (I8 ? 16 * i + 2 * g + h : 16 * i + 8 * h + g)] = o[i][nt][2 * h + e];
+            if (g == 0) reinterpret_cast<float2*>(st + L::ROWS * L::PITCH)[r] = make_float2(mx[nt][e], l);
         }
     __syncthreads();
-    const int live = nblocks < WARPS ? nblocks : WARPS;       // warps that had a block
-    for (int i = threadIdx.x; i < L::ROWS * D; i += L::THREADS) {
-        const int r = i / D, d = i - r * D, rr = row0 + r;
-        if (rr >= R) break;
-        const float* x = reinterpret_cast<const float*>(smem_raw) + r * (D + 2);
-        constexpr int STRIDE = L::WARP / 4;
-        float m = -INFINITY, l = 0.0f, v = 0.0f;
-        for (int w = 0; w < live; ++w) m = fmaxf(m, x[w * STRIDE + D]);
-        for (int w = 0; w < live; ++w) {
-            const float f = x[w * STRIDE + D] == -INFINITY ? 0.0f : ca_ex2(x[w * STRIDE + D] - m);
-            l += x[w * STRIDE + D + 1] * f;
-            v += f == 0.0f ? 0.0f : x[w * STRIDE + d] * f;
-        }
-        if (a.part != nullptr) {
-            float* y = a.part + ((((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * L::ROWS + r) * (D + 2);
-            y[d] = v;
-            if (d == 0) {
-                y[D] = m;
-                y[D + 1] = l;
-            }
+    constexpr int E = D / 32;
+    const int live = nblocks < WARPS ? nblocks : WARPS, rows = R - row0 < L::ROWS ? R - row0 : L::ROWS;      // warps that had a block; rows of this tile
+    const float* states = reinterpret_cast<const float*>(smem_raw);
+    for (int r = warp; r < rows; r += WARPS) {
+        const float2 ml = lane < live ? reinterpret_cast<const float2*>(states + lane * (L::WARP / 4) + L::ROWS * L::PITCH)[r] : make_float2(-INFINITY, 0.0f);
+        float m = ml.x, l = ml.y, v[E];
+        ca_join<E, 8>(live, m, l, v, [&](int s, float (&z)[E]) { ca_load<E>(states + s * (L::WARP / 4) + r * L::PITCH + lane * E, z); });
+        if (a.part == nullptr) {
+            ca_output<D>(a, kvh, row0 + r, lane, v, l);
         } else {
-            const int tk = rr / G, hd = kvh * G + rr - tk * G;
-            a.out[(int64_t)tk * a.hq * D + hd * D + d] = f32_to_bf16(l == 0.0f ? 0.0f : v / l);
+            const int64_t at = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * L::ROWS + r;
+            ca_store<E>(a.part + at * D + lane * E, v);
+            if (lane == 0) a.part_ml[at] = make_float2(m, l);
         }
     }
 }
 
-// Joins the ranges: one warp per query row.  Lane s holds the maximum and sum of range s; the outputs are taken four ranges at a time.
+// Joins the ranges: a warp to a query row.
 template <int D>
 __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ CaArgs a, int tiles, int rows) {
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, G = a.hq / a.hk, R = G * a.n;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, R = a.hq / a.hk * a.n, i = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (i >= a.hk * R) return;
+    constexpr int E = D / 32;
     const int kvh = i / R, r = i - kvh * R, tile = r / rows;
     const int64_t T = ca_pos(a.pos_dev, a.pos, a.cap, a.n) + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
-    const int active = (int)((T + chunk - 1) / chunk), stride = rows * (D + 2);
-    const float* x = a.part + ((int64_t)kvh * tiles + tile) * a.nsplit * stride + (r - tile * rows) * (D + 2);
-    constexpr int E = D / 32;
+    const int active = (int)((T + chunk - 1) / chunk);
+    const int64_t first = ((int64_t)kvh * tiles + tile) * a.nsplit * rows + (r - tile * rows);
     float m = -INFINITY, l = 0.0f, v[E] = {};
     for (int s0 = 0; s0 < active; s0 += 32) {
-        const bool on = s0 + lane < active;
-        const float* y = x + (int64_t)(s0 + lane) * stride;
-        const float ms = on ? y[D] : -INFINITY, ls = on ? y[D + 1] : 0.0f, mn = fmaxf(m, warp_max(ms));
-        const float f = ms == -INFINITY ? 0.0f : ca_ex2(ms - mn), old = m == -INFINITY ? 0.0f : ca_ex2(m - mn);
-        float lw = ls * f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
-        l = l * old + lw;
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] *= old;
-        m = mn;
         const int count = active - s0 < 32 ? active - s0 : 32;
-        for (int s = 0; s < count; s += 4) {
-            float z[4][E], w[4];
+        const float2 ml = lane < count ? a.part_ml[first + (int64_t)(s0 + lane) * rows] : make_float2(-INFINITY, 0.0f);
+        float m2 = ml.x, l2 = ml.y, v2[E];
+        ca_join<E, 10>(count, m2, l2, v2, [&](int s, float (&z)[E]) { ca_load<E>(a.part + (first + (int64_t)(s0 + s) * rows) * D + lane * E, z); });
+        const float top = fmaxf(m, m2), f1 = m == -INFINITY ? 0.0f : ca_ex2(m - top), f2 = m2 == -INFINITY ? 0.0f : ca_ex2(m2 - top);
+        l = l * f1 + l2 * f2;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = __shfl_sync(0xffffffffu, f, (s + j) & 31);
-#pragma unroll
-                for (int e = 0; e < E; ++e) z[j][e] = s + j < count ? x[(int64_t)(s0 + s + j) * stride + lane * E + e] : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (s + j < count && w[j] != 0.0f)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] += z[j][e] * w[j];
-        }
+        for (int e = 0; e < E; ++e) v[e] = (f1 == 0.0f ? 0.0f : v[e] * f1) + (f2 == 0.0f ? 0.0f : v2[e] * f2);
+        m = top;
     }
-    const int tk = r / G, hd = kvh * G + r - tk * G;
-    uint16_t* o = a.out + (int64_t)tk * a.hq * D + hd * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(o + e) = l == 0.0f ? 0u : pack_bf16x2(v[e] / l, v[e + 1] / l);
+    ca_output<D>(a, kvh, r, lane, v, l);
 }
 
 static CaPlan ca_plan(int64_t positions, int R, int hk) {
@@ -471,7 +432,7 @@ static int launch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
 }
 template <int D, bool I8>
 static int dispatch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) { return p.nt == 1 ? launch_ca<D, I8, 1>(a, p, st) : launch_ca<D, I8, 2>(a, p, st); }
-static int64_t ca_scratch(const CaPlan& p, int hk, int d) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * p.rows * (d + 2) * 4; }
+static int64_t ca_states(const CaPlan& p, int hk) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * p.rows; }      // partial states of query rows
 
 }  // namespace scmx
 
@@ -479,7 +440,7 @@ using namespace scmx;
 
 extern "C" int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int hk, int d) {
     if (positions < 1 || n < 1 || n > CA_MAX_ROWS || hk < 1 || hq < hk || hq % hk || (d != 64 && d != 128)) return 0;
-    return ca_scratch(ca_plan(positions, hq / hk * n, hk), hk, d);
+    return ca_states(ca_plan(positions, hq / hk * n, hk), hk) * (d + 2) * 4;
 }
 
 extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,
@@ -496,11 +457,11 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
     CaArgs a;
     const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk);
     a.nsplit = p.nsplit; a.unit = p.unit;
-    const int64_t need = ca_scratch(p, hk, d);
+    const int64_t states = ca_states(p, hk), need = states * (d + 2) * 4;
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",
                  (long long)scratch_bytes, (long long)need);
     a.q = q; a.q_hs = q_head_stride; a.q_rs = q_row_stride; a.k = k; a.v = v; a.ks = k_scales; a.vs = v_scales; a.mask = mask; a.pos_dev = pos_dev; a.pos = pos;
-    a.part = need ? static_cast<float*>(scratch) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.scale = scale * CA_LOG2E;
+    a.part = need ? static_cast<float*>(scratch) : nullptr; a.part_ml = need ? reinterpret_cast<float2*>(a.part + states * d) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.scale = scale * CA_LOG2E;
     const cudaStream_t st = (cudaStream_t)stream;
     int rc = p.tc ? cache_attn_tc(a, p, d, int8, status, st)
              : d == 128 ? (int8 ? dispatch_ca<128, true>(a, p, st) : dispatch_ca<128, false>(a, p, st))

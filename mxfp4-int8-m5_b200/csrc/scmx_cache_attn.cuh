@@ -1,5 +1,6 @@
 // What the two kernels of attention to a cache share: arguments, the cut into ranges of positions.
 #pragma once
+#include <string.h>
 #include "scmx_common.cuh"
 #include "scmx_ptx.cuh"
 
@@ -16,7 +17,8 @@ struct CaArgs {
     const float *ks, *vs;            // [hk, cap] (INT8)
     const int64_t* mask;             // [n] or null: row i sees rows 0 .. i
     const int32_t* pos_dev;
-    float* part;                     // [hk, tiles, nsplit, rows of a tile, D + 2] or null (nsplit 1)
+    float* part;                     // sums of weighted values [hk, tiles, nsplit, rows of a CTA, D], or null (nsplit 1)
+    float2* part_ml;                 // their maxima (exponents of 2) and sums of weights, [hk, tiles, nsplit, rows]
     uint16_t* out;                   // bf16 [n, hq d]
     int64_t q_hs, q_rs, pos, cap;
     int n, hq, hk, nsplit, unit;
@@ -31,6 +33,62 @@ __device__ __forceinline__ int64_t ca_pos(const int32_t* pos_dev, int64_t pos, i
 __device__ __forceinline__ int64_t ca_chunk(int64_t T, int nsplit, int unit) {
     const int64_t c = (T + nsplit - 1) / nsplit;
     return (c + unit - 1) / unit * unit;
+}
+
+__device__ __forceinline__ float ca_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// E = D / 32 consecutive values of a row to a lane.
+template <int E> struct CaVec;
+template <> struct CaVec<2> { typedef float2 type; };
+template <> struct CaVec<4> { typedef float4 type; };
+template <int E>
+__device__ __forceinline__ void ca_load(const float* p, float (&v)[E]) {
+    const typename CaVec<E>::type x = *reinterpret_cast<const typename CaVec<E>::type*>(p);
+    memcpy(v, &x, sizeof(x));
+}
+template <int E>
+__device__ __forceinline__ void ca_store(float* p, const float (&v)[E]) {
+    typename CaVec<E>::type x;
+    memcpy(&x, v, sizeof(x));
+    *reinterpret_cast<typename CaVec<E>::type*>(p) = x;
+}
+// A query row of the output, v / total (zeros where nothing was seen).
+template <int D>
+__device__ __forceinline__ void ca_output(const CaArgs& a, int kvh, int row, int lane, const float (&v)[D / 32], float total) {
+    const int G = a.hq / a.hk, tok = row / G;
+    uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)tok * a.hq * D + (kvh * G + row - tok * G) * D) + lane * (D / 64);
+#pragma unroll
+    for (int e = 0; e < D / 32; e += 2) o[e / 2] = total == 0.0f ? 0u : pack_bf16x2(v[e] / total, v[e + 1] / total);
+}
+// Joins partial softmax states of one row by a whole warp: state s < count (count <= 32) has its maximum and sum in lane s's (m, l); values(s, v) gives the lane's E
+// values of it.  (m, l) become the joined maximum and sum, in every lane.
+template <int E, int BATCH, typename Values>
+__device__ __forceinline__ void ca_join(int count, float& m, float& l, float (&v)[E], Values values) {
+    const float top = warp_max(m), f = m == -INFINITY ? 0.0f : ca_ex2(m - top);
+    float total = l * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.0f;
+    for (int s = 0; s < count; s += BATCH) {
+        float z[BATCH][E];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (s + j < count) values(s + j, z[j]);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const float w = __shfl_sync(0xffffffffu, f, (s + j) & 31);
+            if (s + j < count && w != 0.0f)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = fmaf(z[j][e], w, v[e]);
+        }
+    }
+    m = top;
+    l = total;
 }
 
 // How a call is cut.  tc: by the tcgen05 kernel, `nt` query tiles of 128 in a CTA and `copies` of the rows in a tile; otherwise nt groups of eight query rows.

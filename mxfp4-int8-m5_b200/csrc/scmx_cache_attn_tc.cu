@@ -38,12 +38,13 @@ struct CtSmem {
     static constexpr int C_OFF = V_OFF + VS * KB * CT_TILE;
     static constexpr int SC_OFF = C_OFF + NS * CT_TILE;                       // scales: [CT_SCALES][keys, values][128] float
     static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
-    // kfull, kempty [KS], vfull, vempty [VS], codes full, empty [NS], scales [CT_SCALES], S, P, O [2]
-    static constexpr int NBAR = 2 * KS + 2 * VS + 2 * NS + (I8 ? CT_SCALES : 0) + 6;
+    // kfull, kempty [KS], vfull, vempty [VS], codes full, empty [NS], scales [CT_SCALES], S, P, O [2], queries
+    static constexpr int NBAR = 2 * KS + 2 * VS + 2 * NS + (I8 ? CT_SCALES : 0) + 7;
     static constexpr int MISC_OFF = BAR_OFF + 8 * NBAR;
     static constexpr int TOTAL = MISC_OFF + 32 + 1024;
-    static constexpr int ML_OFF = K_OFF + 256 * (D + 1) * 4;                  // outputs of 256 lanes from K_OFF on, then their maxima and sums, in place of operands
-    static_assert(MQ == 2 || ML_OFF + 2048 <= SC_OFF, "joined outputs fit the operands' memory");
+    static constexpr int PITCH = D + 4;                                       // outputs of 256 lanes from Q_OFF on, then maxima and sums, in place of operands
+    static constexpr int ML_OFF = Q_OFF + 256 * PITCH * 4;
+    static_assert(ML_OFF + 2048 <= SC_OFF, "joined outputs fit the operands' memory");
     static_assert(TOTAL <= 232448, "shared memory of an SM");
 };
 
@@ -69,13 +70,13 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
     cache_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CaArgs a, int32_t* status,
                          uint64_t wait_ns) {
     using L = CtSmem<D, I8, MQ>;
-    constexpr int KB = L::KB, KS = L::KS, VS = L::VS, NS = L::NS, THREADS = I8 ? 448 : 320;
+    constexpr int KB = L::KB, KS = L::KS, VS = L::VS, NS = L::NS;
     constexpr int RP = 128 / COPIES, ROWS = MQ * RP, NCH = 4 / COPIES;      // rows of a tile, of the CTA; 32-key pieces of a thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BAR_OFF;
     const uint32_t b_kf = bars, b_ke = b_kf + 8 * KS, b_vf = b_ke + 8 * KS, b_ve = b_vf + 8 * VS, b_cf = b_ve + 8 * VS, b_ce = b_cf + 8 * NS, b_sc = b_ce + 8 * NS,
-                   b_s = b_sc + (I8 ? 8 * CT_SCALES : 0), b_p = b_s + 16, b_o = b_p + 16;
+                   b_s = b_sc + (I8 ? 8 * CT_SCALES : 0), b_p = b_s + 16, b_o = b_p + 16, b_q = b_o + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
     uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF + 8);      // new rows with values that are not finite
@@ -88,17 +89,22 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
             const uint32_t b = bars + 8 * i;
             const bool weights = b == b_p || b == b_p + 8;                                                        // one arrival per softmax warp
             const bool converted = I8 && ((b >= b_kf && b < b_ke) || (b >= b_vf && b < b_ve) || (b >= b_ce && b < b_s));      // one per converting warp
-            mbar_init(b, weights || converted ? 4 : 1);
+            mbar_init(b, b == b_q ? 8 : weights || converted ? 4 : 1);
         }
         *abort_flag = 0;
         bad[0] = bad[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        proxy_fence();
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
     pdl_launch_dependents();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     pdl_wait();
 
     const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * ROWS;
@@ -107,27 +113,6 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
     const int nkeys = t1 > t0 ? (int)(t1 - t0) : 0, ntiles = (nkeys + 127) / 128, units = ntiles * MQ;
     const int dnew = (int)(t0 - pos > -(int64_t)nkeys - 64 ? t0 - pos : -(int64_t)nkeys - 64);      // the range's first key, counted from the first new row
 
-    // queries: K-major tiles with the 128-byte swizzle; a negative scale is taken by the queries
-    if (ntiles) {
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        for (int i = tid; i < MQ * 128 * (D / 8); i += THREADS) {
-            const int c = i % (D / 8), l = i / (D / 8), r = row0 + l / 128 * RP + l % 128 % RP, tok = r / G;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (r < R) {
-                const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 8 * c);
-                const uint2 x = p[0], y = p[1];
-                if constexpr (I8) w = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x5410), __byte_perm(y.x, y.y, 0x7632));
-                else w = make_uint4(x.x, x.y, y.x, y.y);
-                w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-            }
-            *reinterpret_cast<uint4*>(smem + L::Q_OFF + (l / 128 * KB + c / 8) * CT_TILE + l % 128 * 128 + (((c & 7) ^ (l & 7)) << 4)) = w;
-        }
-        proxy_fence();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     int fail = 0;
 
     if (warp == 0) {
@@ -178,7 +163,7 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
             if (MQ == 1 || m == 1) umma_commit(on, b_ke + 8 * ks);
             return true;
         };
-        bool ok = units == 0 || scores(0);
+        bool ok = units == 0 || (wait(b_q, 0, 72) && scores(0));
         if (ok && units > 1) ok = scores(1);
         for (int u = 0; u < units && ok; ++u) {
             const int m = u & 1, j = MQ == 2 ? u >> 1 : u, vs = j % VS;
@@ -194,6 +179,26 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
         }
         if (!on) fail = fail > 0 ? -1 : fail;      // one lane reports
     } else if (warp < 10) {
+        // queries: K-major tiles with the 128-byte swizzle; a negative scale is taken by the queries
+        if (ntiles) {
+            const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll 4
+            for (int i = tid - 64; i < MQ * 128 * (D / 8); i += 256) {
+                const int c = i % (D / 8), l = i / (D / 8), r = row0 + l / 128 * RP + l % 128 % RP, tok = r / G;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (r < R) {
+                    const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 8 * c);
+                    const uint2 x = p[0], y = p[1];
+                    if constexpr (I8) w = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x5410), __byte_perm(y.x, y.y, 0x7632));
+                    else w = make_uint4(x.x, x.y, y.x, y.y);
+                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+                }
+                *reinterpret_cast<uint4*>(smem + L::Q_OFF + (l / 128 * KB + c / 8) * CT_TILE + l % 128 * 128 + (((c & 7) ^ (l & 7)) << 4)) = w;
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_q);
+        }
         const int m = (warp - 2) >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = row / G;
         const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
         const int c0 = copy * (128 / COPIES);                   // the thread's first key of a tile
@@ -351,81 +356,45 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
             if (__any_sync(0xffffffffu, w)) fail = w == 1 ? 75 : -1;
             tc_fence_after();
         }
+        // every lane's output to shared memory, then a warp to a row: the states of its copies and streams are joined
+        constexpr int E = D / 32, STATES = MQ == 2 ? 1 : 2 * COPIES;
         const bool mine = fail == 0 && units > m;
-        float* out = reinterpret_cast<float*>(smem + L::K_OFF);
+        float* out = reinterpret_cast<float*>(smem + L::Q_OFF);
         float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
-        // what a value that is not finite adds to a row that sees it
-        auto odd_values = [&](uint64_t see, int d) {
-            float x = 0.0f;
-            for (uint64_t b = see; b; b &= b - 1) {
-                const float v = bf16_to_f32(static_cast<const uint16_t*>(a.v)[((int64_t)kvh * a.cap + pos + (__ffsll((long long)b) - 1)) * D + d]);
-                if ((__float_as_uint(v) & 0x7F800000u) == 0x7F800000u) x += v;
-            }
-            return x;
-        };
-        // a result: value d of a query row, with the maximum and sum of its positions in this range
-        auto put = [&](int rr, int d, float v, float mxl, float total) {
-            if (a.part != nullptr) {
-                float* y = a.part + ((((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS + (rr - row0)) * (D + 2);
-                y[d] = v;
-                if (d == 0) {
-                    y[D] = mxl;
-                    y[D + 1] = total;
+        const int slot = 128 * m + l;
+        ml[slot] = mine && sum != 0.0f ? make_float2(mx * sl, sum) : make_float2(-INFINITY, 0.0f);
+        for (int c = 0; c < D / 32 && mine; ++c) {
+            uint32_t v[32];
+            tmem_ld32(to + 32 * c, v);
+            tmem_ld_fence(v);
+            float4* p = reinterpret_cast<float4*>(out + slot * L::PITCH + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)      // INT8: values 1 and 2 of four change places again
+                p[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + (I8 ? 2 : 1)]), __uint_as_float(v[4 * i + (I8 ? 1 : 2)]), __uint_as_float(v[4 * i + 3]));
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
+        const int rows = units == 0 ? 0 : R - row0 < ROWS ? R - row0 : ROWS;
+        for (int r = warp - 2; r < rows; r += 8) {
+            const int s = lane < STATES ? lane : 0, at = MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r;
+            const float2 z = lane < STATES ? ml[at] : make_float2(-INFINITY, 0.0f);
+            float top = z.x, total = z.y, v[E];
+            ca_join<E, STATES>(STATES, top, total, v, [&](int s, float (&z)[E]) { ca_load<E>(out + (MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r) * L::PITCH + lane * E, z); });
+            if (odd) {                       // new rows' values that are not finite, to a row that sees them
+                const int tk = (row0 + r) / G;
+                for (uint64_t b = (a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull) & odd; b; b &= b - 1) {
+                    const uint16_t* p = static_cast<const uint16_t*>(a.v) + ((int64_t)kvh * a.cap + pos + (__ffsll((long long)b) - 1)) * D + lane * E;
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if ((p[e] & 0x7F80u) == 0x7F80u) v[e] += bf16_to_f32(p[e]);
                 }
+            }
+            if (a.part == nullptr) {
+                ca_output<D>(a, kvh, row0 + r, lane, v, total);
             } else {
-                const int tk = rr / G;
-                a.out[(int64_t)tk * a.hq * D + (kvh * G + rr - tk * G) * D + d] = f32_to_bf16(total == 0.0f ? 0.0f : v / total);
-            }
-        };
-        auto place = [](int c) { return I8 ? (c & ~3) | ((c & 1) << 1) | ((c >> 1) & 1) : c; };      // the value that a column holds
-        const float mxl = sum == 0.0f ? -INFINITY : mx * sl;
-        if constexpr (MQ == 2) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const uint64_t see = bits & ((uint64_t)bad[1] << 32 | bad[0]);
-            for (int c = 0; c < D / 32 && mine; ++c) {      // a tensor-memory load is the whole warp's
-                uint32_t v[32];
-                tmem_ld32(to + 32 * c, v);
-                tmem_ld_fence(v);
-                if (row < R)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int d = place(32 * c + i);
-                        put(row, d, __uint_as_float(v[i]) + (see ? odd_values(see, d) : 0.0f), mxl, sum);
-                    }
-            }
-        } else {
-            const int slot = 128 * m + l;
-            ml[slot] = mine ? make_float2(mxl, sum) : make_float2(-INFINITY, 0.0f);
-            if (mine)
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(to + 32 * c, v);
-                    tmem_ld_fence(v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) out[slot * (D + 1) + place(32 * c + i)] = __uint_as_float(v[i]);
-                }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
-            for (int i = 128 * m + l; i < RP * D; i += 256) {
-                const int r = i / D, d = i - r * D, rr = row0 + r;
-                if (rr >= R || units == 0) break;
-                float top = -INFINITY, total = 0.0f, v = 0.0f;
-#pragma unroll
-                for (int s = 0; s < 2 * COPIES; ++s) top = fmaxf(top, ml[(s & 1) * 128 + (s >> 1) * RP + r].x);
-#pragma unroll
-                for (int s = 0; s < 2 * COPIES; ++s) {
-                    const int at = (s & 1) * 128 + (s >> 1) * RP + r;
-                    const float2 z = ml[at];
-                    const float f = z.x == -INFINITY ? 0.0f : ex2_approx(z.x - top);
-                    total += z.y * f;
-                    if (f != 0.0f) v += out[at * (D + 1) + d] * f;
-                }
-                if (odd) {
-                    const int tk = rr / G;
-                    const uint64_t b = a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull;
-                    v += odd_values(b & odd, d);
-                }
-                put(rr, d, v, top, total);
+                const int64_t to_row = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS + r;
+                ca_store<E>(a.part + to_row * D + lane * E, v);
+                if (lane == 0) a.part_ml[to_row] = make_float2(top, total);
             }
         }
     } else if (I8) {

@@ -5,13 +5,13 @@
 // key tiles (128 positions) in turn and are joined at the end; with two, each stream has a query tile of its own.  A `unit` is a stream's work
 // on one key tile: S = Q K^T (128 x 128, float32 in tensor memory), softmax, O += P V with P (bfloat16) read from tensor memory, where it
 // overwrites S.
-//   warp 0        TMA producer of key and value tiles
-//   warp 1        all MMAs (the warp stays converged, one lane issues)
-//   warps 2-9     two softmax warpgroups, one per stream, a thread per lane of tensor memory.  The maximum is raised when it has grown by
+//   warps 0-7     two softmax warpgroups, one per stream, a thread per lane of tensor memory.  The maximum is raised when it has grown by
 //                 more than 2^8
-//   warps 10-13   (INT8) codes of a tile to bfloat16 operands, exactly; a position's key scale multiplies its scores, its value scale its
-//                 weights.  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are laid
-//                 out alike, and outputs put back
+//   warps 8-15    (INT8) codes of a tile from memory to bfloat16 operands, exactly; a position's key scale multiplies its scores, its value scale
+//                 its weights.  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are
+//                 laid out alike, and outputs put back.  Tiles ahead are prefetched into L2
+//   last four     one warp issues all MMAs (it stays converged, one lane issues), one loads key and value tiles by TMA (bfloat16)
+// Registers are shared out by role (setmaxnreg): the softmax holds a row's scores.
 // Up to 64 query rows leave lanes idle: a tile then holds two or four copies of them, each copy's threads take a half or a quarter of a tile's
 // keys, and their weights for the other keys are zero.  The copies are joined like the streams.  So the softmax of few rows is spread over all
 // threads, and the products, which a memory-bound call has time for, stay whole tiles.
@@ -23,23 +23,25 @@
 
 namespace scmx {
 
-constexpr int CT_TILE = 128 * 128;        // bytes of a [128 rows x 64 bfloat16] or [128 x 128 INT8] block
-constexpr int CT_SCALES = 4;              // tiles whose scales are held
+constexpr int CT_TILE = 128 * 128;        // bytes of a [128 rows x 64 bfloat16] block
+constexpr int CT_SCALES = 8;              // tiles whose scales are held
+constexpr int CT_AHEAD = 6;               // tiles that are prefetched into L2
 
 template <int D, bool I8, int MQ>
 struct CtSmem {
     static constexpr int KB = D / 64;
-    static constexpr int KS = D == 64 ? (I8 ? 2 : 4) : I8 ? (MQ == 2 ? 1 : 2) : (MQ == 2 ? 2 : 3);       // stages of key operands
-    static constexpr int VS = KS;
-    static constexpr int NS = !I8 ? 0 : D == 64 ? 6 : MQ == 2 ? 5 : 3;                                    // stages of INT8 tiles
+    static constexpr int KS = D == 64 ? 4 : I8 || MQ == 2 ? 2 : 3;            // stages of keys
+    static constexpr int VS = D == 64 ? 4 : MQ == 2 ? 2 : 3;                  // stages of values
     static constexpr int Q_OFF = 0;
     static constexpr int K_OFF = Q_OFF + MQ * KB * CT_TILE;
     static constexpr int V_OFF = K_OFF + KS * KB * CT_TILE;
-    static constexpr int C_OFF = V_OFF + VS * KB * CT_TILE;
-    static constexpr int SC_OFF = C_OFF + NS * CT_TILE;                       // scales: [CT_SCALES][keys, values][128] float
+    static constexpr int SC_OFF = V_OFF + VS * KB * CT_TILE;                  // scales: [CT_SCALES][keys, values][128] float
     static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
-    // kfull, kempty [KS], vfull, vempty [VS], codes full, empty [NS], scales [CT_SCALES], S, P, O [2], queries
-    static constexpr int NBAR = 2 * KS + 2 * VS + 2 * NS + (I8 ? CT_SCALES : 0) + 7;
+    // kfull, kempty [KS], vfull, vempty [VS], scales [CT_SCALES], S, P, O [2], queries
+    static constexpr int NBAR = 2 * KS + 2 * VS + (I8 ? CT_SCALES : 0) + 7;
+    // threads, and registers of a thread by role: together no more than the block is launched with
+    static constexpr int THREADS = I8 ? 640 : 384, LAUNCH_REGS = I8 ? 96 : 168, SOFT_REGS = I8 ? 128 : 192, CONV_REGS = 72, MISC_REGS = I8 ? 72 : 120;
+    static_assert(256 * SOFT_REGS + (I8 ? 256 * CONV_REGS : 0) + 128 * MISC_REGS <= THREADS * LAUNCH_REGS, "registers of a block");
     static constexpr int MISC_OFF = BAR_OFF + 8 * NBAR;
     static constexpr int TOTAL = MISC_OFF + 32 + 1024;
     static constexpr int PITCH = D + 4;                                       // outputs of 256 lanes from Q_OFF on, then maxima and sums, in place of operands
@@ -64,39 +66,47 @@ __device__ __forceinline__ uint32_t ct_seen(uint64_t bits, int b) {
     return b < 64 ? (uint32_t)(bits >> b) : 0u;
 }
 
+template <bool UP, int N>
+__device__ __forceinline__ void set_regs() {
+    if (UP) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // MQ: query tiles; COPIES of the rows in a tile (1 with two tiles).
 template <int D, bool I8, int MQ, int COPIES>
-__global__ void __launch_bounds__(I8 ? 448 : 320, 1)
+__global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     cache_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CaArgs a, int32_t* status,
                          uint64_t wait_ns) {
     using L = CtSmem<D, I8, MQ>;
-    constexpr int KB = L::KB, KS = L::KS, VS = L::VS, NS = L::NS;
+    constexpr int KB = L::KB, KS = L::KS, VS = L::VS;
     constexpr int RP = 128 / COPIES, ROWS = MQ * RP, NCH = 4 / COPIES;      // rows of a tile, of the CTA; 32-key pieces of a thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BAR_OFF;
-    const uint32_t b_kf = bars, b_ke = b_kf + 8 * KS, b_vf = b_ke + 8 * KS, b_ve = b_vf + 8 * VS, b_cf = b_ve + 8 * VS, b_ce = b_cf + 8 * NS, b_sc = b_ce + 8 * NS,
-                   b_s = b_sc + (I8 ? 8 * CT_SCALES : 0), b_p = b_s + 16, b_o = b_p + 16, b_q = b_o + 16;
+    const uint32_t b_kf = bars, b_ke = b_kf + 8 * KS, b_vf = b_ke + 8 * KS, b_ve = b_vf + 8 * VS, b_sc = b_ve + 8 * VS, b_s = b_sc + (I8 ? 8 * CT_SCALES : 0),
+                   b_p = b_s + 16, b_o = b_p + 16, b_q = b_o + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
     uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF + 8);      // new rows with values that are not finite
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, tid = threadIdx.x;
 
     if (tid == 0) {
-        prefetch_map(&tmK);
-        prefetch_map(&tmV);
+        if (!I8) {
+            prefetch_map(&tmK);
+            prefetch_map(&tmV);
+        }
         for (int i = 0; i < L::NBAR; ++i) {
             const uint32_t b = bars + 8 * i;
-            const bool weights = b == b_p || b == b_p + 8;                                                        // one arrival per softmax warp
-            const bool converted = I8 && ((b >= b_kf && b < b_ke) || (b >= b_vf && b < b_ve) || (b >= b_ce && b < b_s));      // one per converting warp
-            mbar_init(b, b == b_q ? 8 : weights || converted ? 4 : 1);
+            const bool converted = I8 && ((b >= b_kf && b < b_ke) || (b >= b_vf && b < b_ve) || (b >= b_sc && b < b_s));      // one arrival per converting warp
+            mbar_init(b, b == b_q || converted ? 8 : b == b_p || b == b_p + 8 ? 4 : 1);                                     // weights: one per softmax warp
         }
         *abort_flag = 0;
         bad[0] = bad[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         proxy_fence();
     }
-    if (warp == 1) {
+    constexpr int MISC = I8 ? 16 : 8;        // first of the last four warps: MMAs; the one after it: TMA
+    if (warp == MISC) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
@@ -115,31 +125,21 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
 
     int fail = 0;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp > MISC) {
+        set_regs<false, L::MISC_REGS>();
+        if (!I8 && warp == MISC + 1 && lane == 0) {
             for (int j = 0; j < ntiles; ++j) {
-                const int key = (int)t0 + 128 * j;
-                if constexpr (I8) {
-                    bool ok = true;
-                    for (int h = 0; h < 2 && ok; ++h) {
-                        const int i = 2 * j + h, s = i % NS;
-                        if (int w = mbar_wait(b_ce + 8 * s, ((i / NS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; ok = false; break; }
-                        mbar_expect_tx(b_cf + 8 * s, CT_TILE);
-                        tma_load_3d(sbase + L::C_OFF + s * CT_TILE, h ? &tmV : &tmK, 0, key, kvh, b_cf + 8 * s);
-                    }
-                    if (!ok) break;
-                } else {
-                    const int ks = j % KS, vs = j % VS;
-                    if (int w = mbar_wait(b_ke + 8 * ks, ((j / KS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
-                    mbar_expect_tx(b_kf + 8 * ks, KB * CT_TILE);
-                    for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::K_OFF + (ks * KB + c) * CT_TILE, &tmK, c * 128, key, kvh, b_kf + 8 * ks);
-                    if (int w = mbar_wait(b_ve + 8 * vs, ((j / VS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
-                    mbar_expect_tx(b_vf + 8 * vs, KB * CT_TILE);
-                    for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::V_OFF + (vs * KB + c) * CT_TILE, &tmV, c * 128, key, kvh, b_vf + 8 * vs);
-                }
+                const int key = (int)t0 + 128 * j, ks = j % KS, vs = j % VS;
+                if (int w = mbar_wait(b_ke + 8 * ks, ((j / KS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
+                mbar_expect_tx(b_kf + 8 * ks, KB * CT_TILE);
+                for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::K_OFF + (ks * KB + c) * CT_TILE, &tmK, c * 128, key, kvh, b_kf + 8 * ks);
+                if (int w = mbar_wait(b_ve + 8 * vs, ((j / VS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
+                mbar_expect_tx(b_vf + 8 * vs, KB * CT_TILE);
+                for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::V_OFF + (vs * KB + c) * CT_TILE, &tmV, c * 128, key, kvh, b_vf + 8 * vs);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == MISC) {
+        set_regs<false, L::MISC_REGS>();
         const uint32_t on = elect_lane();
         const uint32_t idesc_s = umma_idesc_bf16(128, 128), idesc_o = umma_idesc_bf16(128, D) | IDESC_B_MN;
         int kt = -1, vt = -1;            // last tiles that were waited for
@@ -178,28 +178,37 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
             else ok = scores(u + 2);
         }
         if (!on) fail = fail > 0 ? -1 : fail;      // one lane reports
-    } else if (warp < 10) {
-        // queries: K-major tiles with the 128-byte swizzle; a negative scale is taken by the queries
+    } else if (warp < 8) {
+        set_regs<true, L::SOFT_REGS>();
+        // queries: K-major tiles with the 128-byte swizzle, half a row to a thread; a negative scale is taken by the queries
         if (ntiles) {
             const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 4
-            for (int i = tid - 64; i < MQ * 128 * (D / 8); i += 256) {
-                const int c = i % (D / 8), l = i / (D / 8), r = row0 + l / 128 * RP + l % 128 % RP, tok = r / G;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (r < R) {
-                    const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 8 * c);
-                    const uint2 x = p[0], y = p[1];
-                    if constexpr (I8) w = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(y.x, y.y, 0x5410), __byte_perm(y.x, y.y, 0x7632));
-                    else w = make_uint4(x.x, x.y, y.x, y.y);
-                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+            const int ql = tid & 127, half = tid >> 7;
+#pragma unroll
+            for (int t = 0; t < MQ; ++t) {
+                const int r = row0 + t * 128 + ql % RP, qt = r / G;
+                const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + (r < R ? r - qt * G : 0)) * a.q_hs + (int64_t)(r < R ? qt : 0) * a.q_rs) + half * (D / 8);
+                uint2 x[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) x[i] = p[i];
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint2 u = x[2 * i], v = x[2 * i + 1];
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (r < R) {
+                        if constexpr (I8) w = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
+                        else w = make_uint4(u.x, u.y, v.x, v.y);
+                        w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+                    }
+                    const int c = half * (D / 16) + i;
+                    *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * KB + c / 8) * CT_TILE + ql * 128 + (((c & 7) ^ (ql & 7)) << 4)) = w;
                 }
-                *reinterpret_cast<uint4*>(smem + L::Q_OFF + (l / 128 * KB + c / 8) * CT_TILE + l % 128 * 128 + (((c & 7) ^ (l & 7)) << 4)) = w;
             }
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_q);
         }
-        const int m = (warp - 2) >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = row / G;
+        const int m = warp >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = row / G;
         const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
         const int c0 = copy * (128 / COPIES);                   // the thread's first key of a tile
         uint64_t bits = 0;
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
         const int rows = units == 0 ? 0 : R - row0 < ROWS ? R - row0 : ROWS;
-        for (int r = warp - 2; r < rows; r += 8) {
+        for (int r = warp; r < rows; r += 8) {
             const int s = lane < STATES ? lane : 0, at = MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r;
             const float2 z = lane < STATES ? ml[at] : make_float2(-INFINITY, 0.0f);
             float top = z.x, total = z.y, v[E];
@@ -398,52 +407,76 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
             }
         }
     } else if (I8) {
-        // codes to operands: a thread to a position
-        const int r = tid - 320;
+        set_regs<false, L::CONV_REGS>();
+        // codes to operands: 16 codes of a vector to a thread, CPR threads to a vector, PASSES vectors to a thread
+        constexpr int CPR = D / 16, PASSES = 128 * CPR / 256;
+        const int t = tid - 256, cc = t % CPR, r0 = t / CPR;
         const I8Pairs i8;
-        const float factor = fabsf(a.scale);
-        constexpr int N = NS ? NS : 1;
-        for (int i = 0; i < 2 * ntiles; ++i) {
-            const int j = i >> 1, s = i % N, st = j % KS;
-            const bool val = i & 1;
-            float ksc = 0.0f, vsc = 0.0f;
-            if (!val && t0 + 128 * j + r < t1) {
-                const int64_t at = (int64_t)kvh * a.cap + t0 + 128 * j + r;
-                ksc = a.ks[at] * factor;
-                vsc = a.vs[at];
-            }
-            int w = mbar_wait(b_cf + 8 * s, (i / N) & 1, abort_flag, wait_ns);
-            if (!w) w = mbar_wait((val ? b_ve : b_ke) + 8 * st, ((j / KS) & 1) ^ 1, abort_flag, wait_ns);
-            if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 76 : -1; break; }
-            const uint8_t* src = smem + L::C_OFF + s * CT_TILE + r * 128;
-            uint8_t* dst = smem + (val ? L::V_OFF : L::K_OFF) + st * KB * CT_TILE + r * 128;
+        const int8_t *kc = static_cast<const int8_t*>(a.k) + ((int64_t)kvh * a.cap + t0) * D, *vc = static_cast<const int8_t*>(a.v) + ((int64_t)kvh * a.cap + t0) * D;
+        auto load = [&](const int8_t* p, int j, uint4 (&x)[PASSES]) {
 #pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-                const uint4 c = *reinterpret_cast<const uint4*>(src + ((x ^ (r & 7)) << 4));
-                const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+            for (int i = 0; i < PASSES; ++i) {
+                const int r = 128 * j + r0 + i * (256 / CPR);
+                x[i] = r < nkeys ? __ldg(reinterpret_cast<const uint4*>(p + (int64_t)r * D + 16 * cc)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto ahead = [&](int j) {                 // a tile's keys (thread 0) and values (thread 32) into L2
+            const int n = nkeys - 128 * j < 128 ? nkeys - 128 * j : 128;
+            if (n > 0 && (t & ~32) == 0) {
+                const int8_t* p = (t ? vc : kc) + (int64_t)128 * j * D;
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * D) : "memory");
+            }
+        };
+        auto convert = [&](uint8_t* dst, const uint4 (&x)[PASSES]) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int r = r0 + i * (256 / CPR);
+                const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 uint32_t o[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     o[2 * e] = i8.even(u[e]);
                     o[2 * e + 1] = i8.odd(u[e]);
                 }
-                uint8_t* p = dst + x / 4 * CT_TILE;
-                const int e = 2 * (x & 3);
-                *reinterpret_cast<uint4*>(p + ((e ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4*>(p + (((e + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                uint8_t* p = dst + cc / 4 * CT_TILE + r * 128;
+                const int e = 2 * (cc & 3), swap = cc >> 2;      // the upper half's stores in the other order: all of a vector's fall on different banks
+                const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                *reinterpret_cast<uint4*>(p + (((e + swap) ^ (r & 7)) << 4)) = swap ? hi : lo;
+                *reinterpret_cast<uint4*>(p + (((e + 1 - swap) ^ (r & 7)) << 4)) = swap ? lo : hi;
             }
-            if (!val) {
-                float* sc = reinterpret_cast<float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 256 + r;
-                sc[0] = ksc;
-                sc[128] = vsc;
-            }
+        };
+        // a position's scales: keys' by threads 0-127, values' by the others, loaded a tile ahead
+        const float* scales = (t < 128 ? a.ks : a.vs) + (int64_t)kvh * a.cap + t0 + (t & 127);
+        const float factor = t < 128 ? fabsf(a.scale) : 1.0f;
+        auto scale = [&](int j) { return 128 * j + (t & 127) < nkeys ? __ldg(scales + 128 * j) : 0.0f; };
+        uint4 xk[PASSES], xv[PASSES];
+        for (int j = 1; j < CT_AHEAD; ++j) ahead(j);
+        load(kc, 0, xk);
+        load(vc, 0, xv);
+        float sc = scale(0);
+        auto ready = [&](uint32_t empty, int j, int stages) -> bool {
+            const int w = mbar_wait(empty + 8 * (j % stages), ((j / stages) & 1) ^ 1, abort_flag, wait_ns);
+            if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 76 : -1; return false; }
+            return true;
+        };
+        auto done = [&](uint32_t full) {
             proxy_fence();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(b_ce + 8 * s);
-                mbar_arrive((val ? b_vf : b_kf) + 8 * st);
-                if (!val) mbar_arrive(b_sc + 8 * (j & (CT_SCALES - 1)));
-            }
+            if (lane == 0) mbar_arrive(full);
+        };
+        for (int j = 0; j < ntiles; ++j) {
+            ahead(j + CT_AHEAD);
+            if (!ready(b_ke, j, KS)) break;
+            convert(smem + L::K_OFF + j % KS * KB * CT_TILE, xk);
+            reinterpret_cast<float*>(smem + L::SC_OFF)[(j & (CT_SCALES - 1)) * 256 + t] = sc * factor;
+            if (j + 1 < ntiles) load(kc, j + 1, xk);
+            sc = scale(j + 1);
+            done(b_kf + 8 * (j % KS));
+            if (lane == 0) mbar_arrive(b_sc + 8 * (j & (CT_SCALES - 1)));
+            if (!ready(b_ve, j, VS)) break;
+            convert(smem + L::V_OFF + j % VS * KB * CT_TILE, xv);
+            if (j + 1 < ntiles) load(vc, j + 1, xv);
+            done(b_vf + 8 * (j % VS));
         }
     }
 
@@ -462,7 +495,7 @@ __global__ void __launch_bounds__(I8 ? 448 : 320, 1)
         while (globaltimer_ns() - begin < 200000ull) __nanosleep(1000);   // 0.2 ms for outstanding TMA writes
         __syncthreads();
     }
-    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (warp == MISC) tmem_dealloc(tmem, 512);
 }
 
 template <int D, bool I8, int MQ, int COPIES>
@@ -476,7 +509,7 @@ static int launch_ct(const CUtensorMap& k, const CUtensorMap& v, const CaArgs& a
         configured[dev] = true;
     }
     SCMX_PDL_OK("cache_attn_tc_kernel", launch_pdl(cache_attn_tc_kernel<D, I8, MQ, COPIES>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles),
-                                                   dim3(I8 ? 448 : 320), (size_t)L::TOTAL, st, k, v, a, status, g_wait_limit_ns));
+                                                   dim3(L::THREADS), (size_t)L::TOTAL, st, k, v, a, status, g_wait_limit_ns));
     return SCMX_OK;
 }
 template <int D, bool I8>
@@ -489,10 +522,14 @@ static int dispatch_ct(const CUtensorMap& k, const CUtensorMap& v, const CaArgs&
 int cache_attn_tc(const CaArgs& a, const CaPlan& p, int d, int int8, int32_t* status, cudaStream_t st) {
     SCMX_REQUIRE(a.cap < (1ll << 31) - 128, SCMX_ELIMIT, "cache_attn: a cache of %lld positions", (long long)a.cap);
     CUtensorMap k, v;
-    const int64_t row = int8 ? d : 2 * d;
-    int rc = make_map_planes(&k, a.k, a.hk, a.cap, row, row, row * a.cap, 128);
-    if (!rc) rc = make_map_planes(&v, a.v, a.hk, a.cap, row, row, row * a.cap, 128);
-    if (rc) return rc;
+    if (int8) {
+        memset(&k, 0, sizeof(k));            // codes are loaded by threads
+        memset(&v, 0, sizeof(v));
+    } else {
+        int rc = make_map_planes(&k, a.k, a.hk, a.cap, 2 * d, 2 * d, 2ll * d * a.cap, 128);
+        if (!rc) rc = make_map_planes(&v, a.v, a.hk, a.cap, 2 * d, 2 * d, 2ll * d * a.cap, 128);
+        if (rc) return rc;
+    }
     if (d == 128) return int8 ? dispatch_ct<128, true>(k, v, a, p, status, st) : dispatch_ct<128, false>(k, v, a, p, status, st);
     return int8 ? dispatch_ct<64, true>(k, v, a, p, status, st) : dispatch_ct<64, false>(k, v, a, p, status, st);
 }

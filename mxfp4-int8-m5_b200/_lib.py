@@ -41,11 +41,6 @@ class ScmxF4Job(ctypes.Structure):
     _fields_ = [("bcodes", ctypes.c_void_p), ("factors", ctypes.c_void_p), ("E", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64)]
 
 
-class ScmxKvLayer(ctypes.Structure):
-    """Mirror of `scmx_kv_layer` in include/scmx.h."""
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p)]
-
-
 class ScmxError(RuntimeError):
     """A libscmx entry point returned a non-zero status."""
 
@@ -123,7 +118,7 @@ SIGNATURES = {
     "scmx_norm_route_token": [c_vp, c_vp, c_float, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp],
     "scmx_kv_append": [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp],
     "scmx_kv_read": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_i64, c_vp, c_vp, c_vp],
-    "scmx_kv_keep": [ctypes.POINTER(ScmxKvLayer), c_int, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp],
+    "scmx_kv_keep": [c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_int, c_int, c_i64, c_int, c_vp],
     "scmx_cache_attn_scratch": [c_i64, c_int, c_int, c_int, c_int],
     "scmx_cache_attn": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_float, c_vp, c_vp, c_i64,
                         c_vp, c_vp],
@@ -275,11 +270,15 @@ def require_cuda(*tensors):
 
 def require_here(*tensors, contiguous=True):
     """CUDA tensors of the current device, whose stream a call is launched on."""
+    here = None
     for t in tensors:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda) or (contiguous and not t.is_contiguous()):
+        dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if dev < 0 or (contiguous and not t.is_contiguous()):
             raise TypeError(f"expected {'contiguous ' if contiguous else ''}CUDA tensors; this package has no CPU path")
-        if t.get_device() != torch._C._cuda_getDevice():
-            raise ValueError(f"a tensor on device {t.get_device()}, the current device is {torch._C._cuda_getDevice()}")
+        if here is None:
+            here = torch._C._cuda_getDevice()
+        if dev != here:
+            raise ValueError(f"a tensor on device {dev}, the current device is {here}")
 
 
 _sms = {}
@@ -294,7 +293,7 @@ def sm_count():
     return n
 
 
-_status = {}
+_status, _status_ptr = {}, {}
 
 
 def status_buffer():
@@ -305,6 +304,14 @@ def status_buffer():
         with torch.cuda.device(dev):      # kernels whose entry point takes no status argument report here too
             call("scmx_set_status_word", c_vp(_status[dev].data_ptr()))
     return _status[dev]
+
+
+def status_ptr():
+    """Its address."""
+    p = _status_ptr.get(torch._C._cuda_getDevice())
+    if p is None:
+        p = _status_ptr[torch._C._cuda_getDevice()] = status_buffer().data_ptr()
+    return p
 
 
 _mixer_status = {}

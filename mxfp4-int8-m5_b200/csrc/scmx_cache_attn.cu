@@ -119,22 +119,26 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
 #pragma unroll
     for (int s = 0; s < L::STAGES - 1; ++s) load(warp + s * WARPS, s);
 
-    // query rows, as the B operand: row g of each group of eight
-    auto query = [&](int nt, int s) -> uint2 {
-        const int r = row0 + 8 * nt + g, tok = r / G;
-        if (r >= R) return make_uint2(0, 0);
-        const uint16_t* qp = a.q + (int64_t)(kvh * G + r - tok * G) * a.q_hs + (int64_t)tok * a.q_rs + 16 * s;
-        if constexpr (I8) {      // the four values that one word of codes holds: 0 and 2, 1 and 3
-            const uint2 w = *reinterpret_cast<const uint2*>(qp + 4 * t4);
-            return make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632));
-        }
-        return make_uint2(*reinterpret_cast<const uint32_t*>(qp + 2 * t4), *reinterpret_cast<const uint32_t*>(qp + 8 + 2 * t4));
-    };
+    // query rows, as the B operand: row g of each group of eight (rows past the last are read from row 0 and cleared, so that no load waits for another)
     uint2 qf[NT][KSTEPS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = row0 + 8 * nt + g, rr = r < R ? r : 0, tok = rr / G;
+        const uint16_t* qp = a.q + (int64_t)(kvh * G + rr - tok * G) * a.q_hs + (int64_t)tok * a.q_rs;
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+            if constexpr (I8) qf[nt][s] = *reinterpret_cast<const uint2*>(qp + 16 * s + 4 * t4);
+            else qf[nt][s] = make_uint2(*reinterpret_cast<const uint32_t*>(qp + 16 * s + 2 * t4), *reinterpret_cast<const uint32_t*>(qp + 16 * s + 8 + 2 * t4));
+        }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) qf[nt][s] = query(nt, s);
+        for (int s = 0; s < KSTEPS; ++s) {
+            uint2& w = qf[nt][s];
+            if (I8) w = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632));      // values 0 and 2, 1 and 3 of a word of codes
+            if (row0 + 8 * nt + g >= R) w = make_uint2(0, 0);
+        }
 
     // rows 2 t4 and 2 t4 + 1 of each group: maximum and sum; output: 16 values of the vectors times eight rows
     float o[MT][NT][4], mx[NT][2], sum[NT][2];

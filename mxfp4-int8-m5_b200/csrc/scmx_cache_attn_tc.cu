@@ -10,8 +10,8 @@
 //   warps 8-15    (INT8) codes of a tile from memory to bfloat16 operands, exactly; a position's key scale multiplies its scores, its value scale
 //                 its weights.  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are
 //                 laid out alike, and outputs put back.  Tiles ahead are prefetched into L2
-//   last four     one warp issues all MMAs (it stays converged, one lane issues), one loads key and value tiles by TMA (bfloat16)
-// Registers are shared out by role (setmaxnreg): the softmax holds a row's scores.
+//   last warps    one issues all MMAs (it stays converged, one lane issues), one loads key and value tiles by TMA (bfloat16)
+// INT8: registers are shared out by role (setmaxnreg).
 // Up to 64 query rows leave lanes idle: a tile then holds two or four copies of them, each copy's threads take a half or a quarter of a tile's
 // keys, and their weights for the other keys are zero.  The copies are joined like the streams.  So the softmax of few rows is spread over all
 // threads, and the products, which a memory-bound call has time for, stay whole tiles.
@@ -39,9 +39,9 @@ struct CtSmem {
     static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
     // kfull, kempty [KS], vfull, vempty [VS], scales [CT_SCALES], S, P, O [2], queries
     static constexpr int NBAR = 2 * KS + 2 * VS + (I8 ? CT_SCALES : 0) + 7;
-    // threads, and registers of a thread by role: together no more than the block is launched with
-    static constexpr int THREADS = I8 ? 640 : 384, LAUNCH_REGS = I8 ? 96 : 168, SOFT_REGS = I8 ? 128 : 192, CONV_REGS = 72, MISC_REGS = I8 ? 72 : 120;
-    static_assert(256 * SOFT_REGS + (I8 ? 256 * CONV_REGS : 0) + 128 * MISC_REGS <= THREADS * LAUNCH_REGS, "registers of a block");
+    // threads; INT8: registers of a thread by role, together no more than the block is launched with
+    static constexpr int THREADS = I8 ? 640 : 320, LAUNCH_REGS = 96, SOFT_REGS = 128, CONV_REGS = 72, MISC_REGS = 72;
+    static_assert(256 * SOFT_REGS + 256 * CONV_REGS + 128 * MISC_REGS <= 640 * LAUNCH_REGS, "registers of a block");
     static constexpr int MISC_OFF = BAR_OFF + 8 * NBAR;
     static constexpr int TOTAL = MISC_OFF + 32 + 1024;
     static constexpr int PITCH = D + 4;                                       // outputs of 256 lanes from Q_OFF on, then maxima and sums, in place of operands
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         proxy_fence();
     }
-    constexpr int MISC = I8 ? 16 : 8;        // first of the last four warps: MMAs; the one after it: TMA
+    constexpr int MISC = I8 ? 16 : 8;        // first of the last warps: MMAs; the one after it: TMA
     if (warp == MISC) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     int fail = 0;
 
     if (warp > MISC) {
-        set_regs<false, L::MISC_REGS>();
+        if (I8) set_regs<false, L::MISC_REGS>();
         if (!I8 && warp == MISC + 1 && lane == 0) {
             for (int j = 0; j < ntiles; ++j) {
                 const int key = (int)t0 + 128 * j, ks = j % KS, vs = j % VS;
@@ -136,10 +136,13 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 if (int w = mbar_wait(b_ve + 8 * vs, ((j / VS) & 1) ^ 1, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
                 mbar_expect_tx(b_vf + 8 * vs, KB * CT_TILE);
                 for (int c = 0; c < KB; ++c) tma_load_3d(sbase + L::V_OFF + (vs * KB + c) * CT_TILE, &tmV, c * 128, key, kvh, b_vf + 8 * vs);
+                // the queries first: behind all stages' loads of all multiprocessors they arrive 3 us later
+                if (j == 0)
+                    if (int w = mbar_wait(b_q, 0, abort_flag, wait_ns)) { fail = w == 1 ? 71 : -1; break; }
             }
         }
     } else if (warp == MISC) {
-        set_regs<false, L::MISC_REGS>();
+        if (I8) set_regs<false, L::MISC_REGS>();
         const uint32_t on = elect_lane();
         const uint32_t idesc_s = umma_idesc_bf16(128, 128), idesc_o = umma_idesc_bf16(128, D) | IDESC_B_MN;
         int kt = -1, vt = -1;            // last tiles that were waited for
@@ -179,29 +182,32 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         }
         if (!on) fail = fail > 0 ? -1 : fail;      // one lane reports
     } else if (warp < 8) {
-        set_regs<true, L::SOFT_REGS>();
-        // queries: K-major tiles with the 128-byte swizzle, half a row to a thread; a negative scale is taken by the queries
+        if (I8) set_regs<true, L::SOFT_REGS>();
+        // queries: K-major tiles with the 128-byte swizzle, four values of a row to a lane; a negative scale is taken by the queries
         if (ntiles) {
+            constexpr int LPR = D / 4, RPW = 32 / LPR, PER = ROWS / (8 * RPW);      // lanes of a row, rows of a warp's load, loads of a warp
             const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-            const int ql = tid & 127, half = tid >> 7;
+            const int ql = lane % LPR;
+            constexpr int BATCH = PER < 8 ? PER : 8;       // loads of a warp that are in flight together
+#pragma unroll 1
+            for (int i0 = 0; i0 < PER; i0 += BATCH) {
+                uint2 x[BATCH];
 #pragma unroll
-            for (int t = 0; t < MQ; ++t) {
-                const int r = row0 + t * 128 + ql % RP, qt = r / G;
-                const uint2* p = reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + (r < R ? r - qt * G : 0)) * a.q_hs + (int64_t)(r < R ? qt : 0) * a.q_rs) + half * (D / 8);
-                uint2 x[D / 8];
+                for (int i = 0; i < BATCH; ++i) {          // nothing here waits for a load: rows past the last read row 0
+                    const int r = row0 + ((i0 + i) * 8 + warp) * RPW + lane / LPR, rr = r < R ? r : 0, qt = rr / G;
+                    x[i] = __ldg(reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + rr - qt * G) * a.q_hs + (int64_t)qt * a.q_rs + 4 * ql));
+                }
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) x[i] = p[i];
+                for (int i = 0; i < BATCH; ++i) {
+                    const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR;
+                    uint2 w = I8 ? make_uint2(__byte_perm(x[i].x, x[i].y, 0x5410), __byte_perm(x[i].x, x[i].y, 0x7632)) : x[i];
+                    w.x = row0 + r < R ? w.x ^ flip : 0u;
+                    w.y = row0 + r < R ? w.y ^ flip : 0u;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint2 u = x[2 * i], v = x[2 * i + 1];
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (r < R) {
-                        if constexpr (I8) w = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
-                        else w = make_uint4(u.x, u.y, v.x, v.y);
-                        w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+                    for (int c = 0; c < COPIES; ++c) {
+                        const int to = r + c * RP;
+                        *reinterpret_cast<uint2*>(smem + L::Q_OFF + (to / 128 * KB + ql / 16) * CT_TILE + to % 128 * 128 + ((((ql & 15) >> 1) ^ (to & 7)) << 4) + (ql & 1) * 8) = w;
                     }
-                    const int c = half * (D / 16) + i;
-                    *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * KB + c / 8) * CT_TILE + ql * 128 + (((c & 7) ^ (ql & 7)) << 4)) = w;
                 }
             }
             proxy_fence();
@@ -365,8 +371,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             if (__any_sync(0xffffffffu, w)) fail = w == 1 ? 75 : -1;
             tc_fence_after();
         }
-        // every lane's output to shared memory, then a warp to a row: the states of its copies and streams are joined
-        constexpr int E = D / 32, STATES = MQ == 2 ? 1 : 2 * COPIES;
+        // every lane's output to shared memory, where the states of a row's copies and streams are joined
+        constexpr int STATES = MQ == 2 ? 1 : 2 * COPIES, PIECES = D / 4;
         const bool mine = fail == 0 && units > m;
         float* out = reinterpret_cast<float*>(smem + L::Q_OFF);
         float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
@@ -382,28 +388,65 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 p[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + (I8 ? 2 : 1)]), __uint_as_float(v[4 * i + (I8 ? 1 : 2)]), __uint_as_float(v[4 * i + 3]));
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
         const int rows = units == 0 ? 0 : R - row0 < ROWS ? R - row0 : ROWS;
-        for (int r = warp; r < rows; r += 8) {
-            const int s = lane < STATES ? lane : 0, at = MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r;
-            const float2 z = lane < STATES ? ml[at] : make_float2(-INFINITY, 0.0f);
-            float top = z.x, total = z.y, v[E];
-            ca_join<E, STATES>(STATES, top, total, v, [&](int s, float (&z)[E]) { ca_load<E>(out + (MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r) * L::PITCH + lane * E, z); });
-            if (odd) {                       // new rows' values that are not finite, to a row that sees them
-                const int tk = (row0 + r) / G;
-                for (uint64_t b = (a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull) & odd; b; b &= b - 1) {
-                    const uint16_t* p = static_cast<const uint16_t*>(a.v) + ((int64_t)kvh * a.cap + pos + (__ffsll((long long)b) - 1)) * D + lane * E;
+        const int64_t first = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS;
+        auto state = [](int r, int s) { return MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r; };
+        // a thread to a row: what each of its states is multiplied by (in place of its maximum), the row's maximum and sum
+        if (tid < rows) {
+            float top = -INFINITY, total = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if ((p[e] & 0x7F80u) == 0x7F80u) v[e] += bf16_to_f32(p[e]);
+            for (int s = 0; s < STATES; ++s) top = fmaxf(top, ml[state(tid, s)].x);
+#pragma unroll
+            for (int s = 0; s < STATES; ++s) {
+                float2& z = ml[state(tid, s)];
+                const float f = z.x == -INFINITY ? 0.0f : ex2_approx(z.x - top);
+                total += z.y * f;
+                z.x = f;
+            }
+            if (a.part != nullptr) a.part_ml[first + tid] = make_float2(top, total);
+            ml[tid].y = total;               // (state 0 is row tid itself)
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
+        const float inv_g = 1.0f / (float)G;
+#pragma unroll 1
+        for (int i0 = tid; i0 < rows * PIECES; i0 += 4 * 256) {
+            float4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * 256 < rows * PIECES ? i0 + k * 256 : i0, r = i / PIECES, c = i % PIECES;
+                v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int s = 0; s < STATES; ++s) {
+                    const int at = state(r, s);
+                    const float f = ml[at].x;
+                    float4 x = *reinterpret_cast<const float4*>(out + at * L::PITCH + 4 * c);
+                    if (f == 0.0f) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // nothing seen: the output may not have been written
+                    v[k].x = fmaf(x.x, f, v[k].x); v[k].y = fmaf(x.y, f, v[k].y); v[k].z = fmaf(x.z, f, v[k].z); v[k].w = fmaf(x.w, f, v[k].w);
                 }
             }
-            if (a.part == nullptr) {
-                ca_output<D>(a, kvh, row0 + r, lane, v, total);
-            } else {
-                const int64_t to_row = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS + r;
-                ca_store<E>(a.part + to_row * D + lane * E, v);
-                if (lane == 0) a.part_ml[to_row] = make_float2(top, total);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * 256, r = i / PIECES, c = i % PIECES;
+                if (i >= rows * PIECES) break;
+                const int rr = row0 + r, tk = (int)(((float)rr + 0.5f) * inv_g);      // rr / G: exact, rr is far below 2^20
+                float4& y = v[k];
+                if (odd) {                       // new rows' values that are not finite, to a row that sees them
+                    for (uint64_t b = (a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull) & odd; b; b &= b - 1) {
+                        const uint16_t* p = static_cast<const uint16_t*>(a.v) + ((int64_t)kvh * a.cap + pos + (__ffsll((long long)b) - 1)) * D + 4 * c;
+                        if ((p[0] & 0x7F80u) == 0x7F80u) y.x += bf16_to_f32(p[0]);
+                        if ((p[1] & 0x7F80u) == 0x7F80u) y.y += bf16_to_f32(p[1]);
+                        if ((p[2] & 0x7F80u) == 0x7F80u) y.z += bf16_to_f32(p[2]);
+                        if ((p[3] & 0x7F80u) == 0x7F80u) y.w += bf16_to_f32(p[3]);
+                    }
+                }
+                if (a.part != nullptr) {
+                    *reinterpret_cast<float4*>(a.part + (first + r) * D + 4 * c) = y;
+                } else {
+                    const float total = ml[r].y, inv = total == 0.0f ? 0.0f : 1.0f / total;
+                    *reinterpret_cast<uint2*>(a.out + (int64_t)tk * a.hq * D + (kvh * G + rr - tk * G) * D + 4 * c) =
+                        make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+                }
             }
         }
     } else if (I8) {

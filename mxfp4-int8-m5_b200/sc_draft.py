@@ -69,12 +69,10 @@ def verify_draft(logits, tokens, parents, u=None, temperature=1.0, probs=None):
         _lib.require_here(probs, contiguous=False)
         if probs.shape != logits.shape:
             raise ValueError(f"probs {tuple(probs.shape)} for logits {tuple(logits.shape)}")
-    dev = logits.device
-    rows, count = torch.empty(n, dtype=torch.int32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
-    token = torch.empty(1, dtype=torch.int64, device=dev)
+    rows, count, token = parents.new_empty(n), parents.new_empty(1), tokens.new_empty(1)
     size = _lib.lib().scmx_verify_scratch(n, V)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-    _lib.call("scmx_verify", logits.data_ptr(), int(logits.dtype == torch.float32), max(logits.stride(0), V), tokens.data_ptr(), parents.data_ptr(), _lib.ptr(u),
-              float(temperature), _lib.ptr(probs), 0 if probs is None else max(probs.stride(0), V), n, V, rows.data_ptr(), count.data_ptr(), token.data_ptr(),
+    scratch = tokens.new_empty(size // 8)
+    _lib.call("scmx_verify", logits.data_ptr(), logits.dtype == torch.float32, max(logits.stride(0), V), tokens.data_ptr(), parents.data_ptr(), _lib.ptr(u),
+              temperature, _lib.ptr(probs), 0 if probs is None else max(probs.stride(0), V), n, V, rows.data_ptr(), count.data_ptr(), token.data_ptr(),
               scratch.data_ptr(), size, _lib.stream())
     return rows, count, token

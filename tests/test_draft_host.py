@@ -50,7 +50,7 @@ def test_entry_points_refuse(scmx):
     assert scmx._lib.lib().scmx_kv_append(*append(L=0)) == 0
     for start, n, hk, d, text in ((0, 17, 2, 64, "rows 0"), (-1, 2, 2, 64, "rows -1"), (0, 2, 0, 64, "rows"), (0, 2, 2, 20, "head size")):
         _refused(scmx, "scmx_kv_read", (P, P, P, P, start, n, hk, d, 16, P, P, None), text)
-    layers = (scmx._lib.ScmxKvLayer * 2)()
+    layers = (ctypes.c_void_p * 8)()
     for n, pos, d, text in ((0, 0, 64, "0 rows"), (65, 0, 64, "65 rows"), (4, 13, 64, "rows 13"), (4, 0, 40, "head size"), (4, 0, 64, "layer 0")):
         _refused(scmx, "scmx_kv_keep", (layers, 2, P, n, pos, None, 2, d, 16, 0, None), text)
 

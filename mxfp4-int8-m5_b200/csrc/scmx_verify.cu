@@ -6,10 +6,10 @@
 // Temperature 0: a child is accepted if it is the largest logit of its parent (the lowest index of equal ones), which is also the token.
 //
 // The maxima and sums of all rows are a pass over the logits by the whole device (memory-bound); one cluster then walks the tree, which needs one
-// logit per drafted row.  Where drafts have probabilities, a launch between the two finds what rejections leave of every node with more
-// than one child, a cluster to a node (float32 weights: this mass decides tests whose border a relative error of 1e-6 moves by as much).
-// The last token's weights, sums and cumulative probabilities are float64, made by the walking cluster for its node alone: between 100000
-// neighbours float32 sums would pick another token once in a hundred draws.
+// logit per drafted row.  Where drafts have probabilities, it reads a node's row again when a rejected child has a sibling to be tested on what
+// is left (float32 weights: this mass decides tests whose border a relative error of 1e-6 moves by as much; all such masses ahead, a cluster
+// to a node, took 19 us of the whole device where a pass of the walk takes 3).  The last token's weights, sums and cumulative
+// probabilities are float64: between 100000 neighbours float32 sums would pick another token once in a hundred draws.
 #include <cooperative_groups.h>
 #include "scmx_common.cuh"
 
@@ -19,7 +19,6 @@ namespace scmx {
 
 constexpr int VF_ROWS = 64, VF_THREADS = 256, VF_VECS = 4;                  // first launch: 256 x 4 vectors of 8 logits per CTA
 constexpr int VF_SLICE = VF_THREADS * VF_VECS * 8;
-constexpr int VM_CTAS = 8, VM_THREADS = 512;                                // masses after rejections: a cluster to a node
 constexpr int VW_CTAS = 16, VW_THREADS = 512, VW_WARPS = VW_THREADS / 32;   // walk: a cluster of 16 CTAs, or 8 where the device has no room for one
 constexpr int VW_CACHE = 200 * 1024;                                        // bytes of weights and probabilities that a CTA of it keeps
 
@@ -35,7 +34,6 @@ struct VfArgs {
     const int32_t* parents;
     const float* u;
     VfPart* part;                    // [n, slices]
-    double* masses;                  // [n, 64]: what the first, second, .. rejection leaves of a node
     int32_t *rows, *count;
     int64_t* token;
     int64_t ld, ldp;
@@ -74,8 +72,12 @@ __device__ __forceinline__ void vf_load(const float* row, int v, int V, float fi
     }
 }
 
-// The weight of a logit against its row's maximum in float32, the same in both launches.
-__device__ __forceinline__ float vf_weight(float x, float m, float c) { return exp2f(__fmul_rn(__fsub_rn(x, m), c)); }
+// The weight of a logit against its row's maximum in float32, the same in all launches.
+__device__ __forceinline__ float vf_weight(float x, float m, float c) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fmul_rn(__fsub_rn(x, m), c)));
+    return y;
+}
 
 // Keys order like (value, lower index first); NaN counts as the largest.
 __device__ __forceinline__ unsigned long long vf_key(float f, uint32_t i) {
@@ -179,30 +181,31 @@ __global__ void __launch_bounds__(1024) verify_greedy_kernel(const __grid_consta
 // e^x for x <= 0 in float64, relative error below 1e-13: 2^(k / 64) by a table, e^r of the rest, |r| < ln 2 / 128, by its Taylor series.  The library's function is
 // correct to the last bit and took half of the walk's time.
 __device__ __forceinline__ double vf_exp(double x, const double* table) {
-    if (!(x >= -700.0)) return x != x ? x : 0.0;
     const double big = 6755399441055744.0;                   // 1.5 2^52: adding it rounds to a whole number, whose low bits are those of the sum
     const double t = fma(x, 92.332482616893656877, big);     // 64 / ln 2
     const int k = __double2loint(t);
     const double r = fma(t - big, -0.010830424696249145, x); // ln 2 / 64
     const double p = fma(r, fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0) * table[k & 63];
-    return __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+    const double e = __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+    return x >= -700.0 ? e : x != x ? x : 0.0;               // no branch: eight of these run side by side
 }
 
 // Maximum and sum of a row from its slices, by a warp.
 __device__ __forceinline__ void vf_row_sum(const VfArgs& a, int row, float& m, double& sum) {
     const int lane = threadIdx.x & 31;
-    m = -INFINITY;
-    sum = 0.0;
-    for (int s0 = 0; s0 < a.slices; s0 += 32) {
-        VfPart p;
-        p.sum = 0.0;
-        p.max = -INFINITY;
-        if (s0 + lane < a.slices) p = a.part[(int64_t)row * a.slices + s0 + lane];
-        const float mn = fmaxf(m, warp_max(p.max));
-        const double w = p.max == -INFINITY ? 0.0 : p.sum * (double)vf_weight(p.max, mn, a.c);
-        sum = sum * (m == -INFINITY ? 0.0 : (double)vf_weight(m, mn, a.c)) + warp_sum(w);
-        m = mn;
+    const VfPart* part = a.part + (int64_t)row * a.slices;
+    VfPart p;
+    p.sum = 0.0;
+    p.max = -INFINITY;
+    if (lane < a.slices) p = part[lane];
+    for (int s = lane + 32; s < a.slices; s += 32) {
+        const VfPart z = part[s];
+        const float mn = fmaxf(p.max, z.max);
+        if (mn != -INFINITY) p.sum = p.sum * (double)vf_weight(p.max, mn, a.c) + z.sum * (double)vf_weight(z.max, mn, a.c);
+        p.max = mn;
     }
+    m = warp_max(p.max);
+    sum = warp_sum(p.max == -INFINITY ? 0.0 : p.sum * (double)vf_weight(p.max, m, a.c));
 }
 // A thread's share -> the cluster's sum in every thread; warps' and CTAs' shares stay in warp_part and parts[turn].  Shares are pushed to the other CTAs, so
 // that after the barrier everything is near.  turn alternates: a share is not overwritten before everybody has passed the next barrier.
@@ -222,65 +225,6 @@ __device__ __forceinline__ double vf_reduce(cg::cluster_group& cl, double s, dou
     double t = 0.0;
     for (int r = 0; r < ctas; ++r) t += parts[turn][r];
     return t;
-}
-
-// grid (VM_CTAS, n)
-template <typename T>
-__global__ void __cluster_dims__(VM_CTAS, 1, 1) __launch_bounds__(VM_THREADS) verify_masses_kernel(const __grid_constant__ VfArgs a) {
-    __shared__ double warp_part[VM_THREADS / 32], parts[2][VW_CTAS], sum;
-    __shared__ float max;
-    __shared__ int children;
-    pdl_launch_dependents();
-    pdl_wait();
-    cg::cluster_group cl = cg::this_cluster();
-    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-    if (tid < 32) {
-        int n = 0;
-        for (int c0 = 0; c0 < a.n; c0 += 32) {
-            const int c = c0 + lane;
-            n += __popc(__ballot_sync(0xffffffffu, c > row && c < a.n && a.parents[c] == row));
-        }
-        float m;
-        double s;
-        vf_row_sum(a, row, m, s);
-        if (lane == 0) {
-            children = n;
-            max = m;
-            sum = s;
-        }
-    }
-    __syncthreads();
-    if (children < 2) return;            // the whole cluster: after an only child's rejection nothing is tested
-    cl.sync();                           // shares are pushed to CTAs that run
-    const int nvec = (a.V + 7) / 8, per = (nvec + VM_CTAS - 1) / VM_CTAS, v0 = (int)cl.block_rank() * per, v1 = min(v0 + per, nvec);
-    const T* logits = static_cast<const T*>(a.logits) + (int64_t)row * a.ld;
-    const float* probs = a.probs + (int64_t)row * a.ldp;
-    const float m = max;
-    double left[2] = {sum, 0.0};         // masses before the first and the second rejection; further ones are read back
-    int turn = 0;
-    for (int k = 1; k < children; ++k) {
-        double s = 0.0;
-#pragma unroll 2
-        for (int v = v0 + tid; v < v1; v += VM_THREADS) {
-            float x[8], q[8];
-            vf_load(logits, v, a.V, -INFINITY, x);
-            vf_load(probs, v, a.V, 0.0f, q);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = m == -INFINITY ? 0.0f : fmaxf(fmaf(-q[j], (float)left[0], vf_weight(x[j], m, a.c)), 0.0f);
-            for (int r = 1; r < k; ++r) {
-                const float w = (float)(r == 1 ? left[1] : a.masses[row * VF_ROWS + r - 1]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = fmaxf(fmaf(-q[j], w, x[j]), 0.0f);
-            }
-            s += (double)(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
-        }
-        const double rest = vf_reduce<VM_THREADS / 32>(cl, s, warp_part, parts, turn);
-        if (k == 1) left[1] = rest;
-        if (tid == 0) a.masses[row * VF_ROWS + k - 1] = rest;      // every CTA stores what it will read
-        __syncthreads();
-        if (!(rest > 0.0)) break;        // a rejection that leaves nothing is none, and so are the later ones
-    }
-    cl.sync();                           // nobody leaves while shares may still be pushed to it
 }
 
 template <typename T, bool PROBS>
@@ -307,10 +251,12 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
         const int64_t x = a.tokens[tid];
         tok[tid] = x >= 0 && x < a.V ? (int)x : -1;
     }
-    for (int r = warp; r < a.n; r += VW_WARPS) {
+#pragma unroll
+    for (int i = 0; i < VF_ROWS / VW_WARPS; ++i) {      // side by side: a row's sum is a chain of exchanges
+        const int r = warp + i * VW_WARPS;
         float m;
         double s;
-        vf_row_sum(a, r, m, s);
+        vf_row_sum(a, r < a.n ? r : 0, m, s);
         if (lane == 0) {
             top[r] = m;
             mass[r] = s;
@@ -332,8 +278,39 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
 
     cl.sync();                       // shares are pushed to CTAs that run
 
-    // the walk: every thread takes the same steps
+    const int nvec = (a.V + 7) / 8, w0 = (rank * VW_WARPS + warp) * per, w1 = min(w0 + per, nvec), steps = (per + 31) / 32;      // a warp's vectors of a row
     int node = 0, count = 1, nrej = 0, turn = 0;
+    // the mass that rejections with probabilities leave of the node; left[r]: the mass before rejection r
+    auto rough = [&]() {
+        const T* row = logits + (int64_t)node * a.ld;
+        const float *probs = a.probs + (int64_t)node * a.ldp, m = top[node];
+        double s = 0.0;
+        constexpr int BATCH = 3;         // loads in flight together
+        for (int v = w0 + lane; v < w1; v += 32 * BATCH) {
+            float x[BATCH][8], q[BATCH][8];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                vf_load(row, v + 32 * i < w1 ? v + 32 * i : nvec, a.V, -INFINITY, x[i]);      // (nvec: past the end, all -inf)
+                vf_load(probs, v + 32 * i < w1 ? v + 32 * i : nvec, a.V, 0.0f, q[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i][j] = m == -INFINITY ? 0.0f : vf_weight(x[i][j], m, a.c);
+            for (int r = 0; r < nrej; ++r) {
+                const float l = (float)left[r];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[i][j] = fmaxf(fmaf(-q[i][j], l, x[i][j]), 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) s += (double)(((x[i][0] + x[i][1]) + (x[i][2] + x[i][3])) + ((x[i][4] + x[i][5]) + (x[i][6] + x[i][7])));
+        }
+        return vf_reduce<VW_WARPS>(cl, s, warp_part, parts, turn);
+    };
+
+    // the walk: every thread takes the same steps
     double now = mass[0];            // mass of the node's residual weights
     if (tid == 0) path[0] = 0;
     for (unsigned long long todo = children[0]; todo;) {
@@ -341,7 +318,7 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
         todo &= todo - 1;
         double w = (double)weight[c];
         if (PROBS) {
-            for (int r = 0; r < nrej; ++r) w = fmax(w - (double)prob[c] * (r ? a.masses[node * VF_ROWS + r - 1] : mass[node]), 0.0);
+            for (int r = 0; r < nrej; ++r) w = fmax(w - (double)prob[c] * left[r], 0.0);
         } else {
             for (int r = 0; r < nrej; ++r)
                 if (gone[r] == tok[c]) w = 0.0;
@@ -354,10 +331,14 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
             now = mass[c];
             todo = children[c];
         } else if (PROBS) {
-            const double rest = todo ? a.masses[node * VF_ROWS + nrej] : 1.0;      // the last child's is not tested on
-            if (rest > 0.0) {
-                ++nrej;
-                now = rest;
+            __syncthreads();
+            if (tid == 0) left[nrej] = now;
+            __syncthreads();
+            ++nrej;
+            if (todo) {              // otherwise nothing is tested on what is left
+                const double rest = rough();
+                if (rest > 0.0) now = rest;
+                else --nrej;
             }
         } else if (w > 0.0 && now - w > 0.0) {
             __syncthreads();
@@ -368,88 +349,104 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
         }
     }
 
-    // the last node's weights in float64, its share of a CTA kept in shared memory
-    const int nvec = (a.V + 7) / 8, w0 = (rank * VW_WARPS + warp) * per, w1 = min(w0 + per, nvec), steps = (per + 31) / 32;
-    double* mine = cache + (size_t)warp * steps * 256 + lane;
-    float* mine_q = reinterpret_cast<float*>(cache + (size_t)VW_WARPS * steps * 256) + (size_t)warp * steps * 256 + lane;
-    const float* probs = PROBS ? a.probs + (int64_t)node * a.ldp : nullptr;
+    // the last node's weights in float64; a CTA keeps its share of them, and of the probabilities, in shared memory
     const int tests = nrej;
+    double *mine = cache + (size_t)warp * steps * 256 + lane, *mine_q = mine + (size_t)VW_WARPS * steps * 256;
+    const float* probs = PROBS ? a.probs + (int64_t)node * a.ldp : nullptr;
+    const double m0 = (double)top[node];
     auto first = [&](int v, double (&w)[8]) {        // before any rejection with probabilities
-        float x[8], q[8];
+        float x[8];
         vf_load(logits + (int64_t)node * a.ld, v, a.V, -INFINITY, x);
-        if (PROBS && cached && tests) vf_load(probs, v, a.V, 0.0f, q);
-        const double m = (double)top[node];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = x[j] == -INFINITY ? 0.0 : vf_exp(((double)x[j] - m) * a.cd, table);
+        for (int j = 0; j < 8; ++j) w[j] = x[j] == -INFINITY ? 0.0 : vf_exp(((double)x[j] - m0) * a.cd, table);
         if (!PROBS)
             for (int r = 0; r < tests; ++r)
                 if (gone[r] >> 3 == v)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if ((gone[r] & 7) == j) w[j] = 0.0;
-        if (cached) {
-            const int at = (v - w0) / 32 * 256;
+    };
+    auto reject = [&](double (&w)[8], const double (&q)[8], double mass_before) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                mine[at + j * 32] = w[j];
-                if (PROBS && tests) mine_q[at + j * 32] = q[j];
-            }
+        for (int j = 0; j < 8; ++j) {
+            const double t = fma(-q[j], mass_before, w[j]);
+            w[j] = t > 0.0 ? t : 0.0;
         }
     };
-    auto residual = [&](int v, double (&w)[8]) {     // after nrej of them, once `first` has been through
-        if (!cached) {
-            first(v, w);
+    // the weights after `kept` rejections (masses before them in left[]), of which the last may still be missing in the cache (done < kept), and one more
+    auto residual = [&](int v, int done, int kept, bool more, double (&w)[8]) {
+        const int at = (v - w0) / 32 * 256;
+        double q[8];
+        if (cached) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = mine[at + j * 32];
+            if (PROBS && (done < kept || more))
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = mine_q[at + j * 32];
         } else {
+            first(v, w);
+            done = 0;
+            if (PROBS && (kept || more)) {
+                float y[8];
+                vf_load(probs, v, a.V, 0.0f, y);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = mine[(v - w0) / 32 * 256 + j * 32];
-        }
-        if (PROBS && nrej) {
-            float q[8];
-            if (!cached) vf_load(probs, v, a.V, 0.0f, q);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = mine_q[(v - w0) / 32 * 256 + j * 32];
-            for (int r = 0; r < nrej; ++r) {
-                const double m = left[r];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const double t = fma(-(double)q[j], m, w[j]);
-                    w[j] = t > 0.0 ? t : 0.0;
-                }
+                for (int j = 0; j < 8; ++j) q[j] = (double)y[j];
             }
         }
+        if (PROBS && done < kept) {
+            for (int r = done; r < kept; ++r) reject(w, q, left[r]);
+            if (cached)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mine[at + j * 32] = w[j];
+        }
+        if (PROBS && more) reject(w, q, left[kept]);
     };
     auto sum8 = [](const double (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); };
     double s = 0.0;
 #pragma unroll 2
     for (int v = w0 + lane; v < w1; v += 32) {
         double w[8];
+        float y[8];
+        if (PROBS && cached && tests) vf_load(probs, v, a.V, 0.0f, y);
         first(v, w);
+        if (cached) {
+            const int at = (v - w0) / 32 * 256;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                mine[at + j * 32] = w[j];
+                if (PROBS && tests) mine_q[at + j * 32] = (double)y[j];
+            }
+        }
         s += sum8(w);
     }
     now = vf_reduce<VW_WARPS>(cl, s, warp_part, parts, turn);
+    int kept = 0, done = 0;          // rejections in left[], and in the cached weights
+    bool last = false;               // whether the shares are those after left[kept]
     if (PROBS) {
-        nrej = 0;
         for (int r = 0; r < tests; ++r) {
-            if (tid == 0) left[nrej] = now;
+            if (tid == 0) left[kept] = now;
             __syncthreads();
-            ++nrej;
-            for (;;) {
+            s = 0.0;
+            for (int v = w0 + lane; v < w1; v += 32) {
+                double w[8];
+                residual(v, done, kept, true, w);
+                s += sum8(w);
+            }
+            done = kept;
+            const double rest = vf_reduce<VW_WARPS>(cl, s, warp_part, parts, turn);
+            last = rest > 0.0;
+            if (!last) {             // a rejection that leaves nothing is none, and so are the later ones: the shares are made again without it
                 s = 0.0;
                 for (int v = w0 + lane; v < w1; v += 32) {
                     double w[8];
-                    residual(v, w);
+                    residual(v, done, kept, false, w);
                     s += sum8(w);
                 }
-                const double rest = vf_reduce<VW_WARPS>(cl, s, warp_part, parts, turn);
-                if (rest > 0.0) {
-                    now = rest;
-                    break;
-                }
-                if (nrej == 0) break;
-                --nrej;                  // a rejection that leaves nothing is none: the shares are made again without it
+                now = vf_reduce<VW_WARPS>(cl, s, warp_part, parts, turn);
+                break;
             }
-            if (!(now > 0.0)) break;
+            now = rest;
+            if (r + 1 < tests) ++kept;
         }
     }
     // the owner of the target: the first CTA, warp and element whose cumulative weight exceeds it (the last with any where roundings leave none)
@@ -488,11 +485,11 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
         }
         if (warp == ow) {
             int best = 0;
-            bool done = false;
-            for (int v0 = w0; v0 < w1 && !done; v0 += 32) {
+            bool hit_found = false;
+            for (int v0 = w0; v0 < w1 && !hit_found; v0 += 32) {
                 double w[8];
                 const int v = v0 + lane;
-                if (v < w1) residual(v, w);
+                if (v < w1) residual(v, done, kept, last, w);
                 else
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = 0.0;
@@ -516,7 +513,7 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
                 const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, last >= 0);
                 if (hits) {
                     best = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
-                    done = true;
+                    hit_found = true;
                 } else if (any) {
                     best = __shfl_sync(0xffffffffu, last, 31 - __clz(any));
                 }
@@ -562,7 +559,7 @@ static int launch_walk(const VfArgs& a, cudaStream_t st) {
     cfg.gridDim = dim3(ctas);
     // vectors of a warp, and what a CTA keeps of its share; a larger vocabulary computes it again for every pass
     const int nvec = (a.V + 7) / 8, per = (nvec + ctas * VW_WARPS - 1) / (ctas * VW_WARPS);
-    const int64_t bytes = (int64_t)VW_WARPS * ((per + 31) / 32) * 256 * (PROBS ? 12 : 8);
+    const int64_t bytes = (int64_t)VW_WARPS * ((per + 31) / 32) * 256 * (PROBS ? 16 : 8);
     const int cached = bytes <= VW_CACHE;
     cfg.dynamicSmemBytes = cached ? bytes : 0;
     cfg.numAttrs = g_use_pdl ? 2 : 1;
@@ -579,9 +576,7 @@ static int launch_verify(const VfArgs& a, bool greedy, cudaStream_t st) {
         return SCMX_OK;
     }
     SCMX_PDL_OK("verify_rows_kernel", launch_pdl(verify_rows_kernel<T, false>, grid, dim3(VF_THREADS), 0, st, a));
-    if (a.probs == nullptr) return launch_walk<T, false>(a, st);
-    if (a.n > 2) SCMX_PDL_OK("verify_masses_kernel", launch_pdl(verify_masses_kernel<T>, dim3(VM_CTAS, (unsigned)a.n), dim3(VM_THREADS), 0, st, a));
-    return launch_walk<T, true>(a, st);
+    return a.probs ? launch_walk<T, true>(a, st) : launch_walk<T, false>(a, st);
 }
 
 }  // namespace scmx
@@ -590,7 +585,7 @@ using namespace scmx;
 
 extern "C" int64_t scmx_verify_scratch(int n, int64_t V) {
     if (n < 1 || n > VF_ROWS || V < 1 || V >= (1ll << 30)) return 0;
-    return (int64_t)n * (((V + VF_SLICE - 1) / VF_SLICE) * (int64_t)sizeof(VfPart) + VF_ROWS * 8);
+    return (int64_t)n * ((V + VF_SLICE - 1) / VF_SLICE) * (int64_t)sizeof(VfPart);
 }
 
 extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, float temperature,
@@ -608,7 +603,7 @@ extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int
     SCMX_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= need, SCMX_EINVAL, "verify: %lld bytes of scratch, %lld needed", (long long)scratch_bytes,
                  (long long)need);
     VfArgs a;
-    a.logits = logits; a.probs = greedy ? nullptr : probs; a.tokens = tokens; a.parents = parents; a.u = u; a.part = static_cast<VfPart*>(scratch); a.masses = reinterpret_cast<double*>(a.part + n * ((V + VF_SLICE - 1) / VF_SLICE));
+    a.logits = logits; a.probs = greedy ? nullptr : probs; a.tokens = tokens; a.parents = parents; a.u = u; a.part = static_cast<VfPart*>(scratch);
     a.rows = rows; a.count = count; a.token = token; a.ld = ld; a.ldp = ldp; a.n = n; a.V = (int)V; a.slices = (int)((V + VF_SLICE - 1) / VF_SLICE);
     a.c = greedy ? 1.0f : (float)(1.4426950408889634 / (double)temperature);
     a.cd = greedy ? 1.0 : 1.0 / (double)temperature;

@@ -114,6 +114,13 @@ int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscale, const fl
                   const uint16_t* kn, float eps, int64_t L, int hq, int hk, int d, int full, const float* inv_freq,
                   const float* rope_table, int64_t rope_rows, int64_t pos0, const int32_t* pos_dev, uint16_t* q, int64_t q_head_stride, uint16_t* k, uint16_t* v,
                   int64_t kv_head_stride, int64_t kv_row0, void* stream);
+/* The same with row_pos int32 [L] on the device (or NULL): row r turns as position pos0 + row_pos[r], the place of a drafted row in its tree.
+ * k_scales and v_scales non-null: k and v are the codes of an INT8 cache, written as scmx_kv_append writes the rows that would be stored; head sizes 64,
+ * 128 and 256 on 16-byte aligned buffers, full-width norms of bf16 input with at most 96 heads. */
+int scmx_qkv_norm_rows(const void* src, int src_is_acc, const float* xscale, const float* wscale, const uint16_t* qn, const uint16_t* kn, float eps, int64_t L,
+                       int hq, int hk, int d, int full, const float* inv_freq, const float* rope_table, int64_t rope_rows, int64_t pos0, const int32_t* pos_dev,
+                       const int32_t* row_pos, uint16_t* q, int64_t q_head_stride, void* k, void* v, float* k_scales, float* v_scales, int64_t kv_head_stride,
+                       int64_t kv_row0, void* stream);
 
 /* Batch-1 decode attention: out[h] = softmax(scale * q[h] K^T) V over the first T positions of a KV cache
  * (k_cache, v_cache bf16 [hk, capacity, d]; q bf16 [hq, d]; out bf16 [hq * d]).  T = pos_dev[0] + 1 when pos_dev is

@@ -232,6 +232,17 @@ __device__ __forceinline__ int quant_code(float v, float qi) {
     return (int)fminf(fmaxf(r, -127.0f), 127.0f);
 }
 
+// Scale and factor of a cached vector from the largest magnitude of its bfloat16 values, as their low 15 bits (which order like the values, infinities and NaN
+// last): as quant_scale, but a vector whose 1 / s would overflow is stored as zero, and one that is not finite reads back as NaN.
+__device__ __forceinline__ void kv_scale(uint32_t top, float& s, float& qi) {
+    quant_scale(__uint_as_float(top << 16), s, qi);
+    if (s < 1.17549435e-38f) s = qi = 0.0f;
+    if (top >= 0x7F80u) {
+        s = __uint_as_float(0x7FC00000u);
+        qi = 0.0f;
+    }
+}
+
 // Four quantization codes packed into a word: byte j = int8(rint(v[j] * qi)).  rint is taken by adding 1.5 * 2^23, whose
 // float spacing is exactly 1 (round-half-even), and the low byte of the sum's bit pattern is the two's-complement code;
 // |v * qi| <= 127 by construction of qi, so no clamp is needed.  The product and the sum are rounded separately.

@@ -47,9 +47,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const __grid_cons
 #pragma unroll
             for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             float s, qi;
-            quant_scale(__uint_as_float(top << 16), s, qi);
-            if (s < 1.17549435e-38f) s = qi = 0.0f;                  // 1 / s would overflow: such a vector is stored as zero
-            if (top >= 0x7F80u) { s = __uint_as_float(0x7FC00000u); qi = 0.0f; }      // a value that is not finite: the vector reads back as NaN
+            kv_scale(top, s, qi);
             const int row = first + i * ROWS;
             const int64_t at = pos + row;
             if (row >= a.L || 8 * l >= a.d || at < 0 || at >= a.cap) continue;      // a device-side position beyond the cache: the row is dropped

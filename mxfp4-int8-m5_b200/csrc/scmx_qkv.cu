@@ -15,9 +15,12 @@ struct QkvArgs {
     const uint16_t* kn;       // bf16 [d] or [hk*d]
     const float* inv_freq;    // f32 [d/2] or null: no rotary embedding
     const int32_t* pos_dev;   // null, or one int32 added to pos0 and kv_row0 (a step counter kept on the device)
+    const int32_t* row_pos;   // null, or int32 [L]: row r turns as position pos0 + row_pos[r] (rows of a tree), not pos0 + r
     const float* rope_cs;     // null, or a table f32 [rope_rows, d]: cos (d/2) then sin (d/2) of position * inv_freq
     int64_t rope_rows;
     uint16_t *q, *k, *v;
+    int8_t *kc, *vc;          // INT8 cache instead of k, v: codes and a scale per vector (register form only)
+    float *ks, *vs;
     int64_t q_hs, kv_hs, kv_row0, pos0;
     float eps;
     int hq, hk, d, d_shift, full;
@@ -52,9 +55,9 @@ __global__ void __launch_bounds__(256) qkv_norm_kernel(const QkvArgs a) {
         }
     }
     if (a.inv_freq != nullptr) {
-        const int64_t pos = a.pos0 + step + row;
+        const int64_t pos = a.pos0 + step + (a.row_pos ? (int64_t)a.row_pos[row] : row);
         for (int i = tid; i < half; i += 256) {
-            if (a.rope_cs != nullptr && pos < a.rope_rows) {    // the same values, computed once on the host side
+            if (a.rope_cs != nullptr && pos >= 0 && pos < a.rope_rows) {    // the same values, computed once on the host side
                 cs[i] = a.rope_cs[pos * d + i];
                 sn[i] = a.rope_cs[pos * d + half + i];
             } else {
@@ -166,7 +169,8 @@ __device__ __forceinline__ void widen(const uint32_t (&w)[E / 2], float (&x)[E])
     }
 }
 
-template <bool FROM_ACC, bool FULL, int E, int NT>
+// QUANT: keys and values go to an INT8 cache.
+template <bool FROM_ACC, bool FULL, int E, int NT, bool QUANT>
 __global__ void __launch_bounds__(256) qkv_norm_vec_kernel(const QkvArgs a) {
     constexpr int D = 32 * E, HALF = 16 * E;
     __shared__ double red[8][2];
@@ -186,8 +190,8 @@ __global__ void __launch_bounds__(256) qkv_norm_vec_kernel(const QkvArgs a) {
     const int64_t kv_row = a.kv_row0 + step + row;
     float cs[E], sn[E];
     if (a.inv_freq != nullptr) {
-        const int64_t pos = a.pos0 + step + row;
-        if (a.rope_cs != nullptr && pos < a.rope_rows) {
+        const int64_t pos = a.pos0 + step + (a.row_pos ? (int64_t)a.row_pos[row] : row);
+        if (a.rope_cs != nullptr && pos >= 0 && pos < a.rope_rows) {
 #pragma unroll
             for (int i = 0; i < E; i += 2) {
                 const float2 c = __ldg(reinterpret_cast<const float2*>(a.rope_cs + pos * D + e0 + i));
@@ -309,28 +313,67 @@ __global__ void __launch_bounds__(256) qkv_norm_vec_kernel(const QkvArgs a) {
                     x[j][1][i] = turn ? __fadd_rn(__fmul_rn(n[0][i], sn[i]), __fmul_rn(n[1][i], cs[i])) : n[1][i];
                 }
             }
+            if (QUANT && g >= a.hq) {
+                // the bfloat16 values that a cache would hold, as INT8: s = amax / 127 over the head's 16 lanes
+                const bool key = g < nh;
+                uint32_t w[2][E / 2], top = 0;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < E / 2; ++i) {
+                        w[b][i] = pack_bf16x2(x[j][b][2 * i], x[j][b][2 * i + 1]);
+                        top = max(top, max(w[b][i] & 0x7FFFu, (w[b][i] >> 16) & 0x7FFFu));
+                    }
+                const unsigned half = (lane & 16) ? 0xFFFF0000u : 0x0000FFFFu;
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(half, top, o));
+                float sc, qi;
+                kv_scale(top, sc, qi);
+                const int64_t at = (int64_t)(g - (key ? a.hq : nh)) * a.kv_hs + kv_row;
+                int8_t* codes = (key ? a.kc : a.vc) + at * D + e0;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t c[(E + 3) / 4];
+#pragma unroll
+                    for (int i = 0; i < E / 2; i += 2) {
+                        const uint32_t lo = w[b][i], hi = i + 1 < E / 2 ? w[b][i + 1 < E / 2 ? i + 1 : i] : 0u;
+                        c[i / 2] = qi > 0.0f ? quant4(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), qi) : 0u;
+                    }
+                    if constexpr (E == 2) *reinterpret_cast<uint16_t*>(codes + b * HALF) = (uint16_t)c[0];
+                    else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(codes + b * HALF) = c[0];
+                    else *reinterpret_cast<uint2*>(codes + b * HALF) = make_uint2(c[0], c[1]);
+                }
+                if ((lane & 15) == 0) (key ? a.ks : a.vs)[at] = sc;
+                continue;
+            }
             store_bf16<E>(out, x[j][0]);
             store_bf16<E>(out + HALF, x[j][1]);
         }
     }
 }
 
-template <int E>
+template <int E, bool QUANT>
 static void (*qkv_vec_kernel(bool acc, bool full, int heads))(QkvArgs) {
-    if (!full) return acc ? qkv_norm_vec_kernel<true, false, E, 2> : qkv_norm_vec_kernel<false, false, E, 2>;
+    if (!full) return acc ? qkv_norm_vec_kernel<true, false, E, 2, QUANT> : qkv_norm_vec_kernel<false, false, E, 2, QUANT>;
     if (acc || heads > 96) return nullptr;
-    return heads <= 32 ? qkv_norm_vec_kernel<false, true, E, 2> : heads <= 48 ? qkv_norm_vec_kernel<false, true, E, 3>
-                                                                              : qkv_norm_vec_kernel<false, true, E, 6>;
+    return heads <= 32 ? qkv_norm_vec_kernel<false, true, E, 2, QUANT> : heads <= 48 ? qkv_norm_vec_kernel<false, true, E, 3, QUANT>
+                                                                                     : qkv_norm_vec_kernel<false, true, E, 6, QUANT>;
+}
+template <bool QUANT>
+static void (*qkv_vec_kernel(int d, bool acc, bool full, int heads))(QkvArgs) {
+    return d == 64 ? qkv_vec_kernel<2, QUANT>(acc, full, heads) : d == 128 ? qkv_vec_kernel<4, QUANT>(acc, full, heads)
+           : d == 256 ? qkv_vec_kernel<8, QUANT>(acc, full, heads) : nullptr;
 }
 
 }  // namespace scmx
 
 using namespace scmx;
 
-extern "C" int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscale, const float* wscale, const uint16_t* qn,
-                             const uint16_t* kn, float eps, int64_t L, int hq, int hk, int d, int full, const float* inv_freq,
-                             const float* rope_table, int64_t rope_rows, int64_t pos0, const int32_t* pos_dev, uint16_t* q, int64_t q_head_stride, uint16_t* k, uint16_t* v,
-                             int64_t kv_head_stride, int64_t kv_row0, void* stream) {
+extern "C" int scmx_qkv_norm_rows(const void* src, int src_is_acc, const float* xscale, const float* wscale, const uint16_t* qn,
+                                  const uint16_t* kn, float eps, int64_t L, int hq, int hk, int d, int full, const float* inv_freq,
+                                  const float* rope_table, int64_t rope_rows, int64_t pos0, const int32_t* pos_dev, const int32_t* row_pos, uint16_t* q,
+                                  int64_t q_head_stride, void* k, void* v, float* k_scales, float* v_scales, int64_t kv_head_stride, int64_t kv_row0,
+                                  void* stream) {
     SCMX_REQUIRE(L >= 0 && hq > 0 && hk > 0, SCMX_EINVAL, "qkv_norm: L=%lld hq=%d hk=%d", (long long)L, hq, hk);
     SCMX_REQUIRE(d >= 8 && (d & (d - 1)) == 0, SCMX_EINVAL, "qkv_norm: head size %d must be a power of two >= 8", d);
     SCMX_REQUIRE(q_head_stride >= L && kv_head_stride >= kv_row0 + L && kv_row0 >= 0 && pos0 >= 0, SCMX_EINVAL,
@@ -339,13 +382,16 @@ extern "C" int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscal
     SCMX_REQUIRE(!src_is_acc || (xscale != nullptr && wscale != nullptr), SCMX_EINVAL, "qkv_norm: int32 input needs xscale and wscale");
     SCMX_REQUIRE(src && qn && kn && q && k && v, SCMX_EINVAL, "qkv_norm: null buffer");
     const int64_t ntot = (int64_t)(hq + 2 * hk) * d;
+    const bool quant = k_scales != nullptr || v_scales != nullptr;
+    SCMX_REQUIRE(!quant || (k_scales && v_scales), SCMX_EINVAL, "qkv_norm: scales of keys and values, or neither");
     const size_t smem = (size_t)ntot * 4 + (size_t)(hq + hk) * 4 + (size_t)d * 4;
     SCMX_REQUIRE(smem <= 48 * 1024, SCMX_ELIMIT, "qkv_norm: a row of %lld values does not fit the 48 KB of shared memory", (long long)ntot);
     if (L == 0) return SCMX_OK;
     QkvArgs a;
-    a.src = src; a.xscale = xscale; a.wscale = wscale; a.qn = qn; a.kn = kn; a.inv_freq = inv_freq; a.pos_dev = pos_dev;
+    a.src = src; a.xscale = xscale; a.wscale = wscale; a.qn = qn; a.kn = kn; a.inv_freq = inv_freq; a.pos_dev = pos_dev; a.row_pos = row_pos;
     a.rope_cs = rope_table; a.rope_rows = rope_table ? rope_rows : 0;
-    a.q = q; a.k = k; a.v = v;
+    a.q = q; a.k = quant ? nullptr : static_cast<uint16_t*>(k); a.v = quant ? nullptr : static_cast<uint16_t*>(v);
+    a.kc = quant ? static_cast<int8_t*>(k) : nullptr; a.vc = quant ? static_cast<int8_t*>(v) : nullptr; a.ks = k_scales; a.vs = v_scales;
     a.q_hs = q_head_stride; a.kv_hs = kv_head_stride; a.kv_row0 = kv_row0; a.pos0 = pos0;
     a.eps = eps; a.hq = hq; a.hk = hk; a.d = d; a.full = full ? 1 : 0;
     a.d_shift = 0;
@@ -355,8 +401,8 @@ extern "C" int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscal
     const void* bufs[] = {src, qn, kn, q, k, v, rope_table};
     bool aligned = true;
     for (const void* p : bufs) aligned = aligned && ((uintptr_t)p & 15) == 0;
-    void (*vec)(QkvArgs) = !aligned ? nullptr : d == 64 ? qkv_vec_kernel<2>(src_is_acc, full, hq + 2 * hk)
-                           : d == 128 ? qkv_vec_kernel<4>(src_is_acc, full, hq + 2 * hk) : d == 256 ? qkv_vec_kernel<8>(src_is_acc, full, hq + 2 * hk) : nullptr;
+    void (*vec)(QkvArgs) = !aligned ? nullptr : quant ? qkv_vec_kernel<true>(d, src_is_acc, full, hq + 2 * hk) : qkv_vec_kernel<false>(d, src_is_acc, full, hq + 2 * hk);
+    SCMX_REQUIRE(!quant || vec != nullptr, SCMX_ELIMIT, "qkv_norm: no INT8 form for head size %d and these buffers", d);
     if (vec != nullptr) {
         SCMX_PDL_OK("qkv_norm_vec_kernel", launch_pdl(vec, dim3((unsigned)L), dim3(256), 0, (cudaStream_t)stream, a));
         return SCMX_OK;
@@ -366,4 +412,12 @@ extern "C" int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscal
     else
         SCMX_PDL_OK("qkv_norm_kernel", launch_pdl(qkv_norm_kernel<false>, dim3((unsigned)L), dim3(256), smem, (cudaStream_t)stream, a));
     return SCMX_OK;
+}
+
+extern "C" int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscale, const float* wscale, const uint16_t* qn,
+                             const uint16_t* kn, float eps, int64_t L, int hq, int hk, int d, int full, const float* inv_freq,
+                             const float* rope_table, int64_t rope_rows, int64_t pos0, const int32_t* pos_dev, uint16_t* q, int64_t q_head_stride, uint16_t* k, uint16_t* v,
+                             int64_t kv_head_stride, int64_t kv_row0, void* stream) {
+    return scmx_qkv_norm_rows(src, src_is_acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, inv_freq, rope_table, rope_rows, pos0, pos_dev, nullptr, q,
+                              q_head_stride, k, v, nullptr, nullptr, kv_head_stride, kv_row0, stream);
 }

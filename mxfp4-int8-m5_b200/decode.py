@@ -16,6 +16,9 @@ the phases of a layer as packets instead of across kernel boundaries, each CTA r
 shared memory, and weights stream ahead of the phases.  Same bits as the chain of kernels; used where its limits
 hold (head size 128, widths multiples of 1024 up to 6144, shares of rows that fit the multiprocessors) and attention="kernel".
 
+DecodeDraft takes several tokens a step: a tree of drafted tokens runs through the prompt path as rows behind the cache's end, the target's probabilities
+decide which of them are kept (speculative decoding).  The caches of all W4A8 decoders may be INT8 (make_cache(dtype=torch.int8)).
+
 DecodeHybrid is the same for hybrid decoders (fused_hybrid.FusedHybrid): GEMVs on bfloat16 or float32 weights with the mixers'
 one-token kernels between them, float32 activations."""
 import ctypes
@@ -24,7 +27,9 @@ import numpy as np
 import torch
 
 from . import _lib
+from . import sc_cache as C
 from . import sc_decode as G
+from . import sc_draft as D
 from . import sc_kernels as S
 from . import hybrid_mixers as MX
 from . import sc_mixers as X
@@ -51,6 +56,11 @@ class _Decoder:
         return self.attn is not None
 
     def _attend(self, at, c, q, k, v, pos_dev):
+        if k is None:                                         # an INT8 cache
+            if self.attn is not None and C.attention_supported(q.shape[0], *c.k.shape[::2]):
+                return C.cache_attention(q, c, at.scale, pos_dev=pos_dev)
+            assert pos_dev is None, "a device-side position needs attention='kernel'"
+            return self.f.sdpa(q, *C.kv_read(c, 0, c.offset + 1), at.scale, False)
         if self.attn is not None:
             return self.attn(q, c, at.scale, n_pos=None if pos_dev is not None else c.offset + 1, pos_dev=pos_dev)
         assert pos_dev is None, "a device-side position needs attention='kernel'"
@@ -194,7 +204,7 @@ class DecodeQwen3(_Decoder):
     def _step(self, tok, cache, pos_dev):
         f, a = self.f, self.args
         S.set_format(f.fmt)
-        if self.persistent:
+        if self.persistent and cache[0].k.dtype == torch.bfloat16:      # an INT8 cache takes the chain of kernels
             return self._step_persistent(tok, cache, pos_dev)
         hq, hk, d, eps = a.num_attention_heads, a.num_key_value_heads, a.head_dim, f.eps
         h = self.model.model.embed_tokens(tok)[0]             # [1, D]
@@ -253,6 +263,97 @@ class DecodeOlmoe(_Decoder):
             else:
                 h = M_.moe_combine(yd, self.pos, scores, h, pn, eps, 1, quant=False)[0]
         return self.head((S.rmsnorm_quant_n(h, self.model.model.norm.weight, eps, 1)[2] if out is None else out)[None])
+
+
+class LookupDraft:
+    """Drafts without a model: continuations of earlier places of the text that end in the same tokens.  A call takes the tokens so far and the most rows that may
+    be drafted, and returns (tokens, parents) of a tree whose row 0 is the last token: up to `places` latest places that share the last `match` (or
+    fewer) tokens, `length` tokens from each, equal beginnings shared."""
+
+    def __init__(self, match=3, length=8, places=2):
+        assert match >= 1 and length >= 1 and places >= 1
+        self.match, self.length, self.places = match, length, places
+
+    def __call__(self, text, most):
+        rows, parents, children = [text[-1]], [-1], {}
+        for m in range(min(self.match, len(text) - 1), 0, -1):
+            tail, found = text[-m:], 0
+            for i in range(len(text) - m - 1, -1, -1):
+                if text[i:i + m] != tail:
+                    continue
+                at = 0
+                for t in text[i + m:i + m + self.length]:
+                    nxt = children.get((at, t))
+                    if nxt is None:
+                        if len(rows) >= most:
+                            return rows, parents
+                        nxt = children[at, t] = len(rows)
+                        rows.append(t)
+                        parents.append(at)
+                    at = nxt
+                found += 1
+                if found == self.places:
+                    break
+            if found:
+                break
+        return rows, parents
+
+
+class DecodeDraft:
+    """Speculative decoding over a FusedQwen3 or FusedOlmoe: `propose` drafts a tree of tokens, one pass of the model reads all its rows, and verify_draft
+    keeps a path of them and draws the token after it, distributed as the model alone would draw (greedy at temperature 0).
+
+    propose(tokens so far, most rows) -> (tokens, parents) or (tokens, parents, probs): sc_draft.DraftTree's lists with row 0 the last token, and probs float32
+    [rows, vocabulary] on the device where children were drawn from them (row i: what row i's children were drawn from)."""
+
+    def __init__(self, fused, propose=None):
+        a = fused.args
+        if not C.attention_supported(a.num_attention_heads, a.num_key_value_heads, a.head_dim):
+            raise ValueError(f"attention of drafted rows: head size {a.head_dim} (64 or 128)")
+        self.f, self.propose = fused, propose or LookupDraft()
+        self.dev = fused.inv_freq.device
+
+    @torch.no_grad()
+    def read(self, tokens, tree, cache):
+        """Logits [n, V] after every row of a tree (tokens int64 [n]); its rows are behind the cache's end."""
+        h = self.f.hidden(tokens.view(1, -1), cache, tree)
+        return self.f.logits(h)[0]
+
+    @torch.no_grad()
+    def keep(self, cache, rows, count):
+        """The accepted rows (verify_draft's list) become the cache's next ones; count: how many, on the host."""
+        C.kv_keep(cache, rows)
+        for c in cache:
+            c.offset += count
+
+    @torch.no_grad()
+    def step(self, text, cache, temperature=0.0, u=None, most=D.MAX_ROWS):
+        """One pass: text (list of ids, the last one not in the cache yet) -> the tokens that it adds, at least one.  u float32 [64]: random numbers in [0, 1)."""
+        assert cache[0].offset + 1 <= cache[0].capacity, "KV cache capacity exceeded"
+        tokens, parents, *probs = self.propose(text, max(1, min(most, D.MAX_ROWS, cache[0].capacity - cache[0].offset)))
+        tree, tok = D.DraftTree(parents, self.dev), torch.tensor(tokens, dtype=torch.int64, device=self.dev)
+        n = len(tree)
+        assert tok.numel() == n and tokens[0] == text[-1], "a tree's first row is the last token"
+        logits = self.read(tok, tree, cache)
+        rows, count, token = D.verify_draft(logits, tok, tree.parents, None if u is None else u[:n], temperature, probs[0] if probs else None)
+        path, last = rows.tolist(), int(token)
+        path = [r for r in path if r >= 0]
+        self.keep(cache, rows, len(path))
+        return [tokens[r] for r in path[1:]] + [last]
+
+    @torch.no_grad()
+    def generate(self, tok, cache, n, text=(), temperature=0.0, generator=None):
+        """n tokens after `tok` (int [1, 1]), as _Decoder.generate; text: the tokens before it, which proposals may look into.  Returns int64 [n]; the cache advances
+        by n positions.  temperature > 0 draws from `generator` (torch.Generator on the device, or None)."""
+        assert cache[0].offset + n <= cache[0].capacity, "KV cache capacity exceeded"
+        text = list(text) + [int(tok)]
+        start, have = cache[0].offset, len(text)
+        while len(text) - have < n:
+            left = n - (len(text) - have)
+            u = torch.rand(D.MAX_ROWS, device=self.dev, generator=generator) if temperature else None
+            text += self.step(text, cache, temperature, u, left)      # a pass of `left` rows adds at most as many tokens
+        assert cache[0].offset == start + n
+        return torch.tensor(text[have:], dtype=torch.int64, device=self.dev)
 
 
 def _row(row, in_parts):

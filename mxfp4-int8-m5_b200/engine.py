@@ -1,7 +1,9 @@
 """Serving loop around a registered model (registry.Bundle): requests own a cache from a pool, a step feeds each of its requests
 the next tokens of its sequence - a portion of a prompt through the prefill path, a single token through the decode path - and
-a finished request returns its cache.  generate() is greedy decoding of one request."""
+a finished request returns its cache.  generate() is greedy decoding of one request, token by token or with drafts."""
 import torch
+
+from . import decode as DEC
 
 
 class CachePool:
@@ -23,9 +25,11 @@ class CachePool:
 
 
 class Engine:
-    def __init__(self, bundle, max_tokens, device="cuda"):
+    def __init__(self, bundle, max_tokens, device="cuda", cache_dtype=None):
+        """cache_dtype: torch.int8 for caches quantized as they are written (W4A8 decoders), None for the model's type."""
         self.bundle, self.device = bundle, device
-        self.pool = CachePool(bundle.prefill.make_cache, max(1, max_tokens))
+        make = bundle.prefill.make_cache
+        self.pool = CachePool(make if cache_dtype is None else lambda capacity: make(capacity, cache_dtype), max(1, max_tokens))
         self.live = {}
 
     def start(self, rid):
@@ -60,13 +64,16 @@ class Engine:
             self.finish(rid)
         return out
 
-    def generate(self, prompt, n, rid="generate"):
-        """n tokens after `prompt` (list of ids), greedy: the prompt through step(), then the decoder's captured graph."""
+    def generate(self, prompt, n, rid="generate", draft=None):
+        """n tokens after `prompt` (list of ids), greedy: the prompt through step(), then the decoder's captured graph, or, with draft (a proposal as
+        decode.DecodeDraft takes it, for instance decode.LookupDraft()), passes over trees of drafted tokens."""
         assert n >= 1 and len(prompt) + n - 1 <= self.pool.capacity, "prompt and continuation exceed the cache"
         logits = self.step([(rid, prompt, [len(prompt) - 1])])[0]
         first = logits[-1].argmax().reshape(1, 1)
         out = [int(first)]
-        if n > 1:
+        if n > 1 and draft is not None:
+            out += DEC.DecodeDraft(self.bundle.prefill, draft).generate(first, self.live[rid], n - 1, prompt).tolist()
+        elif n > 1:
             out += self.bundle.decode.generate(first, self.live[rid], n - 1).tolist()
         self.finish(rid)
         return out

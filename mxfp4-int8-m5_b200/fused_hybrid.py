@@ -133,8 +133,8 @@ class FusedHybrid:
         parts = [self._portion(t, cache) for t in ids.reshape(-1).contiguous().split(self.portion)]
         return (parts[0] if len(parts) == 1 else torch.cat(parts))[None]
 
-    def make_cache(self, capacity=4096):
-        return HM.make_prompt_cache(self.model, capacity)
+    def make_cache(self, capacity=4096, dtype=None):
+        return HM.make_prompt_cache(self.model, capacity, dtype=dtype)
 
     def logits(self, h):
         """h [1, L, W] -> float32 [1, L, V]."""

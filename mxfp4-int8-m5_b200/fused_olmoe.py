@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from . import host_model as HM
 from . import packed_io
+from . import sc_cache as C
 from . import sc_decode as G
 from . import sc_format as F
 from . import sc_kernels as S
@@ -59,6 +60,8 @@ def pack_olmoe(model, cache_path=None, fmt=F.DEFAULT, on_device=False):
 
 
 class FusedOlmoe:
+    _tree = None          # the draft tree whose rows are read (hidden)
+
     def __init__(self, model, flat, tile_gu=None, tile_d=None, bk=None, two_pass="auto", sort="count", compiled=True):
         """model: host_model.CausalLM (num_experts > 0) on the GPU; flat: pack_olmoe's dict.  Prompts whose average expert has fewer than
         MoeBlock.FUSED_BELOW (480) rows run the grouped GEMMs on the packed weights; from there on, and with two_pass=True, the experts are decoded to INT8
@@ -186,16 +189,14 @@ class FusedOlmoe:
     def _hidden_f4(self, h, cache, L):
         """The blocks on digit planes and the final norm: same bits as the products from INT8."""
         a = self.args
-        H, d, D, E, Fi, nl = a.num_attention_heads, a.head_dim, a.hidden_size, a.num_experts, a.intermediate_size, len(self.layers)
+        D, E, Fi, nl = a.hidden_size, a.num_experts, a.intermediate_size, len(self.layers)
         R = L * a.num_experts_per_tok
         dig, xs = S.quant_digits(h, self.layers[0][0].input_layernorm.weight, self.eps)
         for i, (layer, ws, ex) in enumerate(self.layers):
             at, c, wq, wo = layer.self_attn, cache[i], ws["qkv"], ws["o"]
             fq, fo, fg, fd = M_.f4_factors((wq.bcodes, 1, wq.N, wq.K), (wo.bcodes, 1, wo.N, wo.K), (ex["gu"][1], E, 2 * Fi, D), (ex["down"][1], E, D, Fi))
             y = S.mm_f4(dig, wq.codes, fq, xs, wq.wscale, 1)
-            q, kk, v = S.qkv_fullnorm_y(y, at.q_norm.weight, at.k_norm.weight, self.eps, L, H, d, rope=(self.inv_freq, c.offset, self.rope_cs), cache=c)
-            c.offset += L
-            dig, xs = attend_quant(self.sdpa, q, kk, v, at.scale, L, digits=True)
+            dig, xs = self._attend(at, c, y, L, L, digits=True)
             h = S.mm_f4(dig, wo.codes, fo, xs, wo.wscale, 2, res=h)
             xq, xs, xn = S.rmsnorm_quant_n(h, layer.post_attention_layernorm.weight, self.eps, L)
             inds, scores = self.route(layer, xn, L)
@@ -209,6 +210,20 @@ class FusedOlmoe:
             nn = self.model.model.norm.weight if last else self.layers[i + 1][0].input_layernorm.weight
             h, dig, xs, xn = M_.combine_norm(yd, pos, scores, h, nn, self.eps, quant=False if last else "digits", normed=last)
         return xn
+
+    def _attend(self, at, c, y, L, Mp, digits=False):
+        """INT8 rows (or digit planes) of the attention output from the q|k|v rows y, whose keys and values go to the cache."""
+        a = self.args
+        tree = self._tree
+        q, k, v = S.qkv_fullnorm_y(y, at.q_norm.weight, at.k_norm.weight, self.eps, L, a.num_attention_heads, a.head_dim,
+                                   rope=(self.inv_freq, c.offset, self.rope_cs), cache=c, row_pos=None if tree is None else tree.depths)
+        if tree is not None:                                  # the rows stay behind the cache's end until some are kept
+            o = C.cache_attention(q, c, at.scale, tree.mask)
+            return S.quant_digits(o) if digits else S.act_quant(o, Mp)
+        c.offset += L
+        if k is None:                                         # an INT8 cache: what it holds
+            k, v = C.kv_read(c)
+        return attend_quant(self.sdpa, q, k, v, at.scale, Mp, digits)
 
     def experts(self, ex, xq, xs, inds, L, decoded=None):
         """INT8 rows + routing -> (sorted expert outputs yd bf16 [R, D], pos).  decoded: (gu8, dn8) INT8 copies of this
@@ -237,9 +252,20 @@ class FusedOlmoe:
         return yd, pos, (xq_s, xs_s, act, xq2, xs2, e_sorted)
 
     @torch.no_grad()
-    def hidden(self, ids, cache):
+    def hidden(self, ids, cache, tree=None):
+        """Final normed hidden states [1, L, D] for ids [1, L]; tree (sc_draft.DraftTree): as in FusedQwen3.hidden."""
+        if tree is None:
+            return self._hidden(ids, cache)
+        assert len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
+        self._tree = tree
+        try:
+            return self._hidden(ids, cache)
+        finally:
+            self._tree = None
+
+    def _hidden(self, ids, cache):
         a = self.args
-        H, d, D = a.num_attention_heads, a.head_dim, a.hidden_size
+        D = a.hidden_size
         h = self.model.model.embed_tokens(ids)[0]
         L = h.shape[0]
         if L > 0 and self._f4(L):
@@ -263,10 +289,7 @@ class FusedOlmoe:
                 self._decode_experts(i + 1)                    # under this layer's attention and GEMMs
             wq, wo = ws["qkv"], ws["o"]
             y = S.mm_epi(xq, wq.unpack(), xs, wq.wscale, 1)
-            q, kk, v = S.qkv_fullnorm_y(y, at.q_norm.weight, at.k_norm.weight, self.eps, L, H, d,
-                                        rope=(self.inv_freq, c.offset, self.rope_cs), cache=c)
-            c.offset += L
-            xq, xs = attend_quant(self.sdpa, q, kk, v, at.scale, Mp)
+            xq, xs = self._attend(at, c, y, L, Mp)
             h = S.mm_epi(xq, wo.unpack(), xs, wo.wscale, 2, res=h)
             xq, xs, xn = S.rmsnorm_quant_n(h, layer.post_attention_layernorm.weight, self.eps)
             inds, scores = self.route(layer, xn, L)
@@ -287,8 +310,9 @@ class FusedOlmoe:
         xn = S.rmsnorm_quant_n(h, self.model.model.norm.weight, self.eps, Mp)[2]
         return xn[:L][None]
 
-    def make_cache(self, capacity=4096):
-        return HM.make_prompt_cache(self.model, capacity)
+    def make_cache(self, capacity=4096, dtype=None):
+        """dtype=torch.int8: keys and values quantized as they are written (host_model.QuantKVCache)."""
+        return HM.make_prompt_cache(self.model, capacity, dtype=dtype)
 
     def logits(self, h):
         return G.head_product(self.model)(h) if h.dim() == 3 and h.shape[:2] == (1, 1) else self.model.head(h)

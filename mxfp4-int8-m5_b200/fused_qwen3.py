@@ -19,6 +19,7 @@ import torch
 from . import fused_dense as FD
 from . import host_model as HM
 from . import packed_io
+from . import sc_cache as C
 from . import sc_decode as G
 from . import sc_format as F
 from . import sc_kernels as S
@@ -82,6 +83,8 @@ def tiles_for(M):
 
 
 class FusedQwen3:
+    _tree = None          # the draft tree whose rows are read (hidden)
+
     def __init__(self, model, packed, resident=False, overlap=True, epilogue="gemm", compiled=True, fmt=None, rot=False,
                  fuse_rope=True):
         """model: host_model.CausalLM on the GPU; packed: {"layers.{i}.{path}": (codes, bcodes, wscale)}.  resident keeps the
@@ -152,13 +155,19 @@ class FusedQwen3:
     def _qkv(self, at, c, src, xs, ws, L):
         a = self.args
         hq, hk, d = a.num_attention_heads, a.num_key_value_heads, a.head_dim
-        kw = dict(rope=(self.inv_freq, c.offset, self.rope_cs), cache=c) if self.fuse_rope else {}
+        kw = dict(rope=(self.inv_freq, c.offset, self.rope_cs), cache=c) if self.fuse_rope or self._tree is not None else {}
+        if self._tree is not None:
+            kw["row_pos"] = self._tree.depths
         if src.dtype == torch.int32:
             q, k, v = S.qkv_epilogue_headnorm(src, xs, ws, at.q_norm.weight, at.k_norm.weight, self.eps, L, hq, hk, d, **kw)
         else:
             q, k, v = S.qkv_headnorm_y(src, at.q_norm.weight, at.k_norm.weight, self.eps, L, hq, hk, d, **kw)
+        if self._tree is not None:                            # the rows stay behind the cache's end until some are kept
+            return q, k, v
         if self.fuse_rope:
             c.offset += L
+            if k is None:                                     # an INT8 cache: what it holds
+                k, v = C.kv_read(c)
         else:
             q, k = HM.rope(q, self.inv_freq, c.offset), HM.rope(k, self.inv_freq, c.offset)
             k, v = c.update_and_fetch(k, v)
@@ -167,6 +176,9 @@ class FusedQwen3:
     def _attention(self, i, at, c, src, xs, ws, L, Mp):
         """-> attention output (None unless it is recorded), its INT8 rows and their scales."""
         q, k, v = self._qkv(at, c, src, xs, ws, L)
+        if self._tree is not None:
+            o = C.cache_attention(q, c, at.scale, self._tree.mask)
+            return (o, *self.act_q(o, Mp))
         own = type(self).act_q is not _ACT_Q or "act_q" in self.__dict__      # a quantizer of the caller's: it wants whole rows
         if own or self.rot is True or (self.record is not None and i in self.record_layers):
             o = self.sdpa(q, k, v, at.scale, True)
@@ -200,15 +212,30 @@ class FusedQwen3:
             mm = lambda g, dig, xs, epi, res=None: S.mm_f4(dig, ws[g].codes, fac[g], xs, ws[g].wscale, epi, res)      # noqa: E731
             dig, xs = S.quant_digits(h, layer.input_layernorm.weight, self.eps)
             q, k, v = self._qkv(at, cache[i], mm("qkv", dig, xs, 1), None, None, L)
-            h = mm("o", *attend_quant(self.sdpa, q, k, v, at.scale, L, digits=True), 2, h)
+            if self._tree is None:
+                rows = attend_quant(self.sdpa, q, k, v, at.scale, L, digits=True)
+            else:
+                rows = S.quant_digits(C.cache_attention(q, cache[i], at.scale, self._tree.mask))
+            h = mm("o", *rows, 2, h)
             act = mm("gu", *S.quant_digits(h, layer.post_attention_layernorm.weight, self.eps), 3)
             h = mm("down", *S.quant_digits(act), 2, h)
         return h
 
     # ---- prefill ------------------------------------------------------------------------------------------------------
     @torch.no_grad()
-    def hidden(self, ids, cache):
-        """Final normed hidden states [1, L, D] for prompt ids [1, L] (prefill into a fresh or offset cache)."""
+    def hidden(self, ids, cache, tree=None):
+        """Final normed hidden states [1, L, D] for prompt ids [1, L] (prefill into a fresh or offset cache).  tree (sc_draft.DraftTree): the ids are its rows,
+        each of which sees the cache and its ancestors; their keys and values are written behind the cache's end, which does not move (sc_cache.kv_keep)."""
+        if tree is None:
+            return self._hidden(ids, cache)
+        assert len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
+        self._tree = tree
+        try:
+            return self._hidden(ids, cache)
+        finally:
+            self._tree = None
+
+    def _hidden(self, ids, cache):
         S.set_format(self.fmt)
         h = self.model.model.embed_tokens(ids)[0]
         L = h.shape[0]
@@ -286,8 +313,9 @@ class FusedQwen3:
                 h = S.res_epilogue(acc, xs, ws["down"].wscale, h)
         return h
 
-    def make_cache(self, capacity=4096):
-        return HM.make_prompt_cache(self.model, capacity)
+    def make_cache(self, capacity=4096, dtype=None):
+        """dtype=torch.int8: keys and values quantized as they are written (host_model.QuantKVCache)."""
+        return HM.make_prompt_cache(self.model, capacity, dtype=dtype)
 
     def logits(self, h):
         return G.head_product(self.model)(h) if h.dim() == 3 and h.shape[:2] == (1, 1) else self.model.head(h)

@@ -567,11 +567,17 @@ class HybridLM:
         return self
 
 
-def make_prompt_cache(model, capacity, device=None):
+def make_prompt_cache(model, capacity, device=None, dtype=None):
+    """A cache per layer.  dtype: torch.int8 for decoders whose layers hold keys and values in QuantKVCache, otherwise the model's."""
     a = model.args
     if isinstance(model, HybridLM):
+        if dtype not in (None, model.dtype):
+            raise ValueError(f"caches of {dtype} for a hybrid decoder in {model.dtype}")
         device = device or model.device
         caches = [MIXERS[e.type][1](e.mixer, capacity, device, model.dtype) for e in a.layers]
         return caches + [TokenCache(capacity, device)] if a.bigram else caches
     device = device or model.model.embed_tokens.weight.device
-    return [KVCache(a.num_key_value_heads, a.head_dim, capacity, device) for _ in model.model.layers]
+    if dtype not in (None, torch.bfloat16, torch.int8):
+        raise ValueError(f"caches of {dtype}: bfloat16 or int8")
+    kind = QuantKVCache if dtype == torch.int8 else KVCache
+    return [kind(a.num_key_value_heads, a.head_dim, capacity, device) for _ in model.model.layers]

@@ -32,6 +32,19 @@ def draft_depths(parents):
     return out
 
 
+class DraftTree:
+    """A tree's parents, and what the kernels read of it, on the device: parents int32 [n], mask (draft_mask) and depths int32 [n] (draft_depths)."""
+    __slots__ = ("list", "parents", "mask", "depths")
+
+    def __init__(self, parents, device="cuda"):
+        self.list = check_tree(parents)
+        self.mask = draft_mask(self.list, device)
+        self.parents, self.depths = torch.tensor([self.list, draft_depths(self.list)], dtype=torch.int32, device=device).unbind()
+
+    def __len__(self):
+        return len(self.list)
+
+
 def _rows(x, what, dtypes):
     if x.dim() != 2 or x.dtype not in dtypes:
         raise ValueError(f"{what} {tuple(x.shape)} {x.dtype}: [rows, vocabulary], {' or '.join(map(str, dtypes))}")

@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from . import sc_cache as C
 from . import sc_format as F
 
 TM, TN, NSG, GROUP_M = 128, 256, 4, 8   # M tile of the GEMM kernel (row padding unit); the rest are informational
@@ -267,7 +268,7 @@ def rope_table(inv_freq, rows):
     return torch.cat([torch.cos(ang), torch.sin(ang)], 1).float().contiguous()
 
 
-def _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, cache, pos_dev=None):
+def _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, cache, pos_dev=None, row_pos=None):
     _lib.require_cuda(src, xscale, wscale, qn, kn)
     ntot = (hq + 2 * hk) * d
     assert src.shape[1] == ntot and src.shape[0] >= L and src.is_contiguous()
@@ -276,6 +277,7 @@ def _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, cache,
     inv_freq, pos0 = (rope[0], rope[1]) if rope is not None else (None, 0)
     table = rope[2] if rope is not None and len(rope) > 2 else None      # optional rope_table(...) of the same inv_freq
     q = torch.empty((hq, L, d), dtype=torch.bfloat16, device=src.device)
+    quant = cache is not None and cache.k.dtype == torch.int8
     if cache is None:
         k = torch.empty((hk, L, d), dtype=torch.bfloat16, device=src.device)
         v = torch.empty_like(k)
@@ -283,30 +285,39 @@ def _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, cache,
     else:
         kbuf, vbuf, cap, row0 = cache.k, cache.v, cache.k.shape[1], cache.offset
         assert kbuf.shape == (hk, cap, d) and kbuf.is_contiguous() and vbuf.is_contiguous()
-        k, v = kbuf[:, :row0 + L], vbuf[:, :row0 + L]
-    _lib.call("scmx_qkv_norm", _lib.ptr(src), int(is_acc), _lib.ptr(xscale), _lib.ptr(wscale), _lib.ptr(qn), _lib.ptr(kn),
+        k, v = (None, None) if quant else (kbuf[:, :row0 + L], vbuf[:, :row0 + L])
+    if row_pos is not None:
+        _lib.require_cuda(row_pos)
+        assert row_pos.dtype == torch.int32 and row_pos.numel() == L
+    if quant and not (d in (64, 128, 256) and (not full or (not is_acc and hq + 2 * hk <= 96)) and all(t.data_ptr() % 16 == 0 for t in (src, qn, kn))):
+        assert pos_dev is None, "a device-side position into an INT8 cache: head sizes 64, 128 and 256"
+        q, k, v = _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, None, None, row_pos)
+        C.kv_append(k, v, cache)
+        return q, None, None
+    _lib.call("scmx_qkv_norm_rows", _lib.ptr(src), int(is_acc), _lib.ptr(xscale), _lib.ptr(wscale), _lib.ptr(qn), _lib.ptr(kn),
               _eps(eps), L, hq, hk, d, int(full), _lib.ptr(inv_freq), _lib.ptr(table),
-              0 if table is None else table.shape[0], int(pos0), _lib.ptr(pos_dev), _lib.ptr(q), L,
-              _lib.ptr(kbuf), _lib.ptr(vbuf), cap, row0, _lib.stream())
+              0 if table is None else table.shape[0], int(pos0), _lib.ptr(pos_dev), _lib.ptr(row_pos), _lib.ptr(q), L,
+              _lib.ptr(kbuf), _lib.ptr(vbuf), _lib.ptr(cache.ks) if quant else None, _lib.ptr(cache.vs) if quant else None, cap, row0, _lib.stream())
     return q, k, v
 
 
 def qkv_epilogue_headnorm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, dtype=torch.bfloat16, deps=(), rope=None,
-                          cache=None):
+                          cache=None, row_pos=None):
     """acc int32 [Mp, (hq + 2 hk) d] -> q [hq, L, d], k [hk, L, d], v [hk, L, d] with per-head RMSNorm of q and k.
     rope=(inv_freq, pos0[, rope_table]): rotary embedding of q and k at positions pos0.. in the same kernel; cache (with .k, .v
-    [hk, capacity, d] and .offset): k and v are written into the cache rows and the filled prefix is returned."""
-    return _qkv_norm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, False, rope, cache)
+    [hk, capacity, d] and .offset): k and v are written into the cache rows and the filled prefix is returned (None for an INT8 cache, host_model.QuantKVCache:
+    sc_cache.kv_read has it).  row_pos int32 [L]: row r turns as position pos0 + row_pos[r]."""
+    return _qkv_norm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, False, rope, cache, None, row_pos)
 
 
-def qkv_headnorm_y(y, qn, kn, eps, L, hq, hk, d, deps=(), rope=None, cache=None, pos_dev=None):
+def qkv_headnorm_y(y, qn, kn, eps, L, hq, hk, d, deps=(), rope=None, cache=None, pos_dev=None, row_pos=None):
     """bf16 y [Mp, (hq + 2 hk) d] -> q [hq, L, d], k [hk, L, d], v [hk, L, d] (q/k per-head RMSNorm)."""
-    return _qkv_norm(y, None, None, qn, kn, eps, L, hq, hk, d, False, rope, cache, pos_dev)
+    return _qkv_norm(y, None, None, qn, kn, eps, L, hq, hk, d, False, rope, cache, pos_dev, row_pos)
 
 
-def qkv_fullnorm_y(y, qn, kn, eps, L, h, d, deps=(), rope=None, cache=None, pos_dev=None):
+def qkv_fullnorm_y(y, qn, kn, eps, L, h, d, deps=(), rope=None, cache=None, pos_dev=None, row_pos=None):
     """bf16 y [Mp, 3 h d] -> q, k, v [h, L, d] with RMSNorm over the full h*d-wide q and k."""
-    return _qkv_norm(y, None, None, qn, kn, eps, L, h, h, d, True, rope, cache, pos_dev)
+    return _qkv_norm(y, None, None, qn, kn, eps, L, h, h, d, True, rope, cache, pos_dev, row_pos)
 
 
 class DecodeAttention:

@@ -68,3 +68,31 @@ def test_entry_points_refuse(scmx):
                      (dict(t=float("nan")), "temperature"), (dict(t=float("inf")), "temperature"), (dict(t=1e-42), "temperature"), (dict(u=None), "random"),
                      (dict(size=8), "scratch"), (dict(tokens=None), "null")):
         _refused(scmx, "scmx_verify", check(**kw), text)
+
+
+def test_lookup_draft(scmx):
+    import importlib
+    L = importlib.import_module(scmx.__name__ + ".decode").LookupDraft
+    text = [1, 2, 3, 4, 5, 9, 1, 2, 3, 4, 6, 7, 1, 2, 3]
+    rows, parents = L(match=3, length=3, places=2)(text, 64)
+    assert rows == [3, 4, 6, 7, 5, 9] and parents == [-1, 0, 1, 2, 1, 4]          # the latest place first, the shared beginning once
+    scmx.sc_draft.check_tree(parents)
+    assert L(length=3)(text, 3) == ([3, 4, 6], [-1, 0, 1])
+    assert L()(text, 1) == ([3], [-1]) and L()([5], 8) == ([5], [-1]) and L()([1, 2, 3], 8) == ([3], [-1])
+    assert L(match=1, length=2, places=1)([4, 4, 4], 8) == ([4, 4], [-1, 0])
+
+
+def test_caches_of_models(scmx):
+    HM = scmx.host_model
+    model = HM.CausalLM(HM.ModelArgs(64, 64, 2, 2, 1, 32, 1e-6, 1e6, 16, True))
+    plain, quant = HM.make_prompt_cache(model, 8), HM.make_prompt_cache(model, 8, dtype=torch.int8)
+    assert all(type(c) is HM.KVCache for c in plain) and all(type(c) is HM.QuantKVCache for c in quant)
+    assert quant[0].k.shape == (1, 8, 32) and quant[0].ks.shape == (1, 8) and quant[0].carried() == []
+    with pytest.raises(ValueError):
+        HM.make_prompt_cache(model, 8, dtype=torch.float16)
+    cfg = {"architecture": "Sebesun", "vocab": 8, "width": 8, "norm": {"eps": 1e-5}, "layers": [
+        {"type": "retention", "mixer": {"heads": 1, "dim": 8, "vdim": 8, "decay": [0.9]}, "mlp": None}]}
+    hybrid = HM.HybridLM(HM.HybridArgs.from_config(cfg), device="cpu", dtype=torch.float32)
+    with pytest.raises(ValueError):
+        HM.make_prompt_cache(hybrid, 8, dtype=torch.int8)
+    assert len(HM.make_prompt_cache(hybrid, 8, dtype=torch.float32)) == 1

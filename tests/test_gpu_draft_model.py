@@ -1,0 +1,224 @@
+"""GPU: INT8 caches and draft trees through the W4A8 decoders: the fused write against its two steps, rows of a tree against the same tokens one after the other,
+speculative generation against the model's own choices, the engine."""
+import importlib
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def mod(scmx, n):
+    return importlib.import_module(scmx.__name__ + "." + n)
+
+
+# ---- keys and values into an INT8 cache ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("full,acc", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (8, 2, 128), (3, 1, 256), (4, 4, 128), (4, 2, 32)])
+@pytest.mark.parametrize("L", [1, 7, 130])
+def test_fused_write_equals_its_steps(scmx, full, acc, hq, hk, d, L):
+    S, HM, C = scmx.sc_kernels, scmx.host_model, scmx.sc_cache
+    if full:
+        hk = hq
+    g = torch.Generator(device="cuda").manual_seed(L + d)
+    ntot = (hq + 2 * hk) * d
+    if acc:
+        src = torch.randint(-200000, 200000, (L, ntot), generator=g, device="cuda", dtype=torch.int32)
+        xs, ws = torch.rand(L, generator=g, device="cuda") * 1e-3 + 1e-4, torch.rand(ntot, generator=g, device="cuda") * 1e-2 + 1e-3
+    else:
+        src, xs, ws = (torch.randn((L, ntot), generator=g, device="cuda") * 3).to(BF), None, None
+    if not acc:
+        src[0, -d:] = 0.0                            # a value of zeros
+        src[L // 2, (hq + hk) * d + 1] = float("nan")
+    qn, kn = ((1 + 0.2 * torch.randn(n, generator=g, device="cuda")).to(BF) for n in ((hq * d, hk * d) if full else (d, d)))
+    inv, off = S.rope_inv_freq(d, 1e4), 5
+    rope = (inv, off, S.rope_table(inv, 64))
+    rows = torch.randint(0, 9, (L,), generator=g, device="cuda", dtype=torch.int32)
+    for row_pos in (None, rows):
+        got, want = HM.QuantKVCache(hk, d, L + 9), HM.QuantKVCache(hk, d, L + 9)
+        for c in (got, want):
+            for t in (c.k, c.v, c.ks, c.vs):
+                t.fill_(3)
+            c.offset = off
+        q, k, v = S._qkv_norm(src, xs, ws, qn, kn, 1e-6, L, hq, hk, d, full, rope, got, None, row_pos)
+        assert k is None and v is None
+        q2, k2, v2 = S._qkv_norm(src, xs, ws, qn, kn, 1e-6, L, hq, hk, d, full, rope, None, None, row_pos)
+        C.kv_append(k2, v2, want)
+        assert torch.equal(q, q2) and torch.equal(got.k, want.k) and torch.equal(got.v, want.v) and torch.equal(got.ks, want.ks)
+        assert torch.equal(got.vs.isnan(), want.vs.isnan()) and torch.equal(got.vs.nan_to_num(), want.vs.nan_to_num())
+        if d >= 64:                                  # the position on the device
+            dev = HM.QuantKVCache(hk, d, L + 9)
+            for t in (dev.k, dev.v, dev.ks, dev.vs):
+                t.fill_(3)
+            q3, _, _ = S._qkv_norm(src, xs, ws, qn, kn, 1e-6, L, hq, hk, d, full, (inv, 0, rope[2]), dev, torch.tensor([off], dtype=torch.int32, device="cuda"), row_pos)
+            assert torch.equal(q3, q) and torch.equal(dev.k, want.k) and torch.equal(dev.v, want.v) and torch.equal(dev.ks, want.ks)
+
+
+def test_rows_turn_where_they_are_told(scmx):
+    """row_pos 0 .. L - 1 is no row_pos; the same position for all rows turns them alike."""
+    S, HM = scmx.sc_kernels, scmx.host_model
+    g = torch.Generator(device="cuda").manual_seed(1)
+    y = torch.randn((6, 4 * 128), generator=g, device="cuda").to(BF)
+    w, inv = torch.ones(128, dtype=BF, device="cuda"), S.rope_inv_freq(128, 1e4)
+    for table in ((), (S.rope_table(inv, 8),)):      # from the table, and beyond its end
+        a, b = HM.KVCache(1, 128, 40), HM.KVCache(1, 128, 40)
+        a.offset = b.offset = 3
+        want = S.qkv_headnorm_y(y, w, w, 1e-6, 6, 2, 1, 128, rope=(inv, 3, *table), cache=a)
+        got = S.qkv_headnorm_y(y, w, w, 1e-6, 6, 2, 1, 128, rope=(inv, 3, *table), cache=b, row_pos=torch.arange(6, dtype=torch.int32, device="cuda"))
+        assert all(torch.equal(x[:, -6:], z[:, -6:]) for x, z in zip(got, want))
+        same = S.qkv_headnorm_y(y[:1].expand(6, -1).contiguous(), w, w, 1e-6, 6, 2, 1, 128, rope=(inv, 3, *table), cache=b,
+                                row_pos=torch.full((6,), 4, dtype=torch.int32, device="cuda"))
+        assert all(torch.equal(same[0][:, i], same[0][:, 0]) for i in range(6))
+
+
+# ---- whole models -------------------------------------------------------------------------------------------------------------
+
+def build(scmx, kind, seed=3, **kw):
+    HM = scmx.host_model
+    if kind == "qwen3":
+        FQ = mod(scmx, "fused_qwen3")
+        model = HM.CausalLM(HM.ModelArgs(1024, 2048, 2, 8, 2, 128, 1e-6, 1e6, 512, True)).init_random(seed, 0.05).cuda()
+        fused = FQ.FusedQwen3(model, FQ.pack_model(model, on_device=True), **kw)
+        return fused, mod(scmx, "decode").DecodeQwen3(fused) if fused.epilogue == "gemm" else None
+    FO = mod(scmx, "fused_olmoe")
+    model = HM.CausalLM(HM.ModelArgs(512, 256, 2, 4, 4, 128, 1e-5, 1e4, 512, False, 8, 2, False, "olmoe")).init_random(seed, 0.05).cuda()
+    fused = FO.FusedOlmoe(model, FO.pack_olmoe(model, on_device=True))
+    return fused, mod(scmx, "decode").DecodeOlmoe(fused)
+
+
+def rel(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+@pytest.mark.parametrize("kind,kw", [("qwen3", {}), ("qwen3", dict(epilogue="row")), ("qwen3", dict(resident=True)), ("qwen3", dict(fuse_rope=False)), ("olmoe", {})])
+@pytest.mark.parametrize("dtype", [None, torch.int8])
+def test_rows_of_a_tree_are_their_paths(scmx, kind, kw, dtype):
+    """Every row's logits are those of its path read as a prompt: the rows quantize alike, attention differs by roundings of its weights (2^-8 a weight, averaged
+    over positions and layers, and the INT8 codes that they turn: a few percent of a logit at the most)."""
+    fused, _ = build(scmx, kind, **kw)
+    D = scmx.sc_draft
+    rng = random.Random(5)
+    prompt = torch.tensor([[rng.randrange(512) for _ in range(45)]], device="cuda")
+    tree = D.DraftTree([-1, 0, 0, 1, 1, 3, 2, 6, 7])
+    tokens = [rng.randrange(512) for _ in range(len(tree))]
+    cache = fused.make_cache(80, dtype)
+    fused.hidden(prompt, cache)
+    got = fused.logits(fused.hidden(torch.tensor([tokens], device="cuda"), cache, tree))[0]
+    assert all(c.offset == 45 for c in cache)
+    for i in (0, 2, 5, 8):
+        path, j = [], i
+        while j >= 0:
+            path.insert(0, tokens[j])
+            j = tree.list[j]
+        other = fused.make_cache(80, dtype)
+        fused.hidden(prompt, other)
+        want = fused.logits(fused.hidden(torch.tensor([path], device="cuda"), other))[0, -1]
+        assert rel(got[i], want) < 0.05, (i, rel(got[i], want))
+    scmx._lib.check_status()
+
+
+@pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
+def test_int8_cache_steps(scmx, kind):
+    """Steps on an INT8 cache: near the bfloat16 cache's (a code is off by at most 1 / 254 of its vector's largest value), and the captured ones the same as the others."""
+    fused, decoder = build(scmx, kind)
+    ids = torch.randint(0, 512, (1, 60), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    plain, quant, again = fused.make_cache(100), fused.make_cache(100, torch.int8), fused.make_cache(100, torch.int8)
+    a, b = (fused.logits(fused.hidden(ids, c)[:, -1:]) for c in (plain, quant))
+    fused.hidden(ids, again)
+    assert rel(b, a) < 0.1
+    tok = a[:, -1].argmax(-1, keepdim=True)
+    x, y = decoder.step(tok, plain), decoder.step(tok, quant)
+    assert rel(y, x) < 0.1 and quant[0].offset == 61
+    quant[0].offset, quant[1].offset = 60, 60
+    steps, t = [], tok
+    for _ in range(12):
+        t = decoder.step(t, quant)[:, -1].argmax(-1, keepdim=True)
+        steps.append(int(t))
+    assert decoder.generate(tok, again, 12).tolist() == steps and again[0].offset == 72
+    assert torch.equal(again[1].k[:, :72], quant[1].k[:, :72]) and torch.equal(again[1].vs[:, :72], quant[1].vs[:, :72])
+    decoder.check_status() if kind == "qwen3" else None
+    scmx._lib.check_status()
+
+
+# Most that a chosen token's logit may be below the largest, in units of the logits' spread.  The rows' logits are within 0.05 of the spread of the prompt's (the
+# bound of test_rows_of_a_tree_are_their_paths, a root mean square); of some 10^4 nearly normal errors the largest is 4 such units, and a choice is
+# turned by two errors, its own and the largest logit's: 2 * 4 * 0.05.  A token that is not the model's is about 3 below.
+MARGIN = 0.4
+
+
+def margins(fused, prompt, tokens, dtype):
+    """How far the model's logit of each generated token is below its largest, reading them as one prompt; in units of the logits' spread."""
+    cache = fused.make_cache(len(prompt) + len(tokens) + 1, dtype)
+    logits = fused.logits(fused.hidden(torch.tensor([prompt + tokens], device="cuda"), cache))[0, len(prompt) - 1:-1].double()
+    return ((logits.amax(-1) - logits.gather(1, torch.tensor(tokens, device="cuda")[:, None])[:, 0]) / logits.std(-1)).max().item()
+
+
+@pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
+@pytest.mark.parametrize("dtype", [None, torch.int8])
+def test_drafted_generation_is_the_models(scmx, kind, dtype):
+    """Greedy generation with drafts: every token is the model's own choice (its logit among the largest, up to what roundings turn), whatever is drafted; a draft that
+    knows the continuation is accepted whole."""
+    fused, decoder = build(scmx, kind)
+    DEC = mod(scmx, "decode")
+    rng = random.Random(1)
+    prompt = [rng.randrange(512) for _ in range(12)] * 3
+    known = []
+
+    def oracle_draft(text, most):
+        """A wrong row beside the right ones."""
+        chain = [text[-1]] + known[len(text) - len(prompt):][:min(most, 7) - 1]
+        if len(chain) + 1 <= most and len(chain) > 1:
+            return chain + [(chain[1] + 1) % 512], list(range(-1, len(chain) - 1)) + [0]
+        return chain, list(range(-1, len(chain) - 1))
+
+    def run(propose, n=24):
+        cache = fused.make_cache(len(prompt) + n, dtype)                # no room behind the last token
+        first = int(fused.logits(fused.hidden(torch.tensor([prompt], device="cuda"), cache)[:, -1:]).argmax())
+        passes = []
+        d = DEC.DecodeDraft(fused, lambda text, most: (passes.append(1), propose(text, most))[1])
+        out = d.generate(torch.tensor([[first]], device="cuda"), cache, n, prompt).tolist()
+        assert cache[0].offset == len(prompt) + n and len(out) == n
+        return [first] + out, len(passes)
+    text, passes = run(lambda text, most: ([text[-1]], [-1]))            # nothing drafted: a token a pass
+    assert passes == 24 and margins(fused, prompt, text, dtype) < MARGIN
+    known[:] = text
+    again, passes = run(oracle_draft)
+    assert margins(fused, prompt, again, dtype) < MARGIN
+    if again == text:
+        assert passes <= 6                                               # 24 tokens, 7 at a time
+    looked, passes = run(DEC.LookupDraft())
+    assert margins(fused, prompt, looked, dtype) < MARGIN and passes <= 24
+    wild, _ = run(lambda text, most: ([text[-1]] + [rng.randrange(512) for _ in range(min(most, 9) - 1)], [-1] + [0] * (min(most, 9) - 1)))
+    assert margins(fused, prompt, wild, dtype) < MARGIN
+    scmx._lib.check_status()
+
+
+def test_sampled_generation_repeats_with_its_generator(scmx):
+    fused, _ = build(scmx, "qwen3")
+    DEC = mod(scmx, "decode")
+    prompt = list(range(5, 25)) * 2
+    out = []
+    for _ in range(2):
+        cache = fused.make_cache(100, torch.int8)
+        fused.hidden(torch.tensor([prompt], device="cuda"), cache)
+        out.append(DEC.DecodeDraft(fused).generate(torch.tensor([[7]], device="cuda"), cache, 20, prompt, 0.8, torch.Generator(device="cuda").manual_seed(4)).tolist())
+    assert out[0] == out[1] and all(0 <= t < 512 for t in out[0])
+
+
+def test_engine_with_drafts(scmx):
+    fused, decoder = build(scmx, "qwen3")
+    R, E, DEC = mod(scmx, "registry"), mod(scmx, "engine"), mod(scmx, "decode")
+    bundle = R.Bundle("qwen3", fused, decoder, 512, scmx._lib.check_status)
+    prompt = list(range(40, 70)) * 2
+    for dtype in (None, torch.int8):
+        engine = E.Engine(bundle, 128, cache_dtype=dtype)
+        plain = engine.generate(prompt, 20)
+        drafted = engine.generate(prompt, 20, draft=DEC.LookupDraft())
+        assert len(plain) == len(drafted) == 20 and not engine.live
+        assert engine.pool.free[0][0].k.dtype == (torch.int8 if dtype else BF)
+        for text in (plain, drafted):
+            assert margins(fused, prompt, text, dtype) < MARGIN
+    bundle.check_status()

@@ -10,7 +10,10 @@
 // score exceeds it by 2^8, so that most blocks neither exchange nor rescale anything.  The warps' states are joined in shared memory, the
 // ranges' by a second launch.
 // INT8 codes become bfloat16 exactly (8 significant bits); a position's key scale multiplies its scores, its value scale its weights.
+#include <cooperative_groups.h>
 #include "scmx_cache_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace scmx {
 
@@ -28,7 +31,7 @@ struct CaShape {
     static constexpr int PITCH = D + 4;                               // a warp's state when the warps are joined: rows of values, then maxima and sums
     static constexpr int STATE = ROWS * (PITCH + 2) * 4;
     static constexpr int WARP = ((RING > STATE ? RING : STATE) + 127) / 128 * 128;
-    static constexpr int TOTAL = WARP * WARPS;
+    static constexpr int TOTAL = WARP * WARPS + ROWS * (D + 2) * 4;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -74,12 +77,12 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * L::ROWS;
     const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
     const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
-    if (t0 >= T) return;
+    if (t0 >= T && !a.cluster) return;
     const unsigned char* kb = static_cast<const unsigned char*>(a.k) + ((int64_t)kvh * a.cap + t0) * ROW;
     const unsigned char* vb = static_cast<const unsigned char*>(a.v) + ((int64_t)kvh * a.cap + t0) * ROW;
     unsigned char* ring = smem_raw + warp * L::WARP;
     const uint32_t ring_s = smem_u32(ring);
-    const int nkeys = (int)(t1 - t0), nblocks = (nkeys + CA_KEYS - 1) / CA_KEYS, ntail = (int)(pos - t0 < nkeys ? pos - t0 : nkeys);      // keys from ntail on are new rows (negative: from before t0)
+    const int nkeys = t1 > t0 ? (int)(t1 - t0) : 0, nblocks = (nkeys + CA_KEYS - 1) / CA_KEYS, ntail = (int)(pos - t0 < nkeys ? pos - t0 : nkeys);      // keys from ntail on are new rows (negative: from before t0)
 
     // copies of block b: pieces lane, lane + 32, .. of 16 bytes; a warp covers whole vectors with each, whose places repeat after DIST
     constexpr int COPIES = CA_KEYS * PIECES / 32, RSTEP = 32 / PIECES, DIST = RSTEP >= 8 ? 1 : 8 / RSTEP;
@@ -357,17 +360,33 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     constexpr int E = D / 32;
     const int live = nblocks < WARPS ? nblocks : WARPS, rows = R - row0 < L::ROWS ? R - row0 : L::ROWS;      // warps that had a block; rows of this tile
     const float* states = reinterpret_cast<const float*>(smem_raw);
+    float* joined = reinterpret_cast<float*>(smem_raw + WARPS * L::WARP);      // this range's state: values, then maxima and sums
     for (int r = warp; r < rows; r += WARPS) {
         const float2 ml = lane < live ? reinterpret_cast<const float2*>(states + lane * (L::WARP / 4) + L::ROWS * L::PITCH)[r] : make_float2(-INFINITY, 0.0f);
         float m = ml.x, l = ml.y, v[E];
         ca_join<E, 8>(live, m, l, v, [&](int s, float (&z)[E]) { ca_load<E>(states + s * (L::WARP / 4) + r * L::PITCH + lane * E, z); });
-        if (a.part == nullptr) {
+        if (a.cluster) {
+            ca_store<E>(joined + r * D + lane * E, v);
+            if (lane == 0) reinterpret_cast<float2*>(joined + L::ROWS * D)[r] = make_float2(m, l);
+        } else if (a.part == nullptr) {
             ca_output<D>(a, kvh, row0 + r, lane, v, l);
         } else {
             const int64_t at = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * L::ROWS + r;
             ca_store<E>(a.part + at * D + lane * E, v);
             if (lane == 0) a.part_ml[at] = make_float2(m, l);
         }
+    }
+    if (a.cluster) {                     // the ranges' states, read where they lie: the rows in turn to the CTAs
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        const int ctas = (int)cl.num_blocks();
+        for (int r = (int)cl.block_rank() + ctas * warp; r < rows; r += ctas * WARPS) {
+            const float2 ml = lane < ctas ? reinterpret_cast<const float2*>(cl.map_shared_rank(joined, lane) + L::ROWS * D)[r] : make_float2(-INFINITY, 0.0f);
+            float m = ml.x, l = ml.y, v[E];
+            ca_join<E, 8>(ctas, m, l, v, [&](int s, float (&z)[E]) { ca_load<E>(cl.map_shared_rank(joined, s) + r * D + lane * E, z); });
+            ca_output<D>(a, kvh, row0 + r, lane, v, l);
+        }
+        cl.sync();                       // nobody leaves while its state may still be read
     }
 }
 
@@ -398,8 +417,14 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
     ca_output<D>(a, kvh, r, lane, v, l);
 }
 
+// A cluster's CTAs join their ranges without a second launch, but they are eight at most: up to so many positions.  Device us, cluster / two launches, 8 key/value
+// heads of 128, one token of two query heads each: 300 positions 5.4 / 6.6, 1500 6.3 / 7.8, 4000 7.6 / 8.7, 6000 8.7 / 9.6, 9000 10.1 / 9.6, 12000 12.0 / 11.7;
+// INT8 1500 6.3 / 7.8, 6000 9.4 / 9.6, 9000 11.2 / 10.4, 12000 12.8 / 11.2.  On the host it is 6 us sooner.
+constexpr int64_t CA_CLUSTER_POSITIONS = 8192;
+
 static CaPlan ca_plan(int64_t positions, int R, int hk) {
     CaPlan p;
+    p.cluster = 0;
     p.tc = R > 16;
     if (p.tc) {
         p.nt = R > 128 ? 2 : 1;
@@ -416,6 +441,10 @@ static CaPlan ca_plan(int64_t positions, int R, int hk) {
     const int64_t most = (positions + p.unit - 1) / p.unit, want = sm_count() / ((int64_t)hk * p.tiles);
     const int64_t s = want < most ? want : most;
     p.nsplit = s < 1 ? 1 : (int)s;
+    if (!p.tc && positions <= CA_CLUSTER_POSITIONS) {
+        p.cluster = 1;
+        p.nsplit = most >= 8 ? 8 : most >= 3 ? 4 : most == 2 ? 2 : 1;
+    }
     if (!p.tc && positions > (int64_t)p.nsplit * p.unit) p.unit = CA_KEYS;      // long enough: ranges end at any block
     return p;
 }
@@ -430,13 +459,28 @@ static int launch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
         SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<D, I8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
         configured[dev] = true;
     }
-    SCMX_PDL_OK("cache_attn_kernel", launch_pdl(cache_attn_kernel<D, I8, NT>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles), dim3(L::THREADS),
-                                                (size_t)L::TOTAL, st, a));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles);
+    cfg.blockDim = dim3(L::THREADS);
+    cfg.dynamicSmemBytes = L::TOTAL;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (g_use_pdl) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.cluster) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        attr[cfg.numAttrs++].val.clusterDim.y = p.nsplit;
+    }
+    SCMX_PDL_OK("cache_attn_kernel", cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, I8, NT>, a));
     return SCMX_OK;
 }
 template <int D, bool I8>
 static int dispatch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) { return p.nt == 1 ? launch_ca<D, I8, 1>(a, p, st) : launch_ca<D, I8, 2>(a, p, st); }
-static int64_t ca_states(const CaPlan& p, int hk) { return p.nsplit == 1 ? 0 : (int64_t)hk * p.tiles * p.nsplit * p.rows; }      // partial states of query rows
+static int64_t ca_states(const CaPlan& p, int hk) { return p.nsplit == 1 || p.cluster ? 0 : (int64_t)hk * p.tiles * p.nsplit * p.rows; }      // partial states of query rows
 
 }  // namespace scmx
 
@@ -460,7 +504,7 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
                      ((uintptr_t)out & 15) == 0, SCMX_EINVAL, "cache_attn: query rows must be 8-byte, caches and the output 16-byte aligned");
     CaArgs a;
     const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk);
-    a.nsplit = p.nsplit; a.unit = p.unit;
+    a.nsplit = p.nsplit; a.unit = p.unit; a.cluster = p.cluster;
     const int64_t states = ca_states(p, hk), need = states * (d + 2) * 4;
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",
                  (long long)scratch_bytes, (long long)need);

@@ -21,7 +21,7 @@ struct CaArgs {
     float2* part_ml;                 // their maxima (exponents of 2) and sums of weights, [hk, tiles, nsplit, rows]
     uint16_t* out;                   // bf16 [n, hq d]
     int64_t q_hs, q_rs, pos, cap;
-    int n, hq, hk, nsplit, unit;
+    int n, hq, hk, nsplit, unit, cluster;      // cluster: the ranges' CTAs are one, and join their states themselves
     float scale;                     // times log2(e)
 };
 
@@ -93,7 +93,7 @@ __device__ __forceinline__ void ca_join(int count, float& m, float& l, float (&v
 
 // How a call is cut.  tc: by the tcgen05 kernel, `nt` query tiles of 128 in a CTA and `copies` of the rows in a tile; otherwise nt groups of eight query rows.
 // `rows` query rows in a CTA, `tiles` of them, `nsplit` ranges of positions that are multiples of `unit`.
-struct CaPlan { int tc, nt, copies, rows, tiles, nsplit, unit; };
+struct CaPlan { int tc, nt, copies, rows, tiles, nsplit, unit, cluster; };
 
 int cache_attn_tc(const CaArgs& a, const CaPlan& p, int d, int int8, int32_t* status, cudaStream_t st);
 

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * L::ROWS;
+    const int kvh = blockIdx.x, split = blockIdx.y, G = a.G, R = G * a.n, row0 = blockIdx.z * L::ROWS;
     const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
     const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
     if (t0 >= T && !a.cluster) return;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     uint2 qf[NT][KSTEPS];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = row0 + 8 * nt + g, rr = r < R ? r : 0, tok = rr / G;
+        const int r = row0 + 8 * nt + g, rr = r < R ? r : 0, tok = ca_tok(a, rr);
         const uint16_t* qp = a.q + (int64_t)(kvh * G + rr - tok * G) * a.q_hs + (int64_t)tok * a.q_rs;
 #pragma unroll
         for (int s = 0; s < KSTEPS; ++s) {
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = row0 + 8 * nt + 2 * t4 + e, tok = r / G;
+                    const int r = row0 + 8 * nt + 2 * t4 + e, tok = ca_tok(a, r);
                     if (r < R) {
                         const uint64_t bits = a.mask ? (uint64_t)a.mask[tok] : (2ull << tok) - 1ull;
 #pragma unroll
@@ -395,12 +395,12 @@ template <int D>
 __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ CaArgs a, int tiles, int rows) {
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31, R = a.hq / a.hk * a.n, i = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, R = a.G * a.n, i = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (i >= a.hk * R) return;
     constexpr int E = D / 32;
     const int kvh = i / R, r = i - kvh * R, tile = r / rows;
     const int64_t T = ca_pos(a.pos_dev, a.pos, a.cap, a.n) + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
-    const int active = (int)((T + chunk - 1) / chunk);
+    const int active = ca_ranges(T, chunk);
     const int64_t first = ((int64_t)kvh * tiles + tile) * a.nsplit * rows + (r - tile * rows);
     float m = -INFINITY, l = 0.0f, v[E] = {};
     for (int s0 = 0; s0 < active; s0 += 32) {
@@ -497,7 +497,7 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
     SCMX_REQUIRE(q && k && v && out && status && (!int8 || (k_scales && v_scales)), SCMX_EINVAL, "cache_attn: null buffer");
     SCMX_REQUIRE(n >= 1 && n <= CA_MAX_ROWS, SCMX_ELIMIT, "cache_attn: %d rows (1 .. %d)", n, CA_MAX_ROWS);
     SCMX_REQUIRE(d == 64 || d == 128, SCMX_EINVAL, "cache_attn: head size %d (64 or 128)", d);
-    SCMX_REQUIRE(hk > 0 && hq > 0 && hq % hk == 0, SCMX_EINVAL, "cache_attn: hq=%d hk=%d", hq, hk);
+    SCMX_REQUIRE(hk > 0 && hq > 0 && hq % hk == 0 && hq / hk <= 4096, SCMX_EINVAL, "cache_attn: hq=%d hk=%d", hq, hk);
     SCMX_REQUIRE(capacity >= n && (pos_dev != nullptr || (pos >= 0 && pos + n <= capacity)), SCMX_EINVAL, "cache_attn: rows %lld .. %lld of a cache of %lld",
                  (long long)pos, (long long)(pos + n), (long long)capacity);
     SCMX_REQUIRE(q_head_stride % 4 == 0 && q_row_stride % 4 == 0 && ((uintptr_t)q & 7) == 0 && ((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 &&
@@ -509,7 +509,7 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",
                  (long long)scratch_bytes, (long long)need);
     a.q = q; a.q_hs = q_head_stride; a.q_rs = q_row_stride; a.k = k; a.v = v; a.ks = k_scales; a.vs = v_scales; a.mask = mask; a.pos_dev = pos_dev; a.pos = pos;
-    a.part = need ? static_cast<float*>(scratch) : nullptr; a.part_ml = need ? reinterpret_cast<float2*>(a.part + states * d) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.scale = scale * CA_LOG2E;
+    a.part = need ? static_cast<float*>(scratch) : nullptr; a.part_ml = need ? reinterpret_cast<float2*>(a.part + states * d) : nullptr; a.out = out; a.cap = capacity; a.n = n; a.hq = hq; a.hk = hk; a.G = hq / hk; a.inv_g = 1.0f / (float)a.G; a.scale = scale * CA_LOG2E;
     const cudaStream_t st = (cudaStream_t)stream;
     int rc = p.tc ? cache_attn_tc(a, p, d, int8, status, st)
              : d == 128 ? (int8 ? dispatch_ca<128, true>(a, p, st) : dispatch_ca<128, false>(a, p, st))

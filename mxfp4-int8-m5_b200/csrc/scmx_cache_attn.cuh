@@ -21,8 +21,9 @@ struct CaArgs {
     float2* part_ml;                 // their maxima (exponents of 2) and sums of weights, [hk, tiles, nsplit, rows]
     uint16_t* out;                   // bf16 [n, hq d]
     int64_t q_hs, q_rs, pos, cap;
-    int n, hq, hk, nsplit, unit, cluster;      // cluster: the ranges' CTAs are one, and join their states themselves
+    int n, hq, hk, G, nsplit, unit, cluster;      // cluster: the ranges' CTAs are one, and join their states themselves
     float scale;                     // times log2(e)
+    float inv_g;                     // 1 / G, G = hq / hk
 };
 
 // First new row's position, and positions of one range: whole units, so a short cache uses the first few ranges only.
@@ -31,9 +32,16 @@ __device__ __forceinline__ int64_t ca_pos(const int32_t* pos_dev, int64_t pos, i
     return p < 0 ? 0 : p > cap - n ? cap - n : p;
 }
 __device__ __forceinline__ int64_t ca_chunk(int64_t T, int nsplit, int unit) {
+    if (T < (1ll << 31) - 4096) {        // 64-bit divisions are hundreds of cycles before a kernel's first load
+        const uint32_t c = ((uint32_t)T + nsplit - 1) / (uint32_t)nsplit;
+        return (c + unit - 1) & ~(uint32_t)(unit - 1);      // units are powers of two
+    }
     const int64_t c = (T + nsplit - 1) / nsplit;
     return (c + unit - 1) / unit * unit;
 }
+__device__ __forceinline__ int ca_ranges(int64_t T, int64_t chunk) { return T < (1ll << 31) ? (int)(((uint32_t)T + (uint32_t)chunk - 1) / (uint32_t)chunk) : (int)((T + chunk - 1) / chunk); }
+// The new row of a query row: row / G.  Exact: row + 1/2 is at least 1 / (2 G) of its size away from whole multiples of G, rows are below 2^18 (64 rows of 4096 heads).
+__device__ __forceinline__ int ca_tok(const CaArgs& a, int row) { return (int)(((float)row + 0.5f) * a.inv_g); }
 
 __device__ __forceinline__ float ca_ex2(float x) {
     float y;
@@ -59,8 +67,8 @@ __device__ __forceinline__ void ca_store(float* p, const float (&v)[E]) {
 // A query row of the output, v / total (zeros where nothing was seen).
 template <int D>
 __device__ __forceinline__ void ca_output(const CaArgs& a, int kvh, int row, int lane, const float (&v)[D / 32], float total) {
-    const int G = a.hq / a.hk, tok = row / G;
-    uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)tok * a.hq * D + (kvh * G + row - tok * G) * D) + lane * (D / 64);
+    const int tok = ca_tok(a, row);
+    uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)tok * a.hq * D + (kvh * a.G + row - tok * a.G) * D) + lane * (D / 64);
 #pragma unroll
     for (int e = 0; e < D / 32; e += 2) o[e / 2] = total == 0.0f ? 0u : pack_bf16x2(v[e] / total, v[e + 1] / total);
 }

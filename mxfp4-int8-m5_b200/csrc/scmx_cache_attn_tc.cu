@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     pdl_wait();
 
-    const int kvh = blockIdx.x, split = blockIdx.y, G = a.hq / a.hk, R = G * a.n, row0 = blockIdx.z * ROWS;
+    const int kvh = blockIdx.x, split = blockIdx.y, G = a.G, R = G * a.n, row0 = blockIdx.z * ROWS;
     const int64_t pos = ca_pos(a.pos_dev, a.pos, a.cap, a.n), T = pos + a.n, chunk = ca_chunk(T, a.nsplit, a.unit);
     const int64_t t0 = split * chunk, t1 = t0 + chunk < T ? t0 + chunk : T;
     const int nkeys = t1 > t0 ? (int)(t1 - t0) : 0, ntiles = (nkeys + 127) / 128, units = ntiles * MQ;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 uint2 x[BATCH];
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {          // nothing here waits for a load: rows past the last read row 0
-                    const int r = row0 + ((i0 + i) * 8 + warp) * RPW + lane / LPR, rr = r < R ? r : 0, qt = rr / G;
+                    const int r = row0 + ((i0 + i) * 8 + warp) * RPW + lane / LPR, rr = r < R ? r : 0, qt = ca_tok(a, rr);
                     x[i] = __ldg(reinterpret_cast<const uint2*>(a.q + (int64_t)(kvh * G + rr - qt * G) * a.q_hs + (int64_t)qt * a.q_rs + 4 * ql));
                 }
 #pragma unroll
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(b_q);
         }
-        const int m = warp >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = row / G;
+        const int m = warp >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = ca_tok(a, row);
         const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
         const int c0 = copy * (128 / COPIES);                   // the thread's first key of a tile
         uint64_t bits = 0;
@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const uint64_t odd = (uint64_t)bad[1] << 32 | bad[0];
-        const float inv_g = 1.0f / (float)G;
 #pragma unroll 1
         for (int i0 = tid; i0 < rows * PIECES; i0 += 4 * 256) {
             float4 v[4];
@@ -429,7 +428,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             for (int k = 0; k < 4; ++k) {
                 const int i = i0 + k * 256, r = i / PIECES, c = i % PIECES;
                 if (i >= rows * PIECES) break;
-                const int rr = row0 + r, tk = (int)(((float)rr + 0.5f) * inv_g);      // rr / G: exact, rr is far below 2^20
+                const int rr = row0 + r, tk = ca_tok(a, rr);
                 float4& y = v[k];
                 if (odd) {                       // new rows' values that are not finite, to a row that sees them
                     for (uint64_t b = (a.mask ? (uint64_t)a.mask[tk] : (2ull << tk) - 1ull) & odd; b; b &= b - 1) {

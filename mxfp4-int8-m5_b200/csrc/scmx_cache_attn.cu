@@ -420,7 +420,9 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
 // A cluster's CTAs join their ranges without a second launch, but they are eight at most: up to so many positions.  Device us, cluster / two launches, 8 key/value
 // heads of 128, one token of two query heads each: 300 positions 5.4 / 6.6, 1500 6.3 / 7.8, 4000 7.6 / 8.7, 6000 8.7 / 9.6, 9000 10.1 / 9.6, 12000 12.0 / 11.7;
 // INT8 1500 6.3 / 7.8, 6000 9.4 / 9.6, 9000 11.2 / 10.4, 12000 12.8 / 11.2.  On the host it is 6 us sooner.
-constexpr int64_t CA_CLUSTER_POSITIONS = 8192;
+// On tcgen05, 8 key/value heads of 128, cluster / two launches: 42 query rows over 1500 positions 10.4 / 10.7, 4000 12.7 / 14.0, 6000 15.0 / 15.9, INT8 4000 14.6 / 14.6,
+// 6000 17.3 / 16.6, 8000 20.5 / 17.6; 84 rows over 4000 16.3 / 15.0, 256 rows 25.3 / 19.9: for tiles that hold copies, and fewer positions.
+constexpr int64_t CA_CLUSTER_POSITIONS = 8192, CA_CLUSTER_POSITIONS_TC = 6144;
 
 static CaPlan ca_plan(int64_t positions, int R, int hk) {
     CaPlan p;
@@ -441,7 +443,7 @@ static CaPlan ca_plan(int64_t positions, int R, int hk) {
     const int64_t most = (positions + p.unit - 1) / p.unit, want = sm_count() / ((int64_t)hk * p.tiles);
     const int64_t s = want < most ? want : most;
     p.nsplit = s < 1 ? 1 : (int)s;
-    if (!p.tc && positions <= CA_CLUSTER_POSITIONS) {
+    if (p.tc ? p.copies > 1 && positions <= CA_CLUSTER_POSITIONS_TC : positions <= CA_CLUSTER_POSITIONS) {
         p.cluster = 1;
         p.nsplit = most >= 8 ? 8 : most >= 3 ? 4 : most == 2 ? 2 : 1;
     }
@@ -459,23 +461,7 @@ static int launch_ca(const CaArgs& a, const CaPlan& p, cudaStream_t st) {
         SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<D, I8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
         configured[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles);
-    cfg.blockDim = dim3(L::THREADS);
-    cfg.dynamicSmemBytes = L::TOTAL;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    if (g_use_pdl) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (p.cluster) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = attr[cfg.numAttrs].val.clusterDim.z = 1;
-        attr[cfg.numAttrs++].val.clusterDim.y = p.nsplit;
-    }
-    SCMX_PDL_OK("cache_attn_kernel", cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, I8, NT>, a));
+    SCMX_PDL_OK("cache_attn_kernel", ca_launch(cache_attn_kernel<D, I8, NT>, a.hk, p, L::THREADS, L::TOTAL, st, a));
     return SCMX_OK;
 }
 template <int D, bool I8>

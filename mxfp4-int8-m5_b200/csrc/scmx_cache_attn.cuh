@@ -103,6 +103,28 @@ __device__ __forceinline__ void ca_join(int count, float& m, float& l, float (&v
 // `rows` query rows in a CTA, `tiles` of them, `nsplit` ranges of positions that are multiples of `unit`.
 struct CaPlan { int tc, nt, copies, rows, tiles, nsplit, unit, cluster; };
 
+// Launches one CTA for every key/value head, range and tile; the ranges of a head as a cluster where they join their states themselves.
+template <typename... KArgs, typename... Args>
+inline cudaError_t ca_launch(void (*kernel)(KArgs...), int hk, const CaPlan& p, int threads, int smem, cudaStream_t st, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)hk, (unsigned)p.nsplit, (unsigned)p.tiles);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (g_use_pdl) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.cluster) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        attr[cfg.numAttrs++].val.clusterDim.y = p.nsplit;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 int cache_attn_tc(const CaArgs& a, const CaPlan& p, int d, int int8, int32_t* status, cudaStream_t st);
 
 }  // namespace scmx

@@ -18,8 +18,11 @@
 // New rows' values that are not finite must not reach rows that do not see them (0 x inf): the threads of a tile that holds new rows clear them
 // in shared memory, with the rows behind the last position, and add them at the end to the rows that see them.
 // Every mbarrier wait is bounded (status word codes 71..76).
+#include <cooperative_groups.h>
 #include "mixers/mix_tc.cuh"
 #include "scmx_cache_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace scmx {
 
@@ -392,8 +395,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         const int64_t first = (((int64_t)kvh * gridDim.z + blockIdx.z) * a.nsplit + split) * ROWS;
         auto state = [](int r, int s) { return MQ == 2 ? r : (s & 1) * 128 + (s >> 1) * RP + r; };
         // a thread to a row: what each of its states is multiplied by (in place of its maximum), the row's maximum and sum
+        float top = -INFINITY, total = 0.0f;
         if (tid < rows) {
-            float top = -INFINITY, total = 0.0f;
 #pragma unroll
             for (int s = 0; s < STATES; ++s) top = fmaxf(top, ml[state(tid, s)].x);
 #pragma unroll
@@ -439,7 +442,9 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                         if ((p[3] & 0x7F80u) == 0x7F80u) y.w += bf16_to_f32(p[3]);
                     }
                 }
-                if (a.part != nullptr) {
+                if (a.cluster) {                 // in place of the row's first state, which no other thread reads here
+                    *reinterpret_cast<float4*>(out + r * L::PITCH + 4 * c) = y;
+                } else if (a.part != nullptr) {
                     *reinterpret_cast<float4*>(a.part + (first + r) * D + 4 * c) = y;
                 } else {
                     const float total = ml[r].y, inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -447,6 +452,10 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                         make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
                 }
             }
+        }
+        if (a.cluster) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (tid < ROWS) ml[tid] = tid < rows ? make_float2(top, total) : make_float2(-INFINITY, 0.0f);
         }
     } else if (I8) {
         set_regs<false, L::CONV_REGS>();
@@ -532,6 +541,21 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (a.cluster) {                     // the ranges' states, read where they lie: the rows in turn to the CTAs, a warp to a row
+        cg::cluster_group cl = cg::this_cluster();
+        cl.sync();
+        constexpr int E = D / 32;
+        const int ctas = (int)cl.num_blocks(), rows = R - row0 < ROWS ? R - row0 : ROWS;
+        float* out = reinterpret_cast<float*>(smem + L::Q_OFF);
+        float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
+        for (int r = (int)cl.block_rank() + ctas * warp; r < rows; r += ctas * (L::THREADS / 32)) {
+            const float2 z = lane < ctas ? cl.map_shared_rank(ml, lane)[r] : make_float2(-INFINITY, 0.0f);
+            float m = z.x, l = z.y, v[E];
+            ca_join<E, 8>(ctas, m, l, v, [&](int s, float (&z)[E]) { ca_load<E>(cl.map_shared_rank(out, s) + r * L::PITCH + lane * E, z); });
+            ca_output<D>(a, kvh, row0 + r, lane, v, l);
+        }
+        cl.sync();                       // nobody leaves while its state may still be read
+    }
     if (*abort_flag) {
         const uint64_t begin = globaltimer_ns();
         while (globaltimer_ns() - begin < 200000ull) __nanosleep(1000);   // 0.2 ms for outstanding TMA writes
@@ -550,8 +574,7 @@ static int launch_ct(const CUtensorMap& k, const CUtensorMap& v, const CaArgs& a
         SCMX_CUDA_OK(cudaFuncSetAttribute(cache_attn_tc_kernel<D, I8, MQ, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
         configured[dev] = true;
     }
-    SCMX_PDL_OK("cache_attn_tc_kernel", launch_pdl(cache_attn_tc_kernel<D, I8, MQ, COPIES>, dim3((unsigned)a.hk, (unsigned)p.nsplit, (unsigned)p.tiles),
-                                                   dim3(L::THREADS), (size_t)L::TOTAL, st, k, v, a, status, g_wait_limit_ns));
+    SCMX_PDL_OK("cache_attn_tc_kernel", ca_launch(cache_attn_tc_kernel<D, I8, MQ, COPIES>, a.hk, p, L::THREADS, L::TOTAL, st, k, v, a, status, (uint64_t)g_wait_limit_ns));
     return SCMX_OK;
 }
 template <int D, bool I8>

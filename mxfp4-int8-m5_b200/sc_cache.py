@@ -107,13 +107,19 @@ def kv_keep(caches, rows, pos=None, pos_dev=None):
         pos, dev = caches[0].offset if pos is None else pos, None
         if not 0 <= pos <= cap - n:
             raise ValueError(f"rows {pos} .. {pos + n} of a cache of {cap}")
-    layers = []
-    for c in caches:
-        own, k, v, ks, vs, size = _tensors(c)
-        if own != int8 or size != shape:
+    layers, here, dt = [], rows.get_device(), _I8 if int8 else _BF16
+    for c in caches:                     # the checks of _tensors, for many layers
+        k, v = c.k, c.v
+        if k.dtype != dt or v.dtype != dt or k.shape != shape or v.shape != shape:
             raise ValueError("kv_keep: caches of one shape and type")
-        layers += (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()) if int8 else (k.data_ptr(), v.data_ptr(), 0, 0)
-    _lib.call("scmx_kv_keep", (ctypes.c_size_t * len(layers))(*layers), len(caches), rows.data_ptr(), n, pos, dev, hk, d, cap, int(int8), _lib.stream())
+        if k.get_device() != here or v.get_device() != here or not (k.is_contiguous() and v.is_contiguous()):
+            _lib.require_here(k, v)
+        if int8:
+            _tensors(c)
+            layers += (k.data_ptr(), v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr())
+        else:
+            layers += (k.data_ptr(), v.data_ptr(), 0, 0)
+    _lib.call("scmx_kv_keep", (ctypes.c_size_t * len(layers))(*layers), len(caches), rows.data_ptr(), n, pos, dev, hk, d, cap, int8, _lib.stream())
 
 
 def attention_supported(hq, hk, d):

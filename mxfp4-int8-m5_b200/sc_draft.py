@@ -45,6 +45,9 @@ class DraftTree:
         return len(self.list)
 
 
+_LOGITS, _PROBS = (torch.bfloat16, torch.float32), (torch.float32,)
+
+
 def _rows(x, what, dtypes):
     if x.dim() != 2 or x.dtype not in dtypes:
         raise ValueError(f"{what} {tuple(x.shape)} {x.dtype}: [rows, vocabulary], {' or '.join(map(str, dtypes))}")
@@ -61,31 +64,32 @@ def verify_draft(logits, tokens, parents, u=None, temperature=1.0, probs=None):
     at the child's token and 0 elsewhere.  At the path's end the token is the first whose cumulative p exceeds u[0].  u float32 [n], uniform in [0, 1).
     So the accepted tokens and the last one are distributed as if the target had chosen each of them.
     temperature 0: greedy (the lowest index of equal logits), u and probs are not read."""
-    logits = _rows(logits, "logits", (torch.bfloat16, torch.float32))
+    logits = _rows(logits, "logits", _LOGITS)
     n, V = logits.shape
     if not 1 <= n <= MAX_ROWS:
         raise ValueError(f"{n} rows (1 .. {MAX_ROWS})")
-    if temperature < 0 or (temperature > 0 and u is None):
-        raise ValueError(f"temperature {temperature}: 0, or positive with random numbers")
     if tokens.dtype != torch.int64 or tokens.numel() != n or parents.dtype != torch.int32 or parents.numel() != n:
         raise ValueError(f"tokens {tuple(tokens.shape)} {tokens.dtype}, parents {tuple(parents.shape)} {parents.dtype}: int64 and int32 [{n}]")
     _lib.require_here(tokens, parents)
     _lib.require_here(logits, contiguous=False)
-    if temperature == 0:
-        u = probs = None
-    if u is not None:
+    numbers = drafts = None
+    ldp = 0
+    if temperature != 0:
+        if u is None or not temperature > 0:
+            raise ValueError(f"temperature {temperature}: 0, or positive with random numbers")
         _lib.require_here(u)
         if u.dtype != torch.float32 or u.numel() != n:
             raise ValueError(f"random numbers {tuple(u.shape)} {u.dtype}: float32 [{n}]")
-    if probs is not None:
-        probs = _rows(probs, "probs", (torch.float32,))
-        _lib.require_here(probs, contiguous=False)
-        if probs.shape != logits.shape:
-            raise ValueError(f"probs {tuple(probs.shape)} for logits {tuple(logits.shape)}")
+        numbers = u.data_ptr()
+        if probs is not None:
+            probs = _rows(probs, "probs", _PROBS)
+            _lib.require_here(probs, contiguous=False)
+            if probs.shape != logits.shape:
+                raise ValueError(f"probs {tuple(probs.shape)} for logits {tuple(logits.shape)}")
+            drafts, ldp = probs.data_ptr(), max(probs.stride(0), V)
     rows, count, token = parents.new_empty(n), parents.new_empty(1), tokens.new_empty(1)
     size = _lib.lib().scmx_verify_scratch(n, V)
     scratch = tokens.new_empty(size // 8)
-    _lib.call("scmx_verify", logits.data_ptr(), logits.dtype == torch.float32, max(logits.stride(0), V), tokens.data_ptr(), parents.data_ptr(), _lib.ptr(u),
-              temperature, _lib.ptr(probs), 0 if probs is None else max(probs.stride(0), V), n, V, rows.data_ptr(), count.data_ptr(), token.data_ptr(),
-              scratch.data_ptr(), size, _lib.stream())
+    _lib.call("scmx_verify", logits.data_ptr(), logits.dtype == torch.float32, max(logits.stride(0), V), tokens.data_ptr(), parents.data_ptr(), numbers,
+              temperature, drafts, ldp, n, V, rows.data_ptr(), count.data_ptr(), token.data_ptr(), scratch.data_ptr(), size, _lib.stream())
     return rows, count, token

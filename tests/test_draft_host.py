@@ -58,7 +58,7 @@ def test_entry_points_refuse(scmx):
         return (q, qhs, qrs, P, P, ks, ks, int8, None, n, pos, None, cap, hq, hk, d, 1.0, P, scratch, size, P, None)
     for kw, text in ((dict(q=None), "null"), (dict(int8=1), "null"), (dict(n=0), "0 rows"), (dict(n=65), "65 rows"), (dict(d=96), "head size"), (dict(hq=5), "hq=5"),
                      (dict(hk=0), "hk=0"), (dict(pos=98), "rows 98"), (dict(pos=-1), "rows -1"), (dict(cap=2), "rows"), (dict(qhs=66), "aligned"),
-                     (dict(q=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(pos=5000, cap=9000, size=8), "scratch"), (dict(pos=5000, cap=9000, scratch=None), "scratch")):
+                     (dict(q=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(pos=50000, cap=90000, size=8), "scratch"), (dict(pos=50000, cap=90000, scratch=None), "scratch")):
         _refused(scmx, "scmx_cache_attn", attn(**kw), text)
     assert scmx._lib.lib().scmx_cache_attn_scratch(5000, 3, 5, 2, 64) == 0
 

@@ -61,6 +61,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
           "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
+// 16 columns of a lane into registers, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Bits of 32 keys, the first `b` positions after the first new row (negative: before it), that a row with these bits sees.
 __device__ __forceinline__ uint32_t ct_seen(uint64_t bits, int b) {
@@ -235,16 +250,18 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             if (I8 && !w) w = mbar_wait(b_sc + 8 * (j & (CT_SCALES - 1)), (j / CT_SCALES) & 1, abort_flag, wait_ns);
             if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 74 : -1; break; }
             tc_fence_after();
-            // scores of piece c: 32 keys, as exponents of 2 once multiplied by sl; unseen ones -inf
+            // scores of piece c: 32 keys in pairs, as exponents of 2 once multiplied by sl; unseen ones -inf
             auto finish = [&](uint32_t (&v)[32], int c) {
                 if constexpr (I8) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 f = *reinterpret_cast<const float4*>(scales + 32 * c + i);
-                        v[i] = __float_as_uint(__uint_as_float(v[i]) * f.x);
-                        v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * f.y);
-                        v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) * f.z);
-                        v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) * f.w);
+                        const float2 x = unpack2(mul2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), pack2(f.x, f.y)));
+                        const float2 y = unpack2(mul2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), pack2(f.z, f.w)));
+                        v[i] = __float_as_uint(x.x);
+                        v[i + 1] = __float_as_uint(x.y);
+                        v[i + 2] = __float_as_uint(y.x);
+                        v[i + 3] = __float_as_uint(y.y);
                     }
                 }
                 if (tail) {
@@ -254,14 +271,22 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                         if (!(seen >> i & 1)) v[i] = 0xFF800000u;
                 }
             };
-            uint32_t r[2][32];
+            constexpr bool HOLD = !I8 || NCH <= 2;      // the scores stay in registers between the two passes; otherwise they are loaded twice
+            uint32_t r[HOLD ? NCH : 2][32];
             float tm = -INFINITY;
-            tmem_ld32(ts + c0, r[0]);
-            tmem_ld_fence(r[0]);
+            if (HOLD) {
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) tmem_ld32(ts + c0 + 32 * c, r[c]);
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) tmem_ld_fence(r[c]);
+            } else {
+                tmem_ld32(ts + c0, r[0]);
+                tmem_ld_fence(r[0]);
+            }
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                uint32_t(&v)[32] = r[c & 1];
-                if (c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
+                uint32_t(&v)[32] = r[HOLD ? c : c & 1];
+                if (!HOLD && c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
                 finish(v, c);
                 float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
@@ -270,7 +295,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                     m1 = fmaxf(m1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
                 }
                 tm = fmaxf(tm, fmaxf(m0, m1));
-                if (c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
+                if (!HOLD && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
             }
             const bool first = u == m, grow = first || (tm - mx) * sl > CA_GROWTH;
             if (__any_sync(0xffffffffu, grow)) {
@@ -278,26 +303,27 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 mx = mn;
                 if (!first) {      // S complete implies the stream's last product complete: MMAs of one thread finish in order
                     sum *= f;
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(to + 32 * c, v);
-                        tmem_ld_fence(v);
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {      // few registers: the scores wait in theirs
+                        uint32_t v[16];
+                        tmem_ld16(to + 16 * c, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st32(to + 32 * c, v);
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st16(to + 16 * c, v);
                     }
                 }
             }
             const float off = -mx * sl;
-            float s0 = 0.0f, s1 = 0.0f;
-            if (NCH > 2) {
+            const uint64_t sl2 = pack2(sl, sl), off2 = pack2(off, off);
+            uint64_t s2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+            if (!HOLD) {
                 tmem_ld32(ts + c0, r[0]);
                 tmem_ld_fence(r[0]);
             }
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                uint32_t(&v)[32] = r[c & 1];
-                if (NCH > 2) {
+                uint32_t(&v)[32] = r[HOLD ? c : c & 1];
+                if (!HOLD) {
                     if (c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
                     finish(v, c);
                 }
@@ -307,12 +333,17 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 for (int i = 0; i < 32; i += 4) {
                     float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = ex2_approx(fmaf(__uint_as_float(v[i + e]), sl, off));
-                    s0 += x[0] + x[1];
-                    s1 += x[2] + x[3];
+                    for (int e = 0; e < 4; e += 2) {
+                        const uint64_t z = pack2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
+                        const float2 y = unpack2(I8 ? add2(z, off2) : fma2(z, sl2, off2));
+                        x[e] = ex2_approx(y.x);
+                        x[e + 1] = ex2_approx(y.y);
+                        s2[e / 2] = add2(s2[e / 2], pack2(x[e], x[e + 1]));
+                    }
                     if constexpr (I8) {
                         const float4 f = *reinterpret_cast<const float4*>(scales + 128 + 32 * c + i);
-                        x[0] *= f.x; x[1] *= f.y; x[2] *= f.z; x[3] *= f.w;
+                        const float2 y = unpack2(mul2(pack2(x[0], x[1]), pack2(f.x, f.y))), w = unpack2(mul2(pack2(x[2], x[3]), pack2(f.z, f.w)));
+                        x[0] = y.x; x[1] = y.y; x[2] = w.x; x[3] = w.y;
                         if (tail)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
@@ -321,9 +352,10 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                     pk[i / 2] = pack_bf16x2(x[0], x[1]);
                     pk[i / 2 + 1] = pack_bf16x2(x[2], x[3]);
                 }
-                if (NCH > 2 && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
+                if (!HOLD && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
                 tmem_st16(ts + c0 / 2 + 16 * c, pk);
             }
+            const float2 sum0 = unpack2(s2[0]), sum1 = unpack2(s2[1]);
             if (COPIES > 1) {            // weights of the other copies' keys
                 uint32_t z[16];
 #pragma unroll
@@ -332,7 +364,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 for (int c = 0; c < 4; ++c)
                     if (c / NCH != copy) tmem_st16(ts + 16 * c, z);
             }
-            sum += s0 + s1;
+            sum += (sum0.x + sum0.y) + (sum1.x + sum1.y);
             tmem_st_wait();
             tc_fence_before();
             if (!I8 && tail && (MQ == 1 || m == 0)) {      // a thread per position

@@ -1,11 +1,14 @@
 // INT8 key/value cache: vectors of new tokens are quantized as they are written, cached rows are read back as bfloat16, and the rows of
 // accepted drafts are moved together.  A head's vector at one position has one float32 scale: s = amax / 127, code = rint(x (1 / s)),
-// the recipe of the activations' INT8.  Bound by memory: every value is loaded and stored once, 16 bytes a load.
+// the recipe of the activations' INT8.  Bound by memory: every value is loaded and stored once.  Measured on a B200: 2048 tokens of 8 heads
+// of 128 written and read back in 7.2 us (two launches and 21 MB that stay in L2); 333 tokens written behind 29667 and all 30000 of 16
+// heads read back in 60.1 us, 375 MB at 6.2 TB/s.  With 1, 2 and 4 vectors of a thread in flight the two take 7.8, 7.2, 7.5 us and 61.1, 60.1,
+// 61.1 us.  A call for one token is its launch, 1.5 us.
 #include "scmx_common.cuh"
 
 namespace scmx {
 
-constexpr int KV_THREADS = 256, KV_TURNS = 4;      // vectors of a thread whose loads are in flight together
+constexpr int KV_THREADS = 256, KV_TURNS = 2;      // vectors of a thread whose loads are in flight together
 
 struct KvWriteArgs {
     const uint16_t *k, *v;           // bf16 [hk, L, d]
@@ -70,7 +73,8 @@ struct KvReadArgs {
     int hk, d, pieces, rows;         // pieces of 16 values of a vector; vectors that a CTA takes in a turn
 };
 
-// A lane takes 16 codes; codes become bfloat16 exactly, and their product with the scale is rounded once.
+// A lane takes 16 codes; codes become bfloat16 exactly, and their product with the scale is rounded once.  Its 32 bytes leave in one store: two
+// stores of 16 each fill half a sector, and reading 30000 positions takes 77 us instead of 60.
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvReadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
@@ -105,9 +109,9 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
                 o[2 * j] = pack_bf16x2(__fmul_rn(bf16_lo(even), s[i]), __fmul_rn(bf16_lo(odd), s[i]));
                 o[2 * j + 1] = pack_bf16x2(__fmul_rn(bf16_hi(even), s[i]), __fmul_rn(bf16_hi(odd), s[i]));
             }
-            uint4* p = reinterpret_cast<uint4*>(out + row * a.d);
-            p[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + row * a.d), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]),
+                         "r"(o[5]), "r"(o[6]), "r"(o[7])
+                         : "memory");
         }
     }
 }
@@ -196,7 +200,8 @@ extern "C" int scmx_kv_read(const int8_t* k_codes, const float* k_scales, const 
     SCMX_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, SCMX_EINVAL, "kv_read: head size %d (a multiple of 16 up to 256)", d);
     if (n == 0) return SCMX_OK;
     SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_read: null buffer");
-    SCMX_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_read: buffers must be 16-byte aligned");
+    SCMX_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 32 == 0 && aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL,
+                 "kv_read: codes must be 16-byte aligned, outputs 32-byte");
     KvReadArgs a;
     a.kc = k_codes; a.vc = v_codes; a.ks = k_scales; a.vs = v_scales; a.k = k; a.v = v;
     a.start = start; a.cap = capacity; a.n = n; a.hk = hk; a.d = d; a.pieces = d / 16; a.rows = KV_THREADS / a.pieces;

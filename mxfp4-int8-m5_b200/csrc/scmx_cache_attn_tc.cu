@@ -18,6 +18,13 @@
 // New rows' values that are not finite must not reach rows that do not see them (0 x inf): the threads of a tile that holds new rows clear them
 // in shared memory, with the rows behind the last position, and add them at the end to the rows that see them.
 // Every mbarrier wait is bounded (status word codes 71..76).
+//
+// Measured on a B200 (8 key/value heads of 128): 60000 bfloat16 positions 45.2 us with 18 query rows (5.4 TB/s), 51.5 with 128, 68 with 256; INT8 48,
+// 61 and 101 us.  bfloat16 up to 128 rows waits for memory.  A pair of units of 256 rows takes 3400 cycles, and its bytes arrive in 2800: a stream's
+// scores, softmax (2050 cycles, half of them the exponentials' rate) and product follow on one another, and two streams are what tensor memory
+// holds.  A second softmax thread per row, or a third of the exponentials from a cubic, changed less than 2 %.  INT8 adds the scales' products and the
+// conversions, which share the issue slots: 6000 cycles for a pair.  Weights in halves against whole tiles: 256 rows 72 -> 70 us, INT8 65 -> 62 us at
+// 128 rows; for bfloat16 at 128 rows, which has its two streams on different tiles, 16.9 -> 17.6 us at 8000 positions, so there they stay whole.
 #include <cooperative_groups.h>
 #include "mixers/mix_tc.cuh"
 #include "scmx_cache_attn.cuh"
@@ -40,10 +47,10 @@ struct CtSmem {
     static constexpr int V_OFF = K_OFF + KS * KB * CT_TILE;
     static constexpr int SC_OFF = V_OFF + VS * KB * CT_TILE;                  // scales: [CT_SCALES][keys, values][128] float
     static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
-    // kfull, kempty [KS], vfull, vempty [VS], scales [CT_SCALES], S, P, O [2], queries
-    static constexpr int NBAR = 2 * KS + 2 * VS + (I8 ? CT_SCALES : 0) + 7;
+    // kfull, kempty [KS], vfull, vempty [VS], scales [CT_SCALES], S [2], P [2][halves], O [2], queries
+    static constexpr int NBAR = 2 * KS + 2 * VS + (I8 ? CT_SCALES : 0) + 9;
     // threads; INT8: registers of a thread by role, together no more than the block is launched with
-    static constexpr int THREADS = I8 ? 640 : 320, LAUNCH_REGS = 96, SOFT_REGS = 128, CONV_REGS = 72, MISC_REGS = 72;
+    static constexpr int THREADS = I8 ? 640 : 320, LAUNCH_REGS = 96, SOFT_REGS = 136, CONV_REGS = 72, MISC_REGS = 56;
     static_assert(256 * SOFT_REGS + 256 * CONV_REGS + 128 * MISC_REGS <= 640 * LAUNCH_REGS, "registers of a block");
     static constexpr int MISC_OFF = BAR_OFF + 8 * NBAR;
     static constexpr int TOTAL = MISC_OFF + 32 + 1024;
@@ -98,11 +105,12 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     using L = CtSmem<D, I8, MQ>;
     constexpr int KB = L::KB, KS = L::KS, VS = L::VS;
     constexpr int RP = 128 / COPIES, ROWS = MQ * RP, NCH = 4 / COPIES;      // rows of a tile, of the CTA; 32-key pieces of a thread
+    constexpr int HALVES = COPIES == 1 && (I8 || MQ == 2) ? 2 : 1;      // weights handed over in halves: the first's product runs while the second is computed
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BAR_OFF;
     const uint32_t b_kf = bars, b_ke = b_kf + 8 * KS, b_vf = b_ke + 8 * KS, b_ve = b_vf + 8 * VS, b_sc = b_ve + 8 * VS, b_s = b_sc + (I8 ? 8 * CT_SCALES : 0),
-                   b_p = b_s + 16, b_o = b_p + 16, b_q = b_o + 16;
+                   b_p = b_s + 16, b_o = b_p + 32, b_q = b_o + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 4);
     uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::MISC_OFF + 8);      // new rows with values that are not finite
@@ -116,7 +124,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         for (int i = 0; i < L::NBAR; ++i) {
             const uint32_t b = bars + 8 * i;
             const bool converted = I8 && ((b >= b_kf && b < b_ke) || (b >= b_vf && b < b_ve) || (b >= b_sc && b < b_s));      // one arrival per converting warp
-            mbar_init(b, b == b_q || converted ? 8 : b == b_p || b == b_p + 8 ? 4 : 1);                                     // weights: one per softmax warp
+            mbar_init(b, b == b_q || converted ? 8 : b >= b_p && b < b_o ? 4 : 1);                                          // weights: one per softmax warp
         }
         *abort_flag = 0;
         bad[0] = bad[1] = 0;
@@ -188,12 +196,17 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         if (ok && units > 1) ok = scores(1);
         for (int u = 0; u < units && ok; ++u) {
             const int m = u & 1, j = MQ == 2 ? u >> 1 : u, vs = j % VS;
-            if (!(ok = wait(b_p + 8 * m, (u >> 1) & 1, 73))) break;
-            if (j != vt && !(ok = wait(b_vf + 8 * vs, (j / VS) & 1, 72))) break;
-            vt = j;
             const uint64_t dv = umma_desc_mn(sbase + L::V_OFF + vs * KB * CT_TILE, CT_TILE);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) umma_bf16_ts(on, tmem + 256 + 128 * m, tmem + 128 * m + 8 * k, dv + 128 * k, idesc_o, k > 0 ? 1u : (uint32_t)(u > 1));
+            for (int h = 0; h < HALVES && ok; ++h) {
+                if (!(ok = wait(b_p + 16 * m + 8 * h, (u >> 1) & 1, 73))) break;
+                if (h == 0 && j != vt && !(ok = wait(b_vf + 8 * vs, (j / VS) & 1, 72))) break;
+                vt = j;
+#pragma unroll
+                for (int k = 8 / HALVES * h; k < 8 / HALVES * (h + 1); ++k)
+                    umma_bf16_ts(on, tmem + 256 + 128 * m, tmem + 128 * m + 8 * k, dv + 128 * k, idesc_o, k > 0 ? 1u : (uint32_t)(u > 1));
+            }
+            if (!ok) break;
             if (MQ == 1 || m == 1) umma_commit(on, b_ve + 8 * vs);
             if (u + 2 >= units) umma_commit(on, b_o + 8 * m);
             else ok = scores(u + 2);
@@ -232,9 +245,11 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(b_q);
         }
-        const int m = warp >> 2, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = ca_tok(a, row);
+        const int m = warp >> 2 & 1, zero = warp >> 3, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = ca_tok(a, row);
         const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
-        const int c0 = copy * (128 / COPIES);                   // the thread's first key of a tile
+        // The thread's first key of a tile.  `zero` keeps it from being a constant with one copy, where the compiler then orders the loads of the two
+        // streams worse (60000 positions, 256 rows, bfloat16 70.3 us and not 68.2, INT8 109 and not 101)
+        const int c0 = copy * (128 / COPIES) + zero * 64;
         uint64_t bits = 0;
         if (row < R) {
             bits = a.mask ? (uint64_t)a.mask[tok] : (2ull << tok) - 1ull;
@@ -301,8 +316,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             if (__any_sync(0xffffffffu, grow)) {
                 const float mn = grow ? fmaxf(mx, tm) : mx, f = ex2_approx((mx - mn) * sl);
                 mx = mn;
+                if (!first) sum *= f;
                 if (!first) {      // S complete implies the stream's last product complete: MMAs of one thread finish in order
-                    sum *= f;
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {      // few registers: the scores wait in theirs
                         uint32_t v[16];
@@ -313,6 +328,13 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                     }
                 }
             }
+            const bool clear = !I8 && tail;                     // values are cleared first
+            auto hand_over = [&](int h) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_p + 16 * m + 8 * h);
+            };
             const float off = -mx * sl;
             const uint64_t sl2 = pack2(sl, sl), off2 = pack2(off, off);
             uint64_t s2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
@@ -354,6 +376,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 }
                 if (!HOLD && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
                 tmem_st16(ts + c0 / 2 + 16 * c, pk);
+                if (HALVES == 2 && c == NCH / 2 - 1 && !clear) hand_over(0);
             }
             const float2 sum0 = unpack2(s2[0]), sum1 = unpack2(s2[1]);
             if (COPIES > 1) {            // weights of the other copies' keys
@@ -365,9 +388,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                     if (c / NCH != copy) tmem_st16(ts + 16 * c, z);
             }
             sum += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-            tmem_st_wait();
-            tc_fence_before();
-            if (!I8 && tail && (MQ == 1 || m == 0)) {      // a thread per position
+            if (clear && (MQ == 1 || m == 0)) {      // a thread per position
                 w = mbar_wait(b_vf + 8 * (j % VS), (j / VS) & 1, abort_flag, wait_ns);
                 if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 74 : -1; break; }
                 const int d = d0 + l;
@@ -396,8 +417,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 }
                 proxy_fence();
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_p + 8 * m);
+            if (HALVES == 2 && clear) hand_over(0);
+            hand_over(HALVES - 1);
         }
         // both streams' products are complete before the operands' memory is used again
         if (fail == 0) {

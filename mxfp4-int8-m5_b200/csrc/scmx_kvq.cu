@@ -126,7 +126,8 @@ struct KvKeepArgs {
     int n, row_bytes;
 };
 
-// One CTA per (head, layer, keys or values): every kept row is loaded before the first one is stored, so rows may change places.
+// One CTA per (head, layer, keys or values): every kept row is loaded before the first one is stored, so rows may change places.  Bound by its
+// launch and two dependent loads: 3 rows in 16 layers 2.8 us, 9 rows in 28 layers 4.2 us.
 __global__ void __launch_bounds__(KEEP_THREADS) kv_keep_kernel(const __grid_constant__ KvKeepArgs a) {
     constexpr int PER = KEEP_ROWS * 32 / KEEP_THREADS;      // 16-byte pieces of a thread: rows of 512 bytes at most
     pdl_launch_dependents();

@@ -276,13 +276,15 @@ class LookupDraft:
 
     def __call__(self, text, most):
         rows, parents, children = [text[-1]], [-1], {}
+        last = text[-1]
+        ends = [i for i in range(len(text) - 1, 0, -1) if text[i - 1] == last]      # behind each earlier place of the last token, the latest first
         for m in range(min(self.match, len(text) - 1), 0, -1):
             tail, found = text[-m:], 0
-            for i in range(len(text) - m - 1, -1, -1):
-                if text[i:i + m] != tail:
+            for e in ends:
+                if e < m or text[e - m:e] != tail:
                     continue
                 at = 0
-                for t in text[i + m:i + m + self.length]:
+                for t in text[e:e + self.length]:
                     nxt = children.get((at, t))
                     if nxt is None:
                         if len(rows) >= most:
@@ -304,7 +306,10 @@ class DecodeDraft:
     keeps a path of them and draws the token after it, distributed as the model alone would draw (greedy at temperature 0).
 
     propose(tokens so far, most rows) -> (tokens, parents) or (tokens, parents, probs): sc_draft.DraftTree's lists with row 0 the last token, and probs float32
-    [rows, vocabulary] on the device where children were drawn from them (row i: what row i's children were drawn from)."""
+    [rows, vocabulary] on the device where children were drawn from them (row i: what row i's children were drawn from).
+
+    Where the model reads that many rows on digit planes (nothing beside the current stream, no buffers of its own), the second pass of as many rows
+    over a cache is captured and later ones are replays: the launches of a pass over 28 layers take the host 4.5 ms."""
 
     def __init__(self, fused, propose=None):
         a = fused.args
@@ -312,6 +317,7 @@ class DecodeDraft:
             raise ValueError(f"attention of drafted rows: head size {a.head_dim} (64 or 128)")
         self.f, self.propose = fused, propose or LookupDraft()
         self.dev = fused.inv_freq.device
+        self._graphs = None                                       # (cache, memory pool, {(rows, temperature): captured pass})
 
     @torch.no_grad()
     def read(self, tokens, tree, cache):
@@ -319,26 +325,83 @@ class DecodeDraft:
         h = self.f.hidden(tokens.view(1, -1), cache, tree)
         return self.f.logits(h)[0]
 
-    @torch.no_grad()
-    def keep(self, cache, rows, count):
-        """The accepted rows (verify_draft's list) become the cache's next ones; count: how many, on the host."""
-        C.kv_keep(cache, rows)
+    def _pass(self, tok, tree, cache, u, temperature, probs):
+        """A tree read, verified and its accepted rows moved -> int64 [n + 1]: the accepted rows (padded with -1), and the token after them."""
+        logits = self.read(tok, tree, cache)
+        rows, _, token = D.verify_draft(logits, tok, tree.parents, u, temperature, probs)
+        C.kv_keep(cache, rows, pos_dev=tree.pos)
+        return torch.cat((rows.long(), token))
+
+    def _captured(self, tokens, parents, cache, u, temperature):
+        """_pass as a replay, or None where it runs launch by launch."""
+        n, f, a = len(tokens), self.f, self.f.args
+        if not f._f4(n) or (cache[0].k.dtype == torch.int8 and a.num_attention_heads + 2 * a.num_key_value_heads > 96):
+            return None
+        if self._graphs is None or self._graphs[0] is not cache or len(self._graphs[2]) >= 128:      # (128: temperatures that keep changing)
+            self._graphs = (cache, torch.cuda.graph_pool_handle(), {})
+        _, pool, known = self._graphs
+        key = (n, float(temperature))
+        if key not in known:
+            known[key] = None
+            return None
+        values = torch.tensor([*tokens, *D.mask_bits(parents), *parents, *D.draft_depths(parents), cache[0].offset], dtype=torch.int64)
+        if known[key] is None:
+            known[key] = self._capture(parents, cache, temperature, values.to(self.dev), u, pool)
+        g, inputs, numbers, out = known[key][:4]
+        inputs.copy_(values)
+        if numbers is not None:
+            numbers.copy_(u)
+        g.replay()
+        return out
+
+    def _capture(self, parents, cache, temperature, inputs, u, pool):
+        """(graph, its inputs int64 [4 n + 1]: tokens, mask, parents, depths, position; its random numbers; its result; what it reads).  The warm-up is this very pass."""
+        n = len(parents)
+        tree, ints, out = D.DraftTree(parents, self.dev), torch.empty(2 * n + 1, dtype=torch.int32, device=self.dev), torch.empty(n + 1, dtype=torch.int64, device=self.dev)
+        tok, tree.mask, (tree.parents, tree.depths, tree.pos) = inputs[:n], inputs[n:2 * n], ints.split((n, n, 1))
+        numbers = None if u is None else u.clone()
+
+        def run():
+            ints.copy_(inputs[2 * n:])
+            out.copy_(self._pass(tok, tree, cache, numbers, temperature, None))
+
+        offsets = [c.offset for c in cache]
+        s = torch.cuda.Stream(device=self.dev)
+        s.wait_stream(torch.cuda.current_stream())
         for c in cache:
-            c.offset += count
+            c.offset = 0                                          # rows and rotary positions come from the position on the device
+        try:
+            with torch.cuda.stream(s):
+                run()
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s, pool=pool):
+                    run()
+        finally:
+            for c, o in zip(cache, offsets):
+                c.offset = o
+        torch.cuda.current_stream().wait_stream(s)
+        return g, inputs, numbers, out, tree, ints
 
     @torch.no_grad()
     def step(self, text, cache, temperature=0.0, u=None, most=D.MAX_ROWS):
         """One pass: text (list of ids, the last one not in the cache yet) -> the tokens that it adds, at least one.  u float32 [64]: random numbers in [0, 1)."""
         assert cache[0].offset + 1 <= cache[0].capacity, "KV cache capacity exceeded"
-        tokens, parents, *probs = self.propose(text, max(1, min(most, D.MAX_ROWS, cache[0].capacity - cache[0].offset)))
-        tree, tok = D.DraftTree(parents, self.dev), torch.tensor(tokens, dtype=torch.int64, device=self.dev)
-        n = len(tree)
-        assert tok.numel() == n and tokens[0] == text[-1], "a tree's first row is the last token"
-        logits = self.read(tok, tree, cache)
-        rows, count, token = D.verify_draft(logits, tok, tree.parents, None if u is None else u[:n], temperature, probs[0] if probs else None)
-        path, last = rows.tolist(), int(token)
+        most = max(1, min(most, D.MAX_ROWS, cache[0].capacity - cache[0].offset))
+        tokens, parents, *probs = self.propose(text, most)
+        tokens, parents = [int(t) for t in tokens], D.check_tree(parents)
+        n = len(tokens)
+        if n != len(parents) or n > most or tokens[0] != text[-1]:
+            raise ValueError(f"a draft of {n} tokens and {len(parents)} parents: as many of both, {most} at most, the first token the text's last")
+        u = None if u is None or not temperature else u[:n]
+        probs = probs[0] if probs else None
+        out = self._captured(tokens, parents, cache, u, temperature) if probs is None else None
+        if out is None:
+            out = self._pass(torch.tensor(tokens, dtype=torch.int64, device=self.dev), D.DraftTree(parents, self.dev), cache, u, temperature, probs)
+        *path, last = out.tolist()
         path = [r for r in path if r >= 0]
-        self.keep(cache, rows, len(path))
+        for c in cache:
+            c.offset += len(path)
         return [tokens[r] for r in path[1:]] + [last]
 
     @torch.no_grad()

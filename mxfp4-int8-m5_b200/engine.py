@@ -31,6 +31,7 @@ class Engine:
         make = bundle.prefill.make_cache
         self.pool = CachePool(make if cache_dtype is None else lambda capacity: make(capacity, cache_dtype), max(1, max_tokens))
         self.live = {}
+        self.drafts = None                                        # decode.DecodeDraft, with its captured passes
 
     def start(self, rid):
         if rid not in self.live:
@@ -72,7 +73,10 @@ class Engine:
         first = logits[-1].argmax().reshape(1, 1)
         out = [int(first)]
         if n > 1 and draft is not None:
-            out += DEC.DecodeDraft(self.bundle.prefill, draft).generate(first, self.live[rid], n - 1, prompt).tolist()
+            if self.drafts is None:
+                self.drafts = DEC.DecodeDraft(self.bundle.prefill)
+            self.drafts.propose = draft
+            out += self.drafts.generate(first, self.live[rid], n - 1, prompt).tolist()
         elif n > 1:
             out += self.bundle.decode.generate(first, self.live[rid], n - 1).tolist()
         self.finish(rid)

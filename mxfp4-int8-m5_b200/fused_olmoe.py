@@ -216,9 +216,10 @@ class FusedOlmoe:
         a = self.args
         tree = self._tree
         q, k, v = S.qkv_fullnorm_y(y, at.q_norm.weight, at.k_norm.weight, self.eps, L, a.num_attention_heads, a.head_dim,
-                                   rope=(self.inv_freq, c.offset, self.rope_cs), cache=c, row_pos=None if tree is None else tree.depths)
+                                   rope=(self.inv_freq, c.offset, self.rope_cs), cache=c, row_pos=None if tree is None else tree.depths,
+                                   pos_dev=None if tree is None else tree.pos)
         if tree is not None:                                  # the rows stay behind the cache's end until some are kept
-            o = C.cache_attention(q, c, at.scale, tree.mask)
+            o = C.cache_attention(q, c, at.scale, tree.mask, tree.pos)
             return S.quant_digits(o) if digits else S.act_quant(o, Mp)
         c.offset += L
         if k is None:                                         # an INT8 cache: what it holds

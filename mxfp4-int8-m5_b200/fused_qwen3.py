@@ -157,7 +157,7 @@ class FusedQwen3:
         hq, hk, d = a.num_attention_heads, a.num_key_value_heads, a.head_dim
         kw = dict(rope=(self.inv_freq, c.offset, self.rope_cs), cache=c) if self.fuse_rope or self._tree is not None else {}
         if self._tree is not None:
-            kw["row_pos"] = self._tree.depths
+            kw.update(row_pos=self._tree.depths, pos_dev=self._tree.pos)
         if src.dtype == torch.int32:
             q, k, v = S.qkv_epilogue_headnorm(src, xs, ws, at.q_norm.weight, at.k_norm.weight, self.eps, L, hq, hk, d, **kw)
         else:
@@ -177,7 +177,7 @@ class FusedQwen3:
         """-> attention output (None unless it is recorded), its INT8 rows and their scales."""
         q, k, v = self._qkv(at, c, src, xs, ws, L)
         if self._tree is not None:
-            o = C.cache_attention(q, c, at.scale, self._tree.mask)
+            o = C.cache_attention(q, c, at.scale, self._tree.mask, self._tree.pos)
             return (o, *self.act_q(o, Mp))
         own = type(self).act_q is not _ACT_Q or "act_q" in self.__dict__      # a quantizer of the caller's: it wants whole rows
         if own or self.rot is True or (self.record is not None and i in self.record_layers):
@@ -215,7 +215,7 @@ class FusedQwen3:
             if self._tree is None:
                 rows = attend_quant(self.sdpa, q, k, v, at.scale, L, digits=True)
             else:
-                rows = S.quant_digits(C.cache_attention(q, cache[i], at.scale, self._tree.mask))
+                rows = S.quant_digits(C.cache_attention(q, cache[i], at.scale, self._tree.mask, self._tree.pos))
             h = mm("o", *rows, 2, h)
             act = mm("gu", *S.quant_digits(h, layer.post_attention_layernorm.weight, self.eps), 3)
             h = mm("down", *S.quant_digits(act), 2, h)

@@ -16,12 +16,17 @@ def check_tree(parents):
     return parents
 
 
-def draft_mask(parents, device="cuda"):
-    """int64 [n]: bit j of entry i is set where j is row i's ancestor or i itself (sc_cache.cache_attention)."""
+def mask_bits(parents):
+    """draft_mask's entries as a list."""
     bits = []
     for i, p in enumerate(check_tree(parents)):
         bits.append((bits[p] if i else 0) | 1 << i)
-    return torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], dtype=torch.int64, device=device)
+    return [b - (1 << 64) if b >> 63 else b for b in bits]
+
+
+def draft_mask(parents, device="cuda"):
+    """int64 [n]: bit j of entry i is set where j is row i's ancestor or i itself (sc_cache.cache_attention)."""
+    return torch.tensor(mask_bits(parents), dtype=torch.int64, device=device)
 
 
 def draft_depths(parents):
@@ -33,10 +38,13 @@ def draft_depths(parents):
 
 
 class DraftTree:
-    """A tree's parents, and what the kernels read of it, on the device: parents int32 [n], mask (draft_mask) and depths int32 [n] (draft_depths)."""
-    __slots__ = ("list", "parents", "mask", "depths")
+    """A tree's parents, and what the kernels read of it, on the device: parents int32 [n], mask (draft_mask) and depths int32 [n] (draft_depths).  pos, if set: one
+    device int32, the cache row of the tree's first row; it is added to the caches' offsets where keys are written, and read in their place by
+    the attention, so that a captured pass can be replayed (caches at offset 0 then)."""
+    __slots__ = ("list", "parents", "mask", "depths", "pos")
 
     def __init__(self, parents, device="cuda"):
+        self.pos = None
         self.list = check_tree(parents)
         self.mask = draft_mask(self.list, device)
         self.parents, self.depths = torch.tensor([self.list, draft_depths(self.list)], dtype=torch.int32, device=device).unbind()

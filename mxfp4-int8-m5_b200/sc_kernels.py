@@ -302,12 +302,13 @@ def _qkv_norm(src, xscale, wscale, qn, kn, eps, L, hq, hk, d, full, rope, cache,
 
 
 def qkv_epilogue_headnorm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, dtype=torch.bfloat16, deps=(), rope=None,
-                          cache=None, row_pos=None):
+                          cache=None, row_pos=None, pos_dev=None):
     """acc int32 [Mp, (hq + 2 hk) d] -> q [hq, L, d], k [hk, L, d], v [hk, L, d] with per-head RMSNorm of q and k.
     rope=(inv_freq, pos0[, rope_table]): rotary embedding of q and k at positions pos0.. in the same kernel; cache (with .k, .v
     [hk, capacity, d] and .offset): k and v are written into the cache rows and the filled prefix is returned (None for an INT8 cache, host_model.QuantKVCache:
-    sc_cache.kv_read has it).  row_pos int32 [L]: row r turns as position pos0 + row_pos[r]."""
-    return _qkv_norm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, False, rope, cache, None, row_pos)
+    sc_cache.kv_read has it).  row_pos int32 [L]: row r turns as position pos0 + row_pos[r].  pos_dev: one device int32 added to pos0 and
+    to the cache rows."""
+    return _qkv_norm(acc, xscale, wscale, qn, kn, eps, L, hq, hk, d, False, rope, cache, pos_dev, row_pos)
 
 
 def qkv_headnorm_y(y, qn, kn, eps, L, hq, hk, d, deps=(), rope=None, cache=None, pos_dev=None, row_pos=None):

@@ -196,6 +196,59 @@ def test_drafted_generation_is_the_models(scmx, kind, dtype):
     scmx._lib.check_status()
 
 
+@pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
+@pytest.mark.parametrize("dtype", [None, torch.int8])
+def test_replayed_passes(scmx, kind, dtype):
+    """Passes of as many rows are replays from the second one on.  Trees, tokens and positions change between them: the rows that stay in the first layer's cache, which
+    no attention has touched, are those of a pass launch by launch, and every token is the model's choice."""
+    fused, _ = build(scmx, kind)
+    DEC = mod(scmx, "decode")
+    rng = random.Random(3)
+    prompt = [rng.randrange(512) for _ in range(30)]
+    caches = [fused.make_cache(110, dtype) for _ in range(2)]
+    for c in caches:
+        fused.hidden(torch.tensor([prompt], device="cuda"), c)
+    drawn = {}
+
+    def propose(text, most):
+        if len(text) not in drawn:
+            n = min(most, rng.choice([1, 6, 6, 6, 17]))
+            drawn[len(text)] = [text[-1]] + [rng.randrange(512) for _ in range(n - 1)], [-1] + [rng.randrange(i) for i in range(1, n)]
+        return drawn[len(text)]
+    d, plain = DEC.DecodeDraft(fused, propose), DEC.DecodeDraft(fused, propose)
+    plain._captured = lambda *a: None
+    text, out = prompt + [7], []
+    tensors = lambda c: (c.k, c.v) + ((c.ks, c.vs) if dtype else ())      # noqa: E731
+    layer = lambda c, n: [t[:, :n] for t in tensors(c[0])]                # noqa: E731
+    while len(text) < 80:
+        new = d.step(text, caches[0])
+        plain.step(text, caches[1])
+        n = len(text)
+        assert all(torch.equal(x, y) for x, y in zip(layer(caches[0], n), layer(caches[1], n)))
+        text, out = text + new, out + new
+        for x, y in zip(*caches):                                 # the same text whatever rounding chose
+            for a, b in zip(tensors(x), tensors(y)):
+                b.copy_(a)
+            y.offset = x.offset
+    replayed = [k for k, g in d._graphs[2].items() if g is not None]
+    assert (6, 0.0) in replayed and caches[0][0].offset == len(text) - 1
+    assert margins(fused, prompt + [7], out, dtype) < MARGIN
+    # the end of the cache, another cache, and a draft of too many rows
+    rest = d.generate(torch.tensor([[text[-1]]], device="cuda"), caches[0], 110 - caches[0][0].offset, text[:-1])
+    assert caches[0][0].offset == 110 and rest.numel() == 110 - len(text) + 1
+    with pytest.raises(AssertionError, match="capacity"):
+        d.step(text + rest.tolist(), caches[0])
+    for c in caches[1]:
+        c.offset = len(prompt)
+    drawn.clear()
+    again = d.generate(torch.tensor([[7]], device="cuda"), caches[1], 20, prompt).tolist()
+    assert margins(fused, prompt + [7], again, dtype) < MARGIN
+    wide = DEC.DecodeDraft(fused, lambda t, most: ([t[-1]] * (most + 1), [-1] + [0] * most))
+    with pytest.raises(ValueError, match="draft"):
+        wide.step([1, 2], caches[1])
+    scmx._lib.check_status()
+
+
 def test_sampled_generation_repeats_with_its_generator(scmx):
     fused, _ = build(scmx, "qwen3")
     DEC = mod(scmx, "decode")

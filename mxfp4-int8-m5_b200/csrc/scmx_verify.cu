@@ -600,7 +600,7 @@ extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int
                  (long long)ld, (long long)ldp);
     SCMX_REQUIRE(logits && tokens && parents && rows && count && token, SCMX_EINVAL, "verify: null buffer");
     const bool greedy = temperature == 0.0f;
-    SCMX_REQUIRE(greedy || (temperature > 0.0f && temperature <= 3.0e38f && 1.0f / temperature <= 3.0e38f), SCMX_EINVAL, "verify: temperature %g", (double)temperature);
+    SCMX_REQUIRE(greedy || (temperature > 0.0f && temperature <= 3.0e38f && 1.45f / temperature <= 3.0e38f), SCMX_EINVAL, "verify: temperature %g", (double)temperature);
     SCMX_REQUIRE(greedy || u != nullptr, SCMX_EINVAL, "verify: sampling needs random numbers");
     SCMX_REQUIRE(((uintptr_t)logits & (is_f32 ? 3 : 1)) == 0 && ((uintptr_t)probs & 3) == 0, SCMX_EINVAL, "verify: unaligned buffer");
     const int64_t need = scmx_verify_scratch(n, V);

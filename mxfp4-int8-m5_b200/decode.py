@@ -393,7 +393,11 @@ class DecodeDraft:
         n = len(tokens)
         if n != len(parents) or n > most or tokens[0] != text[-1]:
             raise ValueError(f"a draft of {n} tokens and {len(parents)} parents: as many of both, {most} at most, the first token the text's last")
-        u = None if u is None or not temperature else u[:n]
+        if not all(0 <= t < self.f.args.vocab_size for t in tokens):
+            raise ValueError(f"drafted tokens {tokens}: 0 .. {self.f.args.vocab_size - 1}")
+        if temperature and (u is None or u.dim() != 1 or u.numel() < n):
+            raise ValueError(f"temperature {temperature}: 0, or random numbers for {n} rows")
+        u = u[:n] if temperature else None
         probs = probs[0] if probs else None
         out = self._captured(tokens, parents, cache, u, temperature) if probs is None else None
         if out is None:

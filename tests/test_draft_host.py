@@ -65,7 +65,7 @@ def test_entry_points_refuse(scmx):
     def check(n=3, V=100, ld=100, u=P, t=1.0, probs=None, ldp=0, size=1 << 20, tokens=P):
         return (P, 1, ld, tokens, P, u, t, probs, ldp, n, V, P, P, P, P, size, None)
     for kw, text in ((dict(n=0), "0 rows"), (dict(n=65), "65 rows"), (dict(V=0), "0 logits"), (dict(ld=99), "99"), (dict(probs=P, ldp=99), "99"), (dict(t=-1.0), "temperature"),
-                     (dict(t=float("nan")), "temperature"), (dict(t=float("inf")), "temperature"), (dict(t=1e-42), "temperature"), (dict(u=None), "random"),
+                     (dict(t=float("nan")), "temperature"), (dict(t=float("inf")), "temperature"), (dict(t=1e-42), "temperature"), (dict(t=4e-39), "temperature"), (dict(u=None), "random"),
                      (dict(size=8), "scratch"), (dict(tokens=None), "null")):
         _refused(scmx, "scmx_verify", check(**kw), text)
 
@@ -96,3 +96,25 @@ def test_caches_of_models(scmx):
     with pytest.raises(ValueError):
         HM.make_prompt_cache(hybrid, 8, dtype=torch.int8)
     assert len(HM.make_prompt_cache(hybrid, 8, dtype=torch.float32)) == 1
+
+
+def test_drafts_are_checked(scmx):
+    """What a proposal or the random numbers may get wrong is refused on the host, before anything is launched."""
+    import importlib
+    from types import SimpleNamespace as N
+    DD = importlib.import_module(scmx.__name__ + ".decode").DecodeDraft
+    d, cache = DD.__new__(DD), [N(offset=4, capacity=8)]
+    d.f = N(args=N(vocab_size=16))
+    chain = lambda n: list(range(-1, n - 1))                # noqa: E731
+    for tokens, parents in (([3, 16], [-1, 0]), ([3, -1], [-1, 0]), ([4, 1], [-1, 0]), ([3, 1], [-1]), ([3], [-1, 0]), ([3, 1], [-1, 1]), ([3] * 5, chain(5)), ([], [])):
+        d.propose = lambda text, most: (tokens, parents)
+        with pytest.raises(ValueError):
+            d.step([1, 3], cache)
+    with pytest.raises(ValueError):
+        d.step([1, 17], cache)                              # the text's last token itself
+    d.propose = lambda text, most: ([3, 2, 1], chain(3))
+    for u in (None, torch.zeros(2), torch.zeros(1), torch.zeros(3, 1)):
+        with pytest.raises(ValueError, match="temperature"):
+            d.step([1, 3], cache, 0.5, u)
+    with pytest.raises(AssertionError):
+        d.step([1, 3], [N(offset=8, capacity=8)])

@@ -6,7 +6,7 @@ A cache is an object with k and v [hk, capacity, d] and `offset`, the positions 
 float32 scales ks and vs [hk, capacity].  Nothing here advances `offset`.
 
 A call of few rows is shorter on the device than on the host: checks ask each tensor as little as they can."""
-import ctypes
+from array import array
 
 import torch
 
@@ -119,7 +119,8 @@ def kv_keep(caches, rows, pos=None, pos_dev=None):
             layers += (k.data_ptr(), v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr())
         else:
             layers += (k.data_ptr(), v.data_ptr(), 0, 0)
-    _lib.call("scmx_kv_keep", (ctypes.c_size_t * len(layers))(*layers), len(caches), rows.data_ptr(), n, pos, dev, hk, d, cap, int8, _lib.stream())
+    table = array("Q", layers)
+    _lib.call("scmx_kv_keep", table.buffer_info()[0], len(caches), rows.data_ptr(), n, pos, dev, hk, d, cap, int8, _lib.stream())
 
 
 def attention_supported(hq, hk, d):

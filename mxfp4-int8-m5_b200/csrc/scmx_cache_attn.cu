@@ -56,6 +56,10 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // Byte offset of 16-byte piece c of vector r in a block: pieces are permuted within groups of eight so that the eight vectors of a matrix
 // load, and the vectors of one INT8 value load, lie in different banks.
 template <int ROW>
@@ -162,8 +166,10 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
     }
 
     const I8Pairs i8;
+    const I8Halves i8h;
     const int lr = lane & 7, lm = lane >> 3;            // row of a matrix load, and which of its four matrices
     int stage = 0;
+    float ref = 0.0f;                                   // INT8: log2 of the scale that the warp's values are relative to
     for (int b = warp; b < nblocks; b += WARPS) {
         cp_wait<L::STAGES - 2>();
         __syncwarp();
@@ -199,19 +205,20 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
                 scores(c, w);
             }
         }
-        float kf[2] = {a.scale, a.scale}, vf[2] = {1.0f, 1.0f};
+        float kf[2] = {a.scale, a.scale}, lg[2] = {0.0f, 0.0f}, inv[2] = {1.0f, 1.0f};
         if constexpr (I8) {
             const float* scales = reinterpret_cast<const float*>(blk + 2 * L::BLOCK);
+            if (b == warp) ref = ca_reference(scales[16 + (lane & 15)]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 kf[h] *= scales[g + 8 * h];
-                vf[h] = scales[16 + g + 8 * h];
+                ca_scale(scales[16 + g + 8 * h], ref, lg[h], inv[h]);
             }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[nt][j] *= kf[j >> 1];
+            for (int j = 0; j < 4; ++j) s[nt][j] = I8 ? fmaf(s[nt][j], kf[j >> 1], lg[j >> 1]) : s[nt][j] * kf[j >> 1];
         const int d0 = b * CA_KEYS - ntail;             // the block's first key, counted from the first new row
         const bool tail = d0 + CA_KEYS > 0;             // some keys are new rows, or past the end
         uint32_t seen = 0xFFFFFFFFu;                    // bit 4 nt + j
@@ -261,25 +268,33 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
                     }
                 }
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], pl[NT][2];                 // weights as an operand; bfloat16: and what its rounding left of them
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float base = mx[nt][e] == -INFINITY ? 0.0f : mx[nt][e];
+                const float base = mx[nt][e] == -INFINITY ? 0.0f : I8 ? mx[nt][e] - CA_SHIFT : mx[nt][e];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float& x = s[nt][2 * h + e];
                     x = ca_ex2(x - base);
-                    sum[nt][e] += x;
                     if constexpr (I8) {
-                        x *= vf[h];
-                        if (tail && !(seen >> (4 * nt + 2 * h + e) & 1)) x = 0.0f;      // its scale may be anything
+                        if (!tail || (seen >> (4 * nt + 2 * h + e) & 1)) sum[nt][e] = fmaf(x, inv[h], sum[nt][e]);      // an unseen one's scale may be anything
+                    } else {
+                        sum[nt][e] += x;
                     }
                 }
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) pb[nt][h] = transpose8(pack_bf16x2(s[nt][2 * h], s[nt][2 * h + 1]));
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (I8) {
+                    pb[nt][h] = transpose8(pack_f16x2(s[nt][2 * h], s[nt][2 * h + 1]));
+                } else {
+                    const uint32_t p = pack_bf16x2(s[nt][2 * h], s[nt][2 * h + 1]);
+                    pb[nt][h] = transpose8(p);
+                    pl[nt][h] = transpose8(pack_bf16x2(s[nt][2 * h] - bf16_lo(p), s[nt][2 * h + 1] - bf16_hi(p)));
+                }
+            }
         }
         // a value that is not finite must not reach rows that do not see it: such blocks, which only new rows can make, go key by key
         bool odd = false;
@@ -324,9 +339,9 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
                 ldsm4_t(vst + ca_at<ROW>(lr + 8 * (lm & 1), i + (lm >> 1)), w);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {           // operand rows g and g + 8: values 2 g and 2 g + 1 of the piece
-                    const uint32_t f[4] = {i8.even(w[2 * e]), i8.odd(w[2 * e]), i8.even(w[2 * e + 1]), i8.odd(w[2 * e + 1])};
+                    const uint32_t f[4] = {i8h.even(w[2 * e]), i8h.odd(w[2 * e]), i8h.even(w[2 * e + 1]), i8h.odd(w[2 * e + 1])};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[i + e][nt], f, pb[nt][0], pb[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[i + e][nt], f, pb[nt][0], pb[nt][1]);
                 }
             }
         } else {
@@ -335,7 +350,10 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
                 uint32_t w[4];                          // values 0-7, 8-15 of keys 0-7, the same of keys 8-15
                 ldsm4_t(vst + ca_at<ROW>(lr + 8 * (lm >> 1), 2 * i + (lm & 1)), w);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_bf16(o[i][nt], w, pb[nt][0], pb[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_bf16(o[i][nt], w, pb[nt][0], pb[nt][1]);
+                    mma_bf16(o[i][nt], w, pl[nt][0], pl[nt][1]);
+                }
             }
         }
         stage = stage + 1 == L::STAGES ? 0 : stage + 1;
@@ -345,18 +363,19 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
 
     // the warps' states, joined: a warp to a row
     float* st = reinterpret_cast<float*>(ring);
+    const float by = I8 ? ca_ex2(ref) : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float l = sum[nt][e];
+            float l = I8 ? sum[nt][e] * CA_DOWN : sum[nt][e];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
             const int r = 8 * nt + 2 * t4 + e;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) st[r * L::PITCH + (I8 ? 16 * i + 2 * g + h : 16 * i + 8 * h + g)] = o[i][nt][2 * h + e];
+                for (int h = 0; h < 2; ++h) st[r * L::PITCH + (I8 ? 16 * i + 2 * g + h : 16 * i + 8 * h + g)] = I8 ? o[i][nt][2 * h + e] * CA_DOWN * by : o[i][nt][2 * h + e];
             if (g == 0) reinterpret_cast<float2*>(st + L::ROWS * L::PITCH)[r] = make_float2(mx[nt][e], l);
         }
     __syncthreads();

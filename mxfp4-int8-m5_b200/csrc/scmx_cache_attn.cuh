@@ -10,6 +10,11 @@ constexpr int CA_KEYS = 16;             // positions of a block
 constexpr int CA_MAX_ROWS = 64;
 constexpr float CA_LOG2E = 1.4426950408889634f;
 constexpr float CA_GROWTH = 8.0f;      // log2 of how far a weight may exceed one before the maximum is raised
+// INT8: a weight and its value's scale s are one power of 2, w = 2^(score + log2(s / r) - max), whose maximum the rows keep, r the largest scale of the first
+// positions; what is summed is w / (s / r), and outputs are multiplied by r at the end.  So w never exceeds 2^8 whatever the scales, and it goes to
+// the product as float16 (the codes are exact in it), 2^6 larger: from 2^14 down to 2^-24, 2^-12 of a weight off where bfloat16 is 2^-8.  Sums and outputs leave
+// 2^20 smaller, so that large values times r stay finite.
+constexpr float CA_SHIFT = 6.0f, CA_LEAST = -90.0f, CA_DOWN = 9.5367431640625e-07f;
 
 struct CaArgs {
     const uint16_t* q;               // bf16, heads q_hs and rows q_rs elements apart
@@ -48,7 +53,24 @@ __device__ __forceinline__ float ca_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
+// log2 r of the largest of a warp's scales.
+__device__ __forceinline__ float ca_reference(float s) {
+    const float r = warp_max(s != s ? 0.0f : s);
+    float lg;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(r));
+    return r > 0.0f && r < INFINITY ? lg : 0.0f;
+}
+// log2(s / r) and r / s of a value's scale, 2^-20 off at most.  A vector of zeros has scale 0, and any other will do; below 2^-90 r the sums' range ends.
+__device__ __forceinline__ void ca_scale(float s, float ref, float& lg, float& inv) {
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s));
+    lg = s == 0.0f ? 0.0f : s != s ? s : fmaxf(lg - ref, CA_LEAST);
+    inv = ca_ex2(-lg);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
 // E = D / 32 consecutive values of a row to a lane.
 template <int E> struct CaVec;
 template <> struct CaVec<2> { typedef float2 type; };

@@ -3,12 +3,12 @@
 //
 // Two streams share the tensor core: while it works for one, the other's softmax runs.  With one query tile of 128 rows the streams take the
 // key tiles (128 positions) in turn and are joined at the end; with two, each stream has a query tile of its own.  A `unit` is a stream's work
-// on one key tile: S = Q K^T (128 x 128, float32 in tensor memory), softmax, O += P V with P (bfloat16) read from tensor memory, where it
-// overwrites S.
+// on one key tile: S = Q K^T (128 x 128, float32 in tensor memory), softmax, O += P V with P (bfloat16; float16 over INT8) read from tensor memory, where
+// it overwrites S.
 //   warps 0-7     two softmax warpgroups, one per stream, a thread per lane of tensor memory.  The maximum is raised when it has grown by
 //                 more than 2^8
-//   warps 8-15    (INT8) codes of a tile from memory to bfloat16 operands, exactly; a position's key scale multiplies its scores, its value scale
-//                 its weights.  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are
+//   warps 8-15    (INT8) codes of a tile from memory to operands, exactly, keys to bfloat16 and values to float16; a position's key scale multiplies
+//                 its scores, and the log2 of its value scale is added to them (CA_SHIFT).  Vectors are stored with values 1 and 2 of every four exchanged, as the conversion leaves them: queries are
 //                 laid out alike, and outputs put back.  Tiles ahead are prefetched into L2
 //   last warps    one issues all MMAs (it stays converged, one lane issues), one loads key and value tiles by TMA (bfloat16)
 // INT8: registers are shared out by role (setmaxnreg).
@@ -34,6 +34,7 @@ namespace cg = cooperative_groups;
 namespace scmx {
 
 constexpr int CT_TILE = 128 * 128;        // bytes of a [128 rows x 64 bfloat16] block
+constexpr uint32_t IDESC_BF16 = 1u << 7 | 1u << 10;      // types of A and B in an instruction descriptor: bfloat16, 0 for float16
 constexpr int CT_SCALES = 8;              // tiles whose scales are held
 constexpr int CT_AHEAD = 6;               // tiles that are prefetched into L2
 
@@ -45,8 +46,8 @@ struct CtSmem {
     static constexpr int Q_OFF = 0;
     static constexpr int K_OFF = Q_OFF + MQ * KB * CT_TILE;
     static constexpr int V_OFF = K_OFF + KS * KB * CT_TILE;
-    static constexpr int SC_OFF = V_OFF + VS * KB * CT_TILE;                  // scales: [CT_SCALES][keys, values][128] float
-    static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1024 : 0);
+    static constexpr int SC_OFF = V_OFF + VS * KB * CT_TILE;                  // [CT_SCALES][keys' scales, values' log2, values' reciprocals][128] float
+    static constexpr int BAR_OFF = SC_OFF + (I8 ? CT_SCALES * 1536 : 0);
     // kfull, kempty [KS], vfull, vempty [VS], scales [CT_SCALES], S [2], P [2][halves], O [2], queries
     static constexpr int NBAR = 2 * KS + 2 * VS + (I8 ? CT_SCALES : 0) + 9;
     // threads; INT8: registers of a thread by role, together no more than the block is launched with
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
     } else if (warp == MISC) {
         if (I8) set_regs<false, L::MISC_REGS>();
         const uint32_t on = elect_lane();
-        const uint32_t idesc_s = umma_idesc_bf16(128, 128), idesc_o = umma_idesc_bf16(128, D) | IDESC_B_MN;
+        const uint32_t idesc_s = umma_idesc_bf16(128, 128), idesc_o = (umma_idesc_bf16(128, D) | IDESC_B_MN) & ~(I8 ? IDESC_BF16 : 0u);      // (INT8: float16)
         int kt = -1, vt = -1;            // last tiles that were waited for
         auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
             if (!wait_warp(bar, parity, abort_flag, wait_ns, code, fail)) return false;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         for (int u = m; u < units; u += 2) {
             const int j = MQ == 2 ? u >> 1 : u, d0 = dnew + 128 * j;
             const bool tail = d0 + 128 > 0;                     // some keys are new rows, or past the end
-            const float* scales = reinterpret_cast<const float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 256 + c0;
+            const float* scales = reinterpret_cast<const float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 384 + c0;
             int w = mbar_wait(b_s + 8 * m, (u >> 1) & 1, abort_flag, wait_ns);
             if (I8 && !w) w = mbar_wait(b_sc + 8 * (j & (CT_SCALES - 1)), (j / CT_SCALES) & 1, abort_flag, wait_ns);
             if (__any_sync(0xffffffffu, w)) { fail = w == 1 ? 74 : -1; break; }
@@ -270,9 +271,9 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 if constexpr (I8) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(scales + 32 * c + i);
-                        const float2 x = unpack2(mul2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), pack2(f.x, f.y)));
-                        const float2 y = unpack2(mul2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), pack2(f.z, f.w)));
+                        const float4 f = *reinterpret_cast<const float4*>(scales + 32 * c + i), g = *reinterpret_cast<const float4*>(scales + 128 + 32 * c + i);
+                        const float2 x = unpack2(fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), pack2(f.x, f.y), pack2(g.x, g.y)));
+                        const float2 y = unpack2(fma2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), pack2(f.z, f.w), pack2(g.z, g.w)));
                         v[i] = __float_as_uint(x.x);
                         v[i + 1] = __float_as_uint(x.y);
                         v[i + 2] = __float_as_uint(y.x);
@@ -286,31 +287,29 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                         if (!(seen >> i & 1)) v[i] = 0xFF800000u;
                 }
             };
-            constexpr bool HOLD = !I8 || NCH <= 2;      // the scores stay in registers between the two passes; otherwise they are loaded twice
-            uint32_t r[HOLD ? NCH : 2][32];
+            // the scores stay in registers between the two passes; where those are too few, only the first half does, and the second waits as exponents in its place
+            constexpr int HELD = I8 && NCH > 2 ? 2 : NCH;
+            uint32_t r[HELD][32];
             float tm = -INFINITY;
-            if (HOLD) {
 #pragma unroll
-                for (int c = 0; c < NCH; ++c) tmem_ld32(ts + c0 + 32 * c, r[c]);
+            for (int half = NCH / HELD - 1; half >= 0; --half) {
 #pragma unroll
-                for (int c = 0; c < NCH; ++c) tmem_ld_fence(r[c]);
-            } else {
-                tmem_ld32(ts + c0, r[0]);
-                tmem_ld_fence(r[0]);
-            }
+                for (int e = 0; e < HELD; ++e) tmem_ld32(ts + c0 + 32 * (HELD * half + e), r[e]);
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                uint32_t(&v)[32] = r[HOLD ? c : c & 1];
-                if (!HOLD && c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
-                finish(v, c);
-                float m0 = -INFINITY, m1 = -INFINITY;
+                for (int e = 0; e < HELD; ++e) tmem_ld_fence(r[e]);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    m0 = fmaxf(m0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
-                    m1 = fmaxf(m1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
+                for (int e = 0; e < HELD; ++e) {
+                    uint32_t(&v)[32] = r[e];
+                    finish(v, HELD * half + e);
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        m0 = fmaxf(m0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+                        m1 = fmaxf(m1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
+                    }
+                    tm = fmaxf(tm, fmaxf(m0, m1));
+                    if (half > 0) tmem_st32(ts + c0 + 32 * (HELD * half + e), v);
                 }
-                tm = fmaxf(tm, fmaxf(m0, m1));
-                if (!HOLD && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
             }
             const bool first = u == m, grow = first || (tm - mx) * sl > CA_GROWTH;
             if (__any_sync(0xffffffffu, grow)) {
@@ -335,19 +334,15 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b_p + 16 * m + 8 * h);
             };
-            const float off = -mx * sl;
+            const float off = I8 ? CA_SHIFT - mx : -mx * sl;
             const uint64_t sl2 = pack2(sl, sl), off2 = pack2(off, off);
             uint64_t s2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-            if (!HOLD) {
-                tmem_ld32(ts + c0, r[0]);
-                tmem_ld_fence(r[0]);
-            }
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                uint32_t(&v)[32] = r[HOLD ? c : c & 1];
-                if (!HOLD) {
-                    if (c + 1 < NCH) tmem_ld32(ts + c0 + 32 * (c + 1), r[(c + 1) & 1]);
-                    finish(v, c);
+                uint32_t(&v)[32] = r[c % HELD];
+                if (c > 0 && c % HELD == 0) {
+#pragma unroll
+                    for (int e = 0; e < HELD; ++e) tmem_ld_fence(r[e]);
                 }
                 const uint32_t seen = tail ? ct_seen(bits, d0 + c0 + 32 * c) : 0xFFFFFFFFu;
                 uint32_t pk[16];
@@ -360,21 +355,26 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                         const float2 y = unpack2(I8 ? add2(z, off2) : fma2(z, sl2, off2));
                         x[e] = ex2_approx(y.x);
                         x[e + 1] = ex2_approx(y.y);
-                        s2[e / 2] = add2(s2[e / 2], pack2(x[e], x[e + 1]));
+                        if (!I8) s2[e / 2] = add2(s2[e / 2], pack2(x[e], x[e + 1]));
                     }
                     if constexpr (I8) {
-                        const float4 f = *reinterpret_cast<const float4*>(scales + 128 + 32 * c + i);
-                        const float2 y = unpack2(mul2(pack2(x[0], x[1]), pack2(f.x, f.y))), w = unpack2(mul2(pack2(x[2], x[3]), pack2(f.z, f.w)));
-                        x[0] = y.x; x[1] = y.y; x[2] = w.x; x[3] = w.y;
-                        if (tail)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (!(seen >> (i + e) & 1)) x[e] = 0.0f;      // its scale may be anything
+                        float4 f = *reinterpret_cast<const float4*>(scales + 256 + 32 * c + i);
+                        if (tail) {                                           // an unseen position's scale may be anything
+                            if (!(seen >> i & 1)) f.x = 0.0f;
+                            if (!(seen >> i & 2)) f.y = 0.0f;
+                            if (!(seen >> i & 4)) f.z = 0.0f;
+                            if (!(seen >> i & 8)) f.w = 0.0f;
+                        }
+                        s2[0] = fma2(pack2(x[0], x[1]), pack2(f.x, f.y), s2[0]);
+                        s2[1] = fma2(pack2(x[2], x[3]), pack2(f.z, f.w), s2[1]);
                     }
-                    pk[i / 2] = pack_bf16x2(x[0], x[1]);
-                    pk[i / 2 + 1] = pack_bf16x2(x[2], x[3]);
+                    pk[i / 2] = I8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]);
+                    pk[i / 2 + 1] = I8 ? pack_f16x2(x[2], x[3]) : pack_bf16x2(x[2], x[3]);
                 }
-                if (!HOLD && c + 1 < NCH) tmem_ld_fence(r[(c + 1) & 1]);
+                if (c + HELD < NCH) {
+                    if (c == 0) tmem_st_wait();
+                    tmem_ld32(ts + c0 + 32 * (c + HELD), v);
+                }
                 tmem_st16(ts + c0 / 2 + 16 * c, pk);
                 if (HALVES == 2 && c == NCH / 2 - 1 && !clear) hand_over(0);
             }
@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         float* out = reinterpret_cast<float*>(smem + L::Q_OFF);
         float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
         const int slot = 128 * m + l;
-        ml[slot] = mine && sum != 0.0f ? make_float2(mx * sl, sum) : make_float2(-INFINITY, 0.0f);
+        ml[slot] = mine && sum != 0.0f ? make_float2(mx * sl, I8 ? sum * CA_DOWN : sum) : make_float2(-INFINITY, 0.0f);
+        const float by = I8 && mine ? ca_ex2(*reinterpret_cast<const float*>(smem + L::MISC_OFF + 16)) : 1.0f;
         for (int c = 0; c < D / 32 && mine; ++c) {
             uint32_t v[32];
             tmem_ld32(to + 32 * c, v);
@@ -441,7 +442,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             float4* p = reinterpret_cast<float4*>(out + slot * L::PITCH + 32 * c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)      // INT8: values 1 and 2 of four change places again
-                p[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + (I8 ? 2 : 1)]), __uint_as_float(v[4 * i + (I8 ? 1 : 2)]), __uint_as_float(v[4 * i + 3]));
+                p[i] = I8 ? make_float4(__uint_as_float(v[4 * i]) * CA_DOWN * by, __uint_as_float(v[4 * i + 2]) * CA_DOWN * by, __uint_as_float(v[4 * i + 1]) * CA_DOWN * by, __uint_as_float(v[4 * i + 3]) * CA_DOWN * by)
+                          : make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const int rows = units == 0 ? 0 : R - row0 < ROWS ? R - row0 : ROWS;
@@ -516,6 +518,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         constexpr int CPR = D / 16, PASSES = 128 * CPR / 256;
         const int t = tid - 256, cc = t % CPR, r0 = t / CPR;
         const I8Pairs i8;
+        const I8Halves i8h;
         const int8_t *kc = static_cast<const int8_t*>(a.k) + ((int64_t)kvh * a.cap + t0) * D, *vc = static_cast<const int8_t*>(a.v) + ((int64_t)kvh * a.cap + t0) * D;
         auto load = [&](const int8_t* p, int j, uint4 (&x)[PASSES]) {
 #pragma unroll
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * D) : "memory");
             }
         };
-        auto convert = [&](uint8_t* dst, const uint4 (&x)[PASSES]) {
+        auto convert = [&](bool halves, uint8_t* dst, const uint4 (&x)[PASSES]) {
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
                 const int r = r0 + i * (256 / CPR);
@@ -539,8 +542,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
                 uint32_t o[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    o[2 * e] = i8.even(u[e]);
-                    o[2 * e + 1] = i8.odd(u[e]);
+                    o[2 * e] = halves ? i8h.even(u[e]) : i8.even(u[e]);
+                    o[2 * e + 1] = halves ? i8h.odd(u[e]) : i8.odd(u[e]);
                 }
                 uint8_t* p = dst + cc / 4 * CT_TILE + r * 128;
                 const int e = 2 * (cc & 3), swap = cc >> 2;      // the upper half's stores in the other order: all of a vector's fall on different banks
@@ -551,7 +554,19 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         };
         // a position's scales: keys' by threads 0-127, values' by the others, loaded a tile ahead
         const float* scales = (t < 128 ? a.ks : a.vs) + (int64_t)kvh * a.cap + t0 + (t & 127);
-        const float factor = t < 128 ? fabsf(a.scale) : 1.0f;
+        const float factor = fabsf(a.scale);
+        float ref = 0.0f;                         // log2 of the scale that values are relative to
+        if (t >= 128) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 32 * i + lane < nkeys ? 32 * i + lane : 0;
+                const float s = nkeys > 0 ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + r) : 0.0f;
+                top = fmaxf(top, s);
+            }
+            ref = ca_reference(top);
+            if (t == 128) *reinterpret_cast<float*>(smem + L::MISC_OFF + 16) = ref;
+        }
         auto scale = [&](int j) { return 128 * j + (t & 127) < nkeys ? __ldg(scales + 128 * j) : 0.0f; };
         uint4 xk[PASSES], xv[PASSES];
         for (int j = 1; j < CT_AHEAD; ++j) ahead(j);
@@ -571,14 +586,16 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         for (int j = 0; j < ntiles; ++j) {
             ahead(j + CT_AHEAD);
             if (!ready(b_ke, j, KS)) break;
-            convert(smem + L::K_OFF + j % KS * KB * CT_TILE, xk);
-            reinterpret_cast<float*>(smem + L::SC_OFF)[(j & (CT_SCALES - 1)) * 256 + t] = sc * factor;
+            convert(false, smem + L::K_OFF + j % KS * KB * CT_TILE, xk);
+            float* own = reinterpret_cast<float*>(smem + L::SC_OFF) + (j & (CT_SCALES - 1)) * 384 + t;
+            if (t < 128) own[0] = sc * factor;
+            else ca_scale(sc, ref, own[0], own[128]);
             if (j + 1 < ntiles) load(kc, j + 1, xk);
             sc = scale(j + 1);
             done(b_kf + 8 * (j % KS));
             if (lane == 0) mbar_arrive(b_sc + 8 * (j & (CT_SCALES - 1)));
             if (!ready(b_ve, j, VS)) break;
-            convert(smem + L::V_OFF + j % VS * KB * CT_TILE, xv);
+            convert(true, smem + L::V_OFF + j % VS * KB * CT_TILE, xv);
             if (j + 1 < ntiles) load(vc, j + 1, xv);
             done(b_vf + 8 * (j % VS));
         }

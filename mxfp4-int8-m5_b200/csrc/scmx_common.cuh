@@ -275,6 +275,22 @@ struct I8Pairs {
     __device__ __forceinline__ uint32_t odd(uint32_t w) const { return even(w >> 8); }
 };
 
+// The same as two float16: a code plus 128 is the low bits of the significand of 1024 + 128 + code, one logic operation and one subtraction for a pair.
+struct I8Halves {
+    uint32_t low, flip;
+    __device__ __forceinline__ I8Halves() {
+        asm volatile("mov.b32 %0, 0x00FF00FF;" : "=r"(low));
+        asm volatile("mov.b32 %0, 0x64806480;" : "=r"(flip));
+    }
+    __device__ __forceinline__ uint32_t even(uint32_t w) const {
+        uint32_t x, d;
+        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(x) : "r"(w), "r"(low), "r"(flip));       // (w & low) ^ flip
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(flip));
+        return d;
+    }
+    __device__ __forceinline__ uint32_t odd(uint32_t w) const { return even(w >> 8); }
+};
+
 // Eight INT8 codes (two words) -> their balanced digits to base eight, x = d0 + 8 d1 + 64 d2 with -4 <= d0, d1 <= 3 and |d2| <= 2, one word of
 // eight e2m1 codes per digit (element i in bits 4 i .. 4 i + 3): a digit d is sign << 3 | |d|, the e2m1 number d / 2.
 // With t = x + 128 the digits plus four are (t + 36) mod 8, ((t + 36) / 8) mod 8 and (t + 36) / 64 + 2, taken from t / 4 + 41 so that bytes do not overflow.

@@ -148,8 +148,8 @@ def bits_of(mask, n):
     return [(1 << i + 1) - 1 for i in range(n)] if mask is None else [b & (1 << n) - 1 for b in mask.tolist()]
 
 
-def attention_oracle(q, c, scale, mask, T=None):
-    """float64 output, and how far a kernel's may be off: weights and outputs are rounded to bfloat16 once (U each), scores are float32 sums of d
+def attention_oracle(q, c, scale, mask, T=None, weight=U):
+    """float64 output, and how far a kernel's may be off: weights and outputs are rounded to bfloat16 once (U each; weight: what a weight may be off), scores are float32 sums of d
     products (an error of (d + 8) 2^-24 sum |q k| scale changes a weight by twice that), sums of weights and outputs float32."""
     hq, n, d = q.shape
     hk, T = c.k.shape[0], c.offset if T is None else T
@@ -166,7 +166,7 @@ def attention_oracle(q, c, scale, mask, T=None):
         size = ((q[h].to(F64).abs() @ k.abs().T) * abs(scale)).masked_fill(~seen, 0.0).amax(1, keepdim=True)
         weighted = p @ torch.where(torch.isfinite(v), v, 0.0).abs()
         out[:, h] = p @ torch.where(torch.isfinite(v), v, 0.0)
-        tol[:, h] = U * (weighted + out[:, h].abs()) * (1 + U) + weighted * (2 * (d + 8) * 2.0 ** -24 * size + (T + n) ** 0.5 * 2.0 ** -22)
+        tol[:, h] = (weight * weighted + U * out[:, h].abs()) * (1 + U) + weighted * (2 * (d + 8) * 2.0 ** -24 * size + (T + n) ** 0.5 * 2.0 ** -22)
     return out.reshape(n, hq * d), tol.reshape(n, hq * d)
 
 
@@ -191,6 +191,41 @@ def test_attention_of_a_tree(scmx, int8, d, hq, hk, n, T):
     mask = scmx.sc_draft.draft_mask(random_parents(random.Random(n), n))
     check_attention(scmx.sc_cache.cache_attention(q, c, scale, mask), q, c, scale, mask)
     check_attention(scmx.sc_cache.cache_attention(q, c, scale), q, c, scale, None)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("int8,hq,hk,n,T", [(False, 8, 4, 1, 900), (False, 4, 4, 11, 10000), (False, 2, 1, 8, 40), (True, 8, 4, 1, 900), (True, 2, 2, 16, 10000), (True, 16, 2, 3, 2500),
+                                            (True, 16, 2, 7, 400), (True, 8, 2, 30, 7000), (True, 8, 1, 20, 9000), (True, 4, 1, 64, 5000)])
+def test_weights_keep_their_bits(scmx, int8, d, hq, hk, n, T):
+    """Weights over INT8 are float16 (half a step is 2^-12 of one, the maximum's exponential, the scale's log2 and reciprocal 2^-20 together), those of up to 16
+    query rows over bfloat16 two bfloat16 (2^-16): 2^-11 and 2^-15 with room for it, where one bfloat16 is 2^-8."""
+    q, c = attention_case(scmx, hq, hk, n, T, d, int8, seed=3 * n + T)
+    mask = scmx.sc_draft.draft_mask(random_parents(random.Random(n), n))
+    want, tol = attention_oracle(q, c, d ** -0.5, mask, weight=2.0 ** -11 if int8 else 2.0 ** -15)
+    off = (scmx.sc_cache.cache_attention(q, c, d ** -0.5, mask).double() - want).abs()
+    assert (off <= tol).all(), f"off by {(off / tol).max().item():.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("hq,hk,n,T", [(4, 2, 1, 700), (4, 4, 12, 9000), (8, 2, 7, 300), (4, 1, 20, 3000), (4, 1, 64, 1200)])
+def test_scales_of_all_sizes(scmx, hq, hk, n, T):
+    """Values whose scales differ by 2^60, among them zeros and the smallest and largest that kv_append writes.  A weight below 2^-14 has a float16 step of 2^-24, 2^-30 of
+    the largest weight's 2^6 at least: half of it for every position, times 127 codes and the largest p s."""
+    q, c = attention_case(scmx, hq, hk, n, T, 128, True, seed=n)
+    g = gen(9)
+    c.vs.mul_(2.0 ** torch.randint(-30, 31, c.vs.shape, generator=g, device="cuda").float())
+    gone = torch.rand(c.vs.shape, generator=g, device="cuda") < 0.05
+    c.vs[gone] = 0.0
+    c.v[gone] = 0
+    for size in (None, 2.0 ** -126, 2.0 ** 120 / 127):
+        if size is not None:
+            c.vs.copy_(torch.where(gone, 0.0, size))
+        want, tol = attention_oracle(q, c, 0.09, None, weight=2.0 ** -11)
+        if size is None:
+            tol += (T + n) * 2.0 ** -31 * 127 * c.vs.double().amax()
+        else:
+            tol += 2.0 ** -126                                        # an output below the normal numbers
+        off = (scmx.sc_cache.cache_attention(q, c, 0.09).double() - want).abs()
+        assert (off <= tol).all(), f"{size}: off by {(off / tol).max().item():.3g} of the tolerance"
 
 
 @pytest.mark.parametrize("int8", [False, True])

@@ -19,11 +19,11 @@
 // in shared memory, with the rows behind the last position, and add them at the end to the rows that see them.
 // Every mbarrier wait is bounded (status word codes 71..76).
 //
-// Measured on a B200 (8 key/value heads of 128): 60000 bfloat16 positions 45.2 us with 18 query rows (5.4 TB/s), 51.5 with 128, 68 with 256; INT8 48,
-// 61 and 101 us.  bfloat16 up to 128 rows waits for memory.  A pair of units of 256 rows takes 3400 cycles, and its bytes arrive in 2800: a stream's
+// Measured on a B200 (8 key/value heads of 128): 60000 bfloat16 positions 45.2 us with 18 query rows (5.4 TB/s), 51.5 with 128, 68 with 256; INT8 49,
+// 63 and 107 us.  bfloat16 up to 128 rows waits for memory.  A pair of units of 256 rows takes 3400 cycles, and its bytes arrive in 2800: a stream's
 // scores, softmax (2050 cycles, half of them the exponentials' rate) and product follow on one another, and two streams are what tensor memory
-// holds.  A second softmax thread per row, or a third of the exponentials from a cubic, changed less than 2 %.  INT8 adds the scales' products and the
-// conversions, which share the issue slots: 6000 cycles for a pair.  Weights in halves against whole tiles: 256 rows 72 -> 70 us, INT8 65 -> 62 us at
+// holds.  A second softmax thread per row, or a third of the exponentials from a cubic, changed less than 2 %.  INT8 adds the scales and the conversions,
+// which share the issue slots: 6000 cycles for a pair; half of its exponents wait in tensor memory (all loaded and scaled twice: 67 us, not 63).  Weights in halves against whole tiles: 256 rows 72 -> 70 us, INT8 65 -> 62 us at
 // 128 rows; for bfloat16 at 128 rows, which has its two streams on different tiles, 16.9 -> 17.6 us at 8000 positions, so there they stay whole.
 #include <cooperative_groups.h>
 #include "mixers/mix_tc.cuh"
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         const int m = warp >> 2 & 1, zero = warp >> 3, q = warp & 3, l = 32 * q + lane, copy = l / RP, row = row0 + (MQ == 2 ? 128 * m : 0) + l % RP, tok = ca_tok(a, row);
         const uint32_t lane_base = (uint32_t)(32 * q) << 16, ts = tmem + 128 * m + lane_base, to = tmem + 256 + 128 * m + lane_base;
         // The thread's first key of a tile.  `zero` keeps it from being a constant with one copy, where the compiler then orders the loads of the two
-        // streams worse (60000 positions, 256 rows, bfloat16 70.3 us and not 68.2, INT8 109 and not 101)
+        // streams worse (60000 positions, 256 rows, bfloat16 70.3 us and not 68.2; INT8 125 and not 114 when scores were scaled twice)
         const int c0 = copy * (128 / COPIES) + zero * 64;
         uint64_t bits = 0;
         if (row < R) {

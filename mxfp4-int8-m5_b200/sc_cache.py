@@ -3,7 +3,7 @@ several new rows to a bfloat16 or INT8 cache, and the move of accepted rows.  CU
 current stream; there is no CPU path.
 
 A cache is an object with k and v [hk, capacity, d] and `offset`, the positions that it holds: bfloat16 (host_model.KVCache), or int8 with
-float32 scales ks and vs [hk, capacity].  Nothing here advances `offset`.
+float32 scales ks and vs [hk, capacity], not negative.  Nothing here advances `offset`.
 
 A call of few rows is shorter on the device than on the host: checks ask each tensor as little as they can."""
 from array import array

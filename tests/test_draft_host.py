@@ -118,3 +118,16 @@ def test_drafts_are_checked(scmx):
             d.step([1, 3], cache, 0.5, u)
     with pytest.raises(AssertionError):
         d.step([1, 3], [N(offset=8, capacity=8)])
+
+
+def test_entry_points_run_as_a_script():
+    """Everything that build() and smoke() call is defined above the lines that run them when the file is the program."""
+    import ast
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "__graft_entry__.py")
+    body = ast.parse(open(path).read()).body
+    guard = next(i for i, node in enumerate(body) if isinstance(node, ast.If) and "__main__" in ast.unparse(node.test))
+    defined = {node.name for node in body[:guard] if isinstance(node, ast.FunctionDef)}
+    later = {node.name for node in body[guard:] if isinstance(node, ast.FunctionDef)}
+    called = {node.func.id for f in body for node in ast.walk(f) if isinstance(node, ast.Call) and isinstance(node.func, ast.Name)}
+    assert {"build", "smoke"} <= defined and not called & later

@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
             bits = a.mask ? (uint64_t)a.mask[tok] : (2ull << tok) - 1ull;
             if (a.n < 64) bits &= (1ull << a.n) - 1ull;
         }
-        const float sl = I8 ? 1.0f : fabsf(a.scale);            // scores times this are exponents of 2 (INT8: the key scales have it)
+        // scores times this are exponents of 2 (INT8: the key scales have it).  Not zero, which would make hidden scores, -inf, NaN
+        const float sl = I8 ? 1.0f : fmaxf(fabsf(a.scale), 1.17549435e-38f);
         float mx = -1e30f, sum = 0.0f;
         for (int u = m; u < units; u += 2) {
             const int j = MQ == 2 ? u >> 1 : u, d0 = dnew + 128 * j;

@@ -229,6 +229,18 @@ def test_scales_of_all_sizes(scmx, hq, hk, n, T):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hq,hk,n,T", [(4, 2, 3, 40), (8, 2, 7, 300), (8, 2, 30, 129), (8, 1, 20, 1000), (8, 2, 40, 2500), (4, 4, 64, 0)])
+def test_scales_of_zero_and_below(scmx, int8, hq, hk, n, T):
+    """A scale of 0 is the mean of what a row sees, also where tiles hide positions; the smallest positive one is next to it; a negative one turns the order round."""
+    q, c = attention_case(scmx, hq, hk, n, T, 128, int8, seed=n)
+    mask = scmx.sc_draft.draft_mask(random_parents(random.Random(n), n))
+    nothing = mask & ~(1 << torch.arange(n, device="cuda"))                # the first row of an empty cache sees nothing
+    for scale in (0.0, -0.0, 1e-45, 1e-38, -1e-20, -0.1):
+        for m in (None, mask, nothing):
+            check_attention(scmx.sc_cache.cache_attention(q, c, scale, m), q, c, scale, m)
+
+
+@pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hq,hk,n,T", [(8, 8, 4, 0), (8, 2, 40, 0), (4, 1, 64, 0), (4, 1, 3, 200), (8, 2, 64, 1)])
 def test_rows_that_see_nothing(scmx, int8, hq, hk, n, T):
     q, c = attention_case(scmx, hq, hk, n, T, 128, int8)

@@ -60,10 +60,11 @@ __device__ __forceinline__ float ca_reference(float s) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(r));
     return r > 0.0f && r < INFINITY ? lg : 0.0f;
 }
-// log2(s / r) and r / s of a value's scale, 2^-20 off at most.  A vector of zeros has scale 0, and any other will do; below 2^-90 r the sums' range ends.
+// log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends.  A vector of zeros has scale 0: any other is right for it, and the least
+// keeps its weight out of the maximum (with r, a score 28 powers of two above all others left these so few bits that the output was half wrong).
 __device__ __forceinline__ void ca_scale(float s, float ref, float& lg, float& inv) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s));
-    lg = s == 0.0f ? 0.0f : s != s ? s : fmaxf(lg - ref, CA_LEAST);
+    lg = s != s ? s : fmaxf(lg - ref, CA_LEAST);      // (log2 of 0 is -inf)
     inv = ca_ex2(-lg);
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {

@@ -240,6 +240,24 @@ def test_scales_of_zero_and_below(scmx, int8, hq, hk, n, T):
             check_attention(scmx.sc_cache.cache_attention(q, c, scale, m), q, c, scale, m)
 
 
+@pytest.mark.parametrize("hq,hk,n,T,at", [(2, 2, 1, 2000, 1000), (2, 2, 1, 2000, 0), (4, 2, 6, 9000, 5000), (8, 2, 20, 2000, 1500), (8, 1, 40, 3000, 2)])
+def test_values_of_zeros_with_the_largest_score(scmx, hq, hk, n, T, at):
+    """A vector of zeros that takes nearly all of a row's weight leaves the others their bits: the output, small as it is, keeps its relative error (a float16 weight's half
+    step 2^-12, the maximum's exponential, log2 and reciprocal: 2^-11 of the weighted magnitudes)."""
+    g = gen(n)
+    q, c = attention_case(scmx, hq, hk, n, T, 128, True, seed=n)
+    along = torch.nn.functional.normalize(torch.randn((hk, 1, 128), generator=g, device="cuda"), dim=-1)
+    k, v = (torch.randn((hk, c.k.shape[1], 128), generator=g, device="cuda") for _ in range(2))
+    k = 0.1 * (k - (k * along).sum(-1, keepdim=True) * along)            # no other key points there
+    for powers in (0, 16, 20, 24, 28, 32, 50, 80):
+        k[:, at], v[:, at] = along[:, 0] * powers * math.log(2), 0.0
+        (c.k, c.ks), (c.v, c.vs) = quantized(k.to(BF)), quantized(v.to(BF))
+        q = (along.repeat_interleave(hq // hk, 0) * 10 + 0.3 * torch.randn((hq, n, 128), generator=g, device="cuda")).to(BF)
+        want, tol = attention_oracle(q, c, 0.1, None, weight=2.0 ** -11)
+        off = (scmx.sc_cache.cache_attention(q, c, 0.1).double() - want).abs()
+        assert (off <= tol).all(), f"{powers}: off by {(off / tol).max().item():.3g} of the tolerance"
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hq,hk,n,T", [(8, 8, 4, 0), (8, 2, 40, 0), (4, 1, 64, 0), (4, 1, 3, 200), (8, 2, 64, 1)])
 def test_rows_that_see_nothing(scmx, int8, hq, hk, n, T):

@@ -487,7 +487,7 @@ int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stri
  * -1; count int32 [1].  Tokens outside 0 .. V - 1 are rejected; without probabilities (all logits -inf, NaN) *token = 0.
  * n <= 64; scratch: scmx_verify_scratch bytes, 16-byte aligned, used by this call alone. */
 int64_t scmx_verify_scratch(int n, int64_t V);
-int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, float temperature,
+int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, double temperature,
                 const float* probs, int64_t ldp, int n, int64_t V, int32_t* rows, int32_t* count, int64_t* token, void* scratch, int64_t scratch_bytes,
                 void* stream);
 

@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libscmx.so")
 MIXERS_PATH = os.path.join(_HERE, "libscmx_mixers.so")
 
-c_i64, c_int, c_float, c_vp = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
+c_i64, c_int, c_float, c_double, c_vp = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
 
 
 class ScmxFormat(ctypes.Structure):
@@ -125,7 +125,7 @@ SIGNATURES = {
     "scmx_cache_attn": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_float, c_vp, c_vp, c_i64,
                         c_vp, c_vp],
     "scmx_verify_scratch": [c_int, c_i64],
-    "scmx_verify": [c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_float, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
+    "scmx_verify": [c_vp, c_int, c_i64, c_vp, c_vp, c_vp, c_double, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp],
     "scmx_gemv_pro": [c_vp, c_int, c_vp, c_float, c_vp, c_vp, c_vp, c_i64, c_i64, _FMT_P, c_int, c_vp, c_vp, c_int, c_int, c_int,
                       c_vp, c_int, c_vp],
     "scmx_gemv_multi_plan": [c_vp, c_int, _FMT_P],

@@ -592,15 +592,15 @@ extern "C" int64_t scmx_verify_scratch(int n, int64_t V) {
     return (int64_t)n * ((V + VF_SLICE - 1) / VF_SLICE) * (int64_t)sizeof(VfPart);
 }
 
-extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, float temperature,
+extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int64_t* tokens, const int32_t* parents, const float* u, double temperature,
                            const float* probs, int64_t ldp, int n, int64_t V, int32_t* rows, int32_t* count, int64_t* token, void* scratch, int64_t scratch_bytes,
                            void* stream) {
     SCMX_REQUIRE(n >= 1 && n <= VF_ROWS, SCMX_ELIMIT, "verify: %d rows (1 .. %d)", n, VF_ROWS);
     SCMX_REQUIRE(V >= 1 && V < (1ll << 30) && ld >= V && (probs == nullptr || ldp >= V), SCMX_EINVAL, "verify: %lld logits, rows %lld and %lld apart", (long long)V,
                  (long long)ld, (long long)ldp);
     SCMX_REQUIRE(logits && tokens && parents && rows && count && token, SCMX_EINVAL, "verify: null buffer");
-    const bool greedy = temperature == 0.0f;
-    SCMX_REQUIRE(greedy || (temperature > 0.0f && temperature <= 3.0e38f && 1.45f / temperature <= 3.0e38f), SCMX_EINVAL, "verify: temperature %g", (double)temperature);
+    const bool greedy = temperature == 0.0;
+    SCMX_REQUIRE(greedy || (temperature > 0.0 && temperature <= 3.0e38 && 1.45 / temperature <= 3.0e38), SCMX_EINVAL, "verify: temperature %g", temperature);
     SCMX_REQUIRE(greedy || u != nullptr, SCMX_EINVAL, "verify: sampling needs random numbers");
     SCMX_REQUIRE(((uintptr_t)logits & (is_f32 ? 3 : 1)) == 0 && ((uintptr_t)probs & 3) == 0, SCMX_EINVAL, "verify: unaligned buffer");
     const int64_t need = scmx_verify_scratch(n, V);
@@ -609,7 +609,7 @@ extern "C" int scmx_verify(const void* logits, int is_f32, int64_t ld, const int
     VfArgs a;
     a.logits = logits; a.probs = greedy ? nullptr : probs; a.tokens = tokens; a.parents = parents; a.u = u; a.part = static_cast<VfPart*>(scratch);
     a.rows = rows; a.count = count; a.token = token; a.ld = ld; a.ldp = ldp; a.n = n; a.V = (int)V; a.slices = (int)((V + VF_SLICE - 1) / VF_SLICE);
-    a.c = greedy ? 1.0f : (float)(1.4426950408889634 / (double)temperature);
-    a.cd = greedy ? 1.0 : 1.0 / (double)temperature;
+    a.c = greedy ? 1.0f : (float)(1.4426950408889634 / temperature);
+    a.cd = greedy ? 1.0 : 1.0 / temperature;      // (a float32 temperature is 2^-25 off: one of 300 draws from 150000 logits would be another token)
     return is_f32 ? launch_verify<float>(a, greedy, (cudaStream_t)stream) : launch_verify<uint16_t>(a, greedy, (cudaStream_t)stream);
 }

@@ -474,6 +474,28 @@ def test_verify_of_a_large_vocabulary(scmx):
         assert check_verify(scmx, logits, tokens, parents, u, 1.0, q) and check_verify(scmx, logits.float(), tokens, parents, u, 0.8, None)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("temp", [0.6, 0.7, 1.3])
+def test_verified_token_at_the_edges_of_its_interval(scmx, temp, dtype):
+    """Random numbers within 2e-8 of an edge of the cumulative probabilities, and 1e-10 at least (what float64 sums of so many weights may be off): temperatures that
+    are no float32 numbers are taken as they are."""
+    V, g = 151936, gen(5)
+    logits = (torch.randn((1, V), generator=g, device="cuda") * 2 + 9 * (torch.rand((1, V), generator=g, device="cuda") < 8 / V)).to(dtype)
+    cdf = torch.cumsum(torch.softmax(logits[0].double() / temp, -1), 0)
+    cdf /= cdf[-1].clone()
+    u = cdf.float()
+    near = (u.double() - cdf).abs()
+    for draft in (None, torch.zeros((1, V), device="cuda")):
+        some = ((near > 1e-10) & (near < 2e-8)).nonzero()[:, 0]
+        some = some[:: max(1, len(some) // 60)].tolist()
+        assert len(some) >= 50
+        for i in some:
+            want = int(torch.searchsorted(cdf, u[i:i + 1].double(), right=True))
+            t = float((cdf[want] - u[i].double()).abs()), float((cdf[want - 1] - u[i].double()).abs()) if want else 1.0
+            if min(t) > 1e-10:
+                assert verify(scmx, logits, [0], [-1], u[i:i + 1].clone(), temp, draft) == ([0], want)
+
+
 def test_verify_reads_strided_rows(scmx):
     logits, tokens, parents, u, q = verify_case(6, 1003, 4, 2, F32, True)
     want = verify(scmx, logits, tokens, parents, u, 1.0, q)

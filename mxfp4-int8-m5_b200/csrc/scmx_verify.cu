@@ -467,11 +467,12 @@ __global__ void __launch_bounds__(VW_THREADS) verify_walk_kernel(const __grid_co
         }
         before += t;
     }
+    if (!(now > 0.0 && now < INFINITY)) owner = -1;      // a NaN or +inf among the logits: every share may be a number but the one that has it
     if (rank == 0 && warp == 1) {
         for (int i = lane; i < a.n; i += 32) a.rows[i] = i < count ? path[i] : -1;
         if (lane == 0) {
             *a.count = count;
-            if (owner < 0) *a.token = 0;       // no probabilities: all logits -inf, or not numbers
+            if (owner < 0) *a.token = 0;       // no probabilities
         }
     }
     if (rank == owner) {

@@ -71,7 +71,8 @@ def verify_draft(logits, tokens, parents, u=None, temperature=1.0, probs=None):
     p <- max(p - q, 0) / Z.  q: probs[node] (float32 [n, V]; the children were drawn from it independently), or, without probs, 1
     at the child's token and 0 elsewhere.  At the path's end the token is the first whose cumulative p exceeds u[0].  u float32 [n], uniform in [0, 1).
     So the accepted tokens and the last one are distributed as if the target had chosen each of them.
-    temperature 0: greedy (the lowest index of equal logits), u and probs are not read."""
+    temperature 0: greedy (the lowest index of equal logits, a NaN the largest), u and probs are not read.  By temperature a row with a NaN or +inf, or nothing but -inf, has
+    no probabilities: its children are rejected, and the token after it is 0."""
     logits = _rows(logits, "logits", _LOGITS)
     n, V = logits.shape
     if not 1 <= n <= MAX_ROWS:

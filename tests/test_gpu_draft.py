@@ -542,6 +542,24 @@ def test_verify_corner_cases(scmx):
     assert verify(scmx, logits, [0, 5, 6, 7], parents, u * 0, 1.0, q) == ([0], 25)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [50304, 262145])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_logit_that_is_no_number(scmx, value, V, dtype):
+    """One NaN or +inf in a long row leaves it no probabilities, wherever it is: children are rejected, the token is 0; other rows are as ever."""
+    logits = torch.randn((3, V), generator=gen(1), device="cuda").to(dtype)
+    u = torch.tensor([0.7, 0.0, 0.0], device="cuda")
+    for draft in (None, torch.full((3, V), 1 / V, device="cuda")):
+        ok = verify(scmx, logits, [0, 5, 9], [-1, 0, 1], u, 1.0, draft)
+        assert ok[0] == [0, 1, 2] and ok[1] > 0
+        for at in (0, 7000, V // 2, V - 1):
+            for row in range(3):
+                bad = logits.clone()
+                bad[row, at] = value
+                rows, token = verify(scmx, bad, [0, 5, 9], [-1, 0, 1], u, 1.0, draft)
+                assert rows == list(range(row + 1)) and token == 0
+
+
 @pytest.mark.parametrize("draft", [False, True])
 def test_verified_tokens_follow_the_target(scmx, draft):
     """The first token after the root has the target's distribution, accepted or not: 4000 trials, chi-square with 7 degrees of freedom below 35 (p = 1e-5)."""

@@ -43,7 +43,7 @@ def _strides(x, unit):
     if L == 1:
         rs = 0
     if cs != 1 or hs % unit or rs % unit or x.data_ptr() % (2 * unit):
-        return x.contiguous(), L * d, d
+        return x.clone(memory_format=torch.contiguous_format), L * d, d      # (contiguous() keeps a view that starts off a boundary as it is)
     return x, hs, rs
 
 

@@ -331,6 +331,29 @@ def test_queries_of_any_strides(scmx):
         assert torch.equal(scmx.sc_cache.cache_attention(x, c, 0.2), want)
 
 
+@pytest.mark.parametrize("hk,L", [(1, 1), (1, 5), (2, 1), (2, 5)])
+@pytest.mark.parametrize("first", [1, 2, 4])
+def test_views_that_start_off_a_boundary(scmx, hk, L, first):
+    """Contiguous views whose first element is not on a 16-byte boundary, and vectors cut out of wider rows."""
+    d, T = 64, 30
+
+    def off(x):
+        flat = torch.empty(x.numel() + first, dtype=BF, device="cuda")
+        flat[first:] = x.reshape(-1)
+        return flat[first:].view_as(x), torch.nn.functional.pad(x, (first, 3))[:, :, first:first + d]
+    q, c = attention_case(scmx, 2 * hk, hk, L, T, d, True, seed=L)
+    want = scmx.sc_cache.cache_attention(q, c, 0.2)
+    for x in off(q):
+        assert torch.equal(x, q) and torch.equal(scmx.sc_cache.cache_attention(x, c, 0.2), want)
+    k, v = (torch.randn((hk, L, d), generator=gen(i), device="cuda").to(BF) for i in range(2))
+    scmx.sc_cache.kv_append(k, v, c)
+    for x, y in zip(off(k), off(v)):
+        other = quant_cache(scmx, hk, c.k.shape[1], d, T)
+        scmx.sc_cache.kv_append(x, y, other)
+        for name in ("k", "v", "ks", "vs"):
+            assert torch.equal(getattr(other, name)[:, T:T + L], getattr(c, name)[:, T:T + L])
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_attention_reads_its_position_from_the_device(scmx, int8):
     q, c = attention_case(scmx, 8, 4, 7, 900, 128, int8, extra=200)

@@ -173,14 +173,14 @@ using namespace scmx;
 extern "C" int scmx_kv_append(const uint16_t* k, int64_t k_head_stride, int64_t k_row_stride, const uint16_t* v, int64_t v_head_stride,
                               int64_t v_row_stride, int64_t L, int hk, int d, int64_t pos, const int32_t* pos_dev, int64_t capacity, int8_t* k_codes,
                               float* k_scales, int8_t* v_codes, float* v_scales, void* stream) {
-    SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_append: null buffer");
     SCMX_REQUIRE(d >= 16 && d <= 256 && d % 16 == 0, SCMX_EINVAL, "kv_append: head size %d (a multiple of 16 up to 256)", d);
     SCMX_REQUIRE(hk > 0 && L >= 0 && L < (1ll << 31) && capacity >= 1, SCMX_EINVAL, "kv_append: L=%lld hk=%d capacity=%lld", (long long)L, hk, (long long)capacity);
     SCMX_REQUIRE(pos_dev != nullptr || (pos >= 0 && pos + L <= capacity), SCMX_EINVAL, "kv_append: rows %lld .. %lld of a cache of %lld", (long long)pos,
                  (long long)(pos + L), (long long)capacity);
+    if (L == 0) return SCMX_OK;      // (tensors of no elements have no address)
+    SCMX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales, SCMX_EINVAL, "kv_append: null buffer");
     SCMX_REQUIRE(k_head_stride % 8 == 0 && k_row_stride % 8 == 0 && v_head_stride % 8 == 0 && v_row_stride % 8 == 0 && aligned16(k) && aligned16(v) &&
                      aligned16(k_codes) && aligned16(v_codes), SCMX_EINVAL, "kv_append: vectors must start on 16-byte boundaries");
-    if (L == 0) return SCMX_OK;
     KvWriteArgs a;
     a.k = k; a.v = v; a.k_hs = k_head_stride; a.v_hs = v_head_stride; a.k_rs = k_row_stride; a.v_rs = v_row_stride;
     a.kc = k_codes; a.vc = v_codes; a.ks = k_scales; a.vs = v_scales;

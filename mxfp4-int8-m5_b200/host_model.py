@@ -113,7 +113,8 @@ class QuantKVCache:
         """Appends bfloat16 k and v [heads, L, d]; the whole sequence's keys and values, read back."""
         L = k.shape[-2]
         assert self.offset + L <= self.capacity, "KV cache capacity exceeded"
-        C.kv_append(k.reshape(self.k.shape[0], L, -1), v.reshape(self.v.shape[0], L, -1), self)
+        heads, _, d = self.k.shape
+        C.kv_append(k.reshape(heads, L, d), v.reshape(heads, L, d), self)
         self.offset += L
         return C.kv_read(self)
 

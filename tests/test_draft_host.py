@@ -70,6 +70,15 @@ def test_entry_points_refuse(scmx):
         _refused(scmx, "scmx_verify", check(**kw), text)
 
 
+def test_no_tokens_are_appended(scmx):
+    """Tensors of no elements have no address: nothing is launched, whatever the pointers; sizes are checked all the same."""
+    append = lambda L, d=64, pos=0: (None, 0, 64, None, 0, 64, L, 2, d, pos, None, 16, P, P, P, P, None)      # noqa: E731
+    assert scmx._lib.lib().scmx_kv_append(*append(0)) == 0 and scmx._lib.lib().scmx_kv_append(*append(0, pos=16)) == 0
+    _refused(scmx, "scmx_kv_append", append(1), "null")
+    _refused(scmx, "scmx_kv_append", append(0, pos=17), "rows 17")
+    _refused(scmx, "scmx_kv_append", append(0, d=24), "head size")
+
+
 def test_lookup_draft(scmx):
     import importlib
     L = importlib.import_module(scmx.__name__ + ".decode").LookupDraft

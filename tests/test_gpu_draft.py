@@ -69,6 +69,16 @@ def test_append_and_read(scmx, hk, L, d, offset, layout):
     assert scmx.sc_cache.kv_read(c, 2, 2)[0].shape == (hk, 0, d)
 
 
+def test_append_of_no_tokens(scmx):
+    c = quant_cache(scmx, 2, 6, 64, 3)
+    none = torch.empty((2, 0, 64), dtype=BF, device="cuda")
+    for dev in (None, torch.tensor([2], dtype=torch.int32, device="cuda")):
+        scmx.sc_cache.kv_append(none, none, c, dev)
+    assert (c.k == 99).all() and (c.vs == 99).all()
+    k, v = c.update_and_fetch(none, none)
+    assert c.offset == 3 and k.shape == v.shape == (2, 3, 64)
+
+
 def test_append_takes_its_position_from_the_device(scmx):
     k, v = (torch.randn((2, 4, 64), generator=gen(i), device="cuda").to(BF) for i in (1, 2))
     for at in (0, 3, 6, 8, -2, 2 ** 31 - 1, -2 ** 31):

@@ -107,7 +107,7 @@ int scmx_rot_quant(const uint16_t* x, const float* signs, int64_t M, int64_t K, 
  * inv_freq f32 [d/2] non-null: rotary embedding (half-split pairs i, i + d/2) at position pos0 + row applied to the
  * normalized q and k; rope_table (optional) f32 [rope_rows, d] holds cos (d/2 values) then sin (d/2) of
  * position * inv_freq per position, (float)cos((double)(float)(pos * inv_freq)): used instead of evaluating them
- * for positions < rope_rows.  pos_dev non-null: one device int32 added to pos0 and kv_row0 (rows beyond the cache are dropped).
+ * for positions < rope_rows.  pos_dev non-null: one device int32 added to pos0 and kv_row0 (rows before or beyond the cache are dropped).
  * Replaces qkv_epilogue_headnorm, qkv_headnorm_y, qkv_fullnorm_y (e2e/sc_kernels.py:333-423,597-637); the rotary step
  * and cache append replace the MLX calls of e2e/fused_qwen3.py:197-203.  d a power of two, row <= 48 KB as float. */
 int scmx_qkv_norm(const void* src, int src_is_acc, const float* xscale, const float* wscale, const uint16_t* qn,

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256) qkv_norm_kernel(const QkvArgs a) {
         const int g = e >> a.d_shift, dd = e & (d - 1);
         const float y0 = rotated(e, normed(e)), y1 = rotated(e + 1, normed(e + 1));
         uint16_t* out;
-        if (g >= a.hq && kv_row >= a.kv_hs) continue;   // a device-side step beyond the cache: drop the row
+        if (g >= a.hq && (kv_row < 0 || kv_row >= a.kv_hs)) continue;   // a device-side step beyond the cache: drop the row
         if (g < a.hq) out = a.q + ((int64_t)g * a.q_hs + row) * d;
         else if (g < nh) out = a.k + ((int64_t)(g - a.hq) * a.kv_hs + kv_row) * d;
         else out = a.v + ((int64_t)(g - nh) * a.kv_hs + kv_row) * d;
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(256) qkv_norm_vec_kernel(const QkvArgs a) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int g = g0 + 16 * j;
-            if (g >= heads || (g >= a.hq && kv_row >= a.kv_hs)) continue;      // past the row; a device-side step beyond the cache
+            if (g >= heads || (g >= a.hq && (kv_row < 0 || kv_row >= a.kv_hs))) continue;      // past the row; a device-side step beyond the cache
             uint16_t* out;
             if (g < a.hq) out = a.q + ((int64_t)g * a.q_hs + row) * D + e0;
             else if (g < nh) out = a.k + ((int64_t)(g - a.hq) * a.kv_hs + kv_row) * D + e0;

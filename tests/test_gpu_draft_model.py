@@ -57,6 +57,47 @@ def test_fused_write_equals_its_steps(scmx, full, acc, hq, hk, d, L):
             assert torch.equal(q3, q) and torch.equal(dev.k, want.k) and torch.equal(dev.v, want.v) and torch.equal(dev.ks, want.ks)
 
 
+@pytest.mark.parametrize("full", [False, True])
+@pytest.mark.parametrize("d,quant", [(32, False), (64, False), (64, True), (128, False), (128, True)])
+def test_rows_outside_the_cache_are_dropped(scmx, full, d, quant):
+    """A position on the device before the cache's first row or past its last: rows inside are written, nothing else is, and queries are as ever.  The caches are cut
+    out of the middle of larger buffers."""
+    S, hq, hk, L, cap = scmx.sc_kernels, 4, 4, 5, 8
+    g = torch.Generator(device="cuda").manual_seed(d)
+    y = torch.randn((L, (hq + 2 * hk) * d), generator=g, device="cuda").to(BF)
+    qn, kn = (torch.ones(hq * d if full else d, dtype=BF, device="cuda") for _ in range(2))
+    inv = S.rope_inv_freq(d, 1e4)
+
+    def cache():
+        c, whole = scmx.host_model.KVCache(hk, d, 1), []
+        for name, shape, dt in (("k", (hk, cap, d), torch.int8 if quant else BF), ("v", (hk, cap, d), torch.int8 if quant else BF)) + (
+                (("ks", (hk, cap), torch.float32), ("vs", (hk, cap), torch.float32)) if quant else ()):
+            n = hk * cap * (d if len(shape) == 3 else 1)
+            whole.append(torch.full((3 * n,), 3, dtype=dt, device="cuda"))
+            setattr(c, name, whole[-1][n:2 * n].view(shape))
+        return c, whole
+    for at in (0, 3, 4, 6, 8, 9, -1, -4, -5, -8, 2 ** 31 - 1, -2 ** 31):
+        c, whole = cache()
+        q, _, _ = S._qkv_norm(y, None, None, qn, kn, 1e-6, L, hq, hk, d, full, (inv, 0), c, torch.tensor([at], dtype=torch.int32, device="cuda"))
+        assert torch.isfinite(q).all()
+        alone = scmx.host_model.KVCache(hk, d, L)
+        q0, k, v = S._qkv_norm(y, None, None, qn, kn, 1e-6, L, hq, hk, d, full, (inv, 0), alone)
+        inside = [i for i in range(L) if 0 <= at + i < cap]
+        want, whole2 = cache()
+        if inside and quant:                         # values do not turn: they tell which rows were written
+            want.offset = at + inside[0]
+            scmx.sc_cache.kv_append(k[:, inside], v[:, inside], want)
+        elif inside:
+            want.v[:, at + inside[0]:at + inside[0] + len(inside)] = v[:, inside]
+        assert torch.equal(c.v, want.v) and (not quant or torch.equal(c.vs, want.vs))
+        rows = [at + i for i in inside]
+        rest = [r for r in range(cap) if r not in rows]
+        assert (c.k[:, rest] == 3).all() and (not quant or (c.ks[:, rest] == 3).all())
+        for t in whole:                              # in front of the cache and behind it
+            n = t.numel() // 3
+            assert (t[:n] == 3).all() and (t[2 * n:] == 3).all()
+
+
 def test_rows_turn_where_they_are_told(scmx):
     """row_pos 0 .. L - 1 is no row_pos; the same position for all rows turns them alike."""
     S, HM = scmx.sc_kernels, scmx.host_model

@@ -60,8 +60,6 @@ def pack_olmoe(model, cache_path=None, fmt=F.DEFAULT, on_device=False):
 
 
 class FusedOlmoe:
-    _tree = None          # the draft tree whose rows are read (hidden)
-
     def __init__(self, model, flat, tile_gu=None, tile_d=None, bk=None, two_pass="auto", sort="count", compiled=True):
         """model: host_model.CausalLM (num_experts > 0) on the GPU; flat: pack_olmoe's dict.  Prompts whose average expert has fewer than
         MoeBlock.FUSED_BELOW (480) rows run the grouped GEMMs on the packed weights; from there on, and with two_pass=True, the experts are decoded to INT8
@@ -186,7 +184,7 @@ class FusedOlmoe:
         return (own and self.record is None and R // a.num_experts <= self.F4_ROWS and self._packed(R) and max(a.hidden_size, a.intermediate_size, self.layers[0][1]["o"].K) <= 8192
                 and M_.f4_fits(a.num_experts, a.hidden_size, a.intermediate_size, self.layers[0][1]["o"].K))
 
-    def _hidden_f4(self, h, cache, L):
+    def _hidden_f4(self, h, cache, L, tree=None):
         """The blocks on digit planes and the final norm: same bits as the products from INT8."""
         a = self.args
         D, E, Fi, nl = a.hidden_size, a.num_experts, a.intermediate_size, len(self.layers)
@@ -196,7 +194,7 @@ class FusedOlmoe:
             at, c, wq, wo = layer.self_attn, cache[i], ws["qkv"], ws["o"]
             fq, fo, fg, fd = M_.f4_factors((wq.bcodes, 1, wq.N, wq.K), (wo.bcodes, 1, wo.N, wo.K), (ex["gu"][1], E, 2 * Fi, D), (ex["down"][1], E, D, Fi))
             y = S.mm_f4(dig, wq.codes, fq, xs, wq.wscale, 1)
-            dig, xs = self._attend(at, c, y, L, L, digits=True)
+            dig, xs = self._attend(at, c, y, L, L, tree, digits=True)
             h = S.mm_f4(dig, wo.codes, fo, xs, wo.wscale, 2, res=h)
             xq, xs, xn = S.rmsnorm_quant_n(h, layer.post_attention_layernorm.weight, self.eps, L)
             inds, scores = self.route(layer, xn, L)
@@ -211,10 +209,9 @@ class FusedOlmoe:
             h, dig, xs, xn = M_.combine_norm(yd, pos, scores, h, nn, self.eps, quant=False if last else "digits", normed=last)
         return xn
 
-    def _attend(self, at, c, y, L, Mp, digits=False):
+    def _attend(self, at, c, y, L, Mp, tree=None, digits=False):
         """INT8 rows (or digit planes) of the attention output from the q|k|v rows y, whose keys and values go to the cache."""
         a = self.args
-        tree = self._tree
         q, k, v = S.qkv_fullnorm_y(y, at.q_norm.weight, at.k_norm.weight, self.eps, L, a.num_attention_heads, a.head_dim,
                                    rope=(self.inv_freq, c.offset, self.rope_cs), cache=c, row_pos=None if tree is None else tree.depths,
                                    pos_dev=None if tree is None else tree.pos)
@@ -255,22 +252,13 @@ class FusedOlmoe:
     @torch.no_grad()
     def hidden(self, ids, cache, tree=None):
         """Final normed hidden states [1, L, D] for ids [1, L]; tree (sc_draft.DraftTree): as in FusedQwen3.hidden."""
-        if tree is None:
-            return self._hidden(ids, cache)
-        assert len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
-        self._tree = tree
-        try:
-            return self._hidden(ids, cache)
-        finally:
-            self._tree = None
-
-    def _hidden(self, ids, cache):
+        assert tree is None or len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
         a = self.args
         D = a.hidden_size
         h = self.model.model.embed_tokens(ids)[0]
         L = h.shape[0]
         if L > 0 and self._f4(L):
-            return self._hidden_f4(h.contiguous(), cache, L)[None]
+            return self._hidden_f4(h.contiguous(), cache, L, tree)[None]
         Mp = S.pad_rows(L)
         if Mp != L:
             h = torch.nn.functional.pad(h, (0, 0, 0, Mp - L))
@@ -290,7 +278,7 @@ class FusedOlmoe:
                 self._decode_experts(i + 1)                    # under this layer's attention and GEMMs
             wq, wo = ws["qkv"], ws["o"]
             y = S.mm_epi(xq, wq.unpack(), xs, wq.wscale, 1)
-            xq, xs = self._attend(at, c, y, L, Mp)
+            xq, xs = self._attend(at, c, y, L, Mp, tree)
             h = S.mm_epi(xq, wo.unpack(), xs, wo.wscale, 2, res=h)
             xq, xs, xn = S.rmsnorm_quant_n(h, layer.post_attention_layernorm.weight, self.eps)
             inds, scores = self.route(layer, xn, L)

@@ -77,14 +77,17 @@ def attend_quant(sdpa, q, k, v, scale, Mp, digits=False):
     return S.quant_digits(o) if digits else S.act_quant(o, Mp)
 
 
+def _given(tree):
+    """The last argument of the pieces of a pass, where it reads a tree: without one a caller's own piece, which may not know of trees, is called as it always was."""
+    return () if tree is None else (tree,)
+
+
 def tiles_for(M):
     """The reference tunes Metal tiles per shape here (e2e/fused_qwen3.py:76-80); the tcgen05 GEMM picks its own N tile."""
     return {"qkv": None, "o": None, "gu": None, "down": None}
 
 
 class FusedQwen3:
-    _tree = None          # the draft tree whose rows are read (hidden)
-
     def __init__(self, model, packed, resident=False, overlap=True, epilogue="gemm", compiled=True, fmt=None, rot=False,
                  fuse_rope=True):
         """model: host_model.CausalLM on the GPU; packed: {"layers.{i}.{path}": (codes, bcodes, wscale)}.  resident keeps the
@@ -152,17 +155,17 @@ class FusedQwen3:
         if self.ring is not None:
             self.ring.released(g)
 
-    def _qkv(self, at, c, src, xs, ws, L):
+    def _qkv(self, at, c, src, xs, ws, L, tree=None):
         a = self.args
         hq, hk, d = a.num_attention_heads, a.num_key_value_heads, a.head_dim
-        kw = dict(rope=(self.inv_freq, c.offset, self.rope_cs), cache=c) if self.fuse_rope or self._tree is not None else {}
-        if self._tree is not None:
-            kw.update(row_pos=self._tree.depths, pos_dev=self._tree.pos)
+        kw = dict(rope=(self.inv_freq, c.offset, self.rope_cs), cache=c) if self.fuse_rope or tree is not None else {}
+        if tree is not None:
+            kw.update(row_pos=tree.depths, pos_dev=tree.pos)
         if src.dtype == torch.int32:
             q, k, v = S.qkv_epilogue_headnorm(src, xs, ws, at.q_norm.weight, at.k_norm.weight, self.eps, L, hq, hk, d, **kw)
         else:
             q, k, v = S.qkv_headnorm_y(src, at.q_norm.weight, at.k_norm.weight, self.eps, L, hq, hk, d, **kw)
-        if self._tree is not None:                            # the rows stay behind the cache's end until some are kept
+        if tree is not None:                                  # the rows stay behind the cache's end until some are kept
             return q, k, v
         if self.fuse_rope:
             c.offset += L
@@ -173,11 +176,11 @@ class FusedQwen3:
             k, v = c.update_and_fetch(k, v)
         return q, k, v
 
-    def _attention(self, i, at, c, src, xs, ws, L, Mp):
+    def _attention(self, i, at, c, src, xs, ws, L, Mp, tree=None):
         """-> attention output (None unless it is recorded), its INT8 rows and their scales."""
-        q, k, v = self._qkv(at, c, src, xs, ws, L)
-        if self._tree is not None:
-            o = C.cache_attention(q, c, at.scale, self._tree.mask, self._tree.pos)
+        q, k, v = self._qkv(at, c, src, xs, ws, L, *_given(tree))
+        if tree is not None:
+            o = C.cache_attention(q, c, at.scale, tree.mask, tree.pos)
             return (o, *self.act_q(o, Mp))
         own = type(self).act_q is not _ACT_Q or "act_q" in self.__dict__      # a quantizer of the caller's: it wants whole rows
         if own or self.rot is True or (self.record is not None and i in self.record_layers):
@@ -205,17 +208,17 @@ class FusedQwen3:
         widths = {w.K for w in self.layers[0][1].values()}
         return max(widths) <= 8192 and M_.f4_fits(1, *widths)
 
-    def _blocks_f4(self, h, cache, L):
+    def _blocks_f4(self, h, cache, L, tree=None):
         """_blocks_gemm_epi on digit planes: same bits."""
         for i, (layer, ws) in enumerate(self.layers):
             at, fac = layer.self_attn, dict(zip(ws, M_.f4_factors(*((w.bcodes, 1, w.N, w.K) for w in ws.values()))))
             mm = lambda g, dig, xs, epi, res=None: S.mm_f4(dig, ws[g].codes, fac[g], xs, ws[g].wscale, epi, res)      # noqa: E731
             dig, xs = S.quant_digits(h, layer.input_layernorm.weight, self.eps)
-            q, k, v = self._qkv(at, cache[i], mm("qkv", dig, xs, 1), None, None, L)
-            if self._tree is None:
+            q, k, v = self._qkv(at, cache[i], mm("qkv", dig, xs, 1), None, None, L, *_given(tree))
+            if tree is None:
                 rows = attend_quant(self.sdpa, q, k, v, at.scale, L, digits=True)
             else:
-                rows = S.quant_digits(C.cache_attention(q, cache[i], at.scale, self._tree.mask, self._tree.pos))
+                rows = S.quant_digits(C.cache_attention(q, cache[i], at.scale, tree.mask, tree.pos))
             h = mm("o", *rows, 2, h)
             act = mm("gu", *S.quant_digits(h, layer.post_attention_layernorm.weight, self.eps), 3)
             h = mm("down", *S.quant_digits(act), 2, h)
@@ -226,21 +229,12 @@ class FusedQwen3:
     def hidden(self, ids, cache, tree=None):
         """Final normed hidden states [1, L, D] for prompt ids [1, L] (prefill into a fresh or offset cache).  tree (sc_draft.DraftTree): the ids are its rows,
         each of which sees the cache and its ancestors; their keys and values are written behind the cache's end, which does not move (sc_cache.kv_keep)."""
-        if tree is None:
-            return self._hidden(ids, cache)
-        assert len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
-        self._tree = tree
-        try:
-            return self._hidden(ids, cache)
-        finally:
-            self._tree = None
-
-    def _hidden(self, ids, cache):
+        assert tree is None or len(tree) == ids.shape[1], f"{ids.shape[1]} ids for a tree of {len(tree)} rows"
         S.set_format(self.fmt)
         h = self.model.model.embed_tokens(ids)[0]
         L = h.shape[0]
         if self._f4(L):
-            h = self._blocks_f4(h.contiguous(), cache, L)
+            h = self._blocks_f4(h.contiguous(), cache, L, tree)
             return S.rmsnorm_quant_n(h, self.model.model.norm.weight, self.eps, L)[2][None]
         Mp = S.pad_rows(L)
         if Mp != L:
@@ -248,13 +242,13 @@ class FusedQwen3:
         h = h.contiguous()
         if self.ring is not None:
             self.ring.begin(self.seq)
-        h = (self._blocks_gemm_epi if self.epilogue == "gemm" else self._blocks_row_epi)(h, cache, L, Mp)
+        h = (self._blocks_gemm_epi if self.epilogue == "gemm" else self._blocks_row_epi)(h, cache, L, Mp, *_given(tree))
         if self.ring is not None:
             self.ring.end()
         xn = S.rmsnorm_quant_n(h, self.model.model.norm.weight, self.eps, Mp)[2]
         return xn[:L][None]
 
-    def _blocks_gemm_epi(self, h, cache, L, Mp):
+    def _blocks_gemm_epi(self, h, cache, L, Mp, tree=None):
         nl = len(self.layers)
         xq, xs = self.rms_q(h, self.layers[0][0].input_layernorm.weight, Mp)
         for i, (layer, ws) in enumerate(self.layers):
@@ -263,7 +257,7 @@ class FusedQwen3:
             y = S.mm_epi(xq, wq, xs, ws["qkv"].wscale, 1)
             self._done(g)
             self._rec(i, "qkv", h, xq, wq, None)
-            o, xq, xs = self._attention(i, at, cache[i], y, None, None, L, Mp)
+            o, xq, xs = self._attention(i, at, cache[i], y, None, None, L, Mp, *_given(tree))
             wq = self._w(g + 1)
             self._rec(i, "o", o, xq, wq, None)
             h = S.mm_epi(xq, wq, xs, ws["o"].wscale, 2, res=h)
@@ -282,7 +276,7 @@ class FusedQwen3:
                 xq, xs = self.rms_q(h, self.layers[i + 1][0].input_layernorm.weight)
         return h
 
-    def _blocks_row_epi(self, h, cache, L, Mp):
+    def _blocks_row_epi(self, h, cache, L, Mp, tree=None):
         nl = len(self.layers)
         xq, xs = self.rms_q(h, self.layers[0][0].input_layernorm.weight, Mp)
         for i, (layer, ws) in enumerate(self.layers):
@@ -291,7 +285,7 @@ class FusedQwen3:
             acc = S.mm_i8_i32(xq, wq)
             self._done(g)
             self._rec(i, "qkv", h, xq, wq, acc)
-            o, xq, xs = self._attention(i, at, cache[i], acc, xs, ws["qkv"].wscale, L, Mp)
+            o, xq, xs = self._attention(i, at, cache[i], acc, xs, ws["qkv"].wscale, L, Mp, *_given(tree))
             wq = self._w(g + 1)
             acc = S.mm_i8_i32(xq, wq)
             self._done(g + 1)

@@ -161,6 +161,38 @@ def test_rows_of_a_tree_are_their_paths(scmx, kind, kw, dtype):
     scmx._lib.check_status()
 
 
+@pytest.mark.parametrize("kind,kw", [("qwen3", {}), ("qwen3", dict(resident=True)), ("qwen3", dict(resident=True, epilogue="row")), ("olmoe", {})])
+def test_a_prompt_beside_a_drafted_pass(scmx, kind, kw, monkeypatch):
+    """A tree belongs to the call that was given it: a prompt and other trees that are read while a pass over a tree is under way, as from another thread, are
+    what they are alone, and so is the pass.  (Models without buffers of weights, which take one pass at a time.)"""
+    fused, _ = build(scmx, kind, **kw)
+    C, D = scmx.sc_cache, scmx.sc_draft
+    ids = torch.randint(0, 512, (1, 7), generator=torch.Generator(device="cuda").manual_seed(8), device="cuda")
+    trees = [None, D.DraftTree([-1] + [0] * 6), D.DraftTree(list(range(-1, 6)))]
+
+    def read(tree):
+        cache = fused.make_cache(40)
+        h = fused.hidden(ids, cache, tree)
+        return h, cache[0].offset, cache[1].k[:, :7].clone()
+    alone = [read(tree) for tree in trees]
+    assert [offset for _, offset, _ in alone] == [7, 0, 0] and not torch.equal(alone[1][0], alone[2][0])
+    inside, real, started = [], C.cache_attention, []
+
+    def attention(*args, **kw):
+        if not started:
+            started.append(1)
+            inside.extend(read(tree) for tree in trees)
+        return real(*args, **kw)
+    monkeypatch.setattr(C, "cache_attention", attention)
+    for i in (1, 2):
+        started.clear()
+        inside.clear()
+        outer = read(trees[i])
+        assert len(inside) == 3
+        for got, want in zip([outer] + inside, [alone[i]] + alone):
+            assert torch.equal(got[0], want[0]) and got[1] == want[1] and torch.equal(got[2], want[2])
+
+
 @pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
 def test_int8_cache_steps(scmx, kind):
     """Steps on an INT8 cache: near the bfloat16 cache's (a code is off by at most 1 / 254 of its vector's largest value), and the captured ones the same as the others."""

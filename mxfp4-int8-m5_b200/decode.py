@@ -313,6 +313,8 @@ class DecodeDraft:
 
     def __init__(self, fused, propose=None):
         a = fused.args
+        if not hasattr(a, "num_key_value_heads"):
+            raise ValueError(f"drafts are read by FusedQwen3 and FusedOlmoe, not by {type(fused).__name__}")
         if not C.attention_supported(a.num_attention_heads, a.num_key_value_heads, a.head_dim):
             raise ValueError(f"attention of drafted rows: head size {a.head_dim} (64 or 128)")
         self.f, self.propose = fused, propose or LookupDraft()

@@ -69,15 +69,18 @@ class Engine:
         """n tokens after `prompt` (list of ids), greedy: the prompt through step(), then the decoder's captured graph, or, with draft (a proposal as
         decode.DecodeDraft takes it, for instance decode.LookupDraft()), passes over trees of drafted tokens."""
         assert n >= 1 and len(prompt) + n - 1 <= self.pool.capacity, "prompt and continuation exceed the cache"
-        logits = self.step([(rid, prompt, [len(prompt) - 1])])[0]
-        first = logits[-1].argmax().reshape(1, 1)
-        out = [int(first)]
-        if n > 1 and draft is not None:
+        if draft is not None and n > 1:
             if self.drafts is None:
                 self.drafts = DEC.DecodeDraft(self.bundle.prefill)
             self.drafts.propose = draft
-            out += self.drafts.generate(first, self.live[rid], n - 1, prompt).tolist()
-        elif n > 1:
-            out += self.bundle.decode.generate(first, self.live[rid], n - 1).tolist()
-        self.finish(rid)
+        try:                                                      # a call that ends early leaves no request behind, which the next one would continue
+            logits = self.step([(rid, prompt, [len(prompt) - 1])])[0]
+            first = logits[-1].argmax().reshape(1, 1)
+            out = [int(first)]
+            if n > 1 and draft is not None:
+                out += self.drafts.generate(first, self.live[rid], n - 1, prompt).tolist()
+            elif n > 1:
+                out += self.bundle.decode.generate(first, self.live[rid], n - 1).tolist()
+        finally:
+            self.finish(rid)
         return out

@@ -140,3 +140,43 @@ def test_entry_points_run_as_a_script():
     later = {node.name for node in body[guard:] if isinstance(node, ast.FunctionDef)}
     called = {node.func.id for f in body for node in ast.walk(f) if isinstance(node, ast.Call) and isinstance(node.func, ast.Name)}
     assert {"build", "smoke"} <= defined and not called & later
+
+
+def test_engine_keeps_nothing_of_a_call_that_ends_early(scmx):
+    """A proposal that raises, a draft that is refused, a decoder that fails: the request is gone, its cache back in the pool, and the next call starts anew.  A model
+    that reads no drafts is refused before its prompt is read."""
+    import importlib
+    from types import SimpleNamespace as N
+    E = importlib.import_module(scmx.__name__ + ".engine")
+
+    class Cache:
+        def __init__(self):
+            self.offset, self.capacity = 0, 32
+
+        def reset(self):
+            self.offset = 0
+    read = []
+
+    def hidden(ids, cache):
+        read.append((cache[0].offset, ids.shape[1]))
+        cache[0].offset += ids.shape[1]
+        return torch.zeros(1, ids.shape[1], 4)
+
+    def fail(*a):
+        raise RuntimeError("decoder")
+    args = N(num_attention_heads=4, num_key_value_heads=2, head_dim=64, vocab_size=8)
+    prefill = N(args=args, inv_freq=torch.zeros(1), make_cache=lambda capacity: [Cache()], hidden=hidden, logits=lambda h: torch.zeros(*h.shape[:2], 8))
+    engine = E.Engine(N(prefill=prefill, decode=N(generate=fail)), 32, device="cpu")
+
+    def gone(text, most):
+        raise KeyError("proposal")
+    for draft, error in ((gone, KeyError), (lambda text, most: ([text[-1], 9], [-1, 0]), ValueError), (None, RuntimeError)):
+        for _ in range(2):
+            with pytest.raises(error):
+                engine.generate([1, 2, 3], 4, draft=draft)
+            assert not engine.live and len(engine.pool.free) == 1 and read.pop() == (0, 3)
+    prefill.args = N(layers=[])                             # a hybrid decoder
+    other = E.Engine(N(prefill=prefill, decode=None), 32, device="cpu")
+    with pytest.raises(ValueError, match="drafts"):
+        other.generate([1, 2, 3], 4, draft=gone)
+    assert not other.live and not read

@@ -387,7 +387,7 @@ class DecodeDraft:
 
     @torch.no_grad()
     def step(self, text, cache, temperature=0.0, u=None, most=D.MAX_ROWS):
-        """One pass: text (list of ids, the last one not in the cache yet) -> the tokens that it adds, at least one.  u float32 [64]: random numbers in [0, 1)."""
+        """One pass: text (list of ids, the last one not in the cache yet) -> the tokens that it adds, at least one.  u float32 [64] on the model's device: random numbers in [0, 1)."""
         assert cache[0].offset + 1 <= cache[0].capacity, "KV cache capacity exceeded"
         most = max(1, min(most, D.MAX_ROWS, cache[0].capacity - cache[0].offset))
         tokens, parents, *probs = self.propose(text, most)
@@ -399,7 +399,9 @@ class DecodeDraft:
             raise ValueError(f"drafted tokens {tokens}: 0 .. {self.f.args.vocab_size - 1}")
         if temperature and (u is None or u.dim() != 1 or u.numel() < n):
             raise ValueError(f"temperature {temperature}: 0, or random numbers for {n} rows")
-        u = u[:n] if temperature else None
+        if temperature and (u.dtype != torch.float32 or u.device != self.dev):      # here: a replay would copy them, rounded, from wherever they are
+            raise TypeError(f"random numbers {u.dtype} on {u.device}: float32 on {self.dev}")
+        u = u[:n].contiguous() if temperature else None
         probs = probs[0] if probs else None
         out = self._captured(tokens, parents, cache, u, temperature) if probs is None else None
         if out is None:

@@ -180,3 +180,21 @@ def test_engine_keeps_nothing_of_a_call_that_ends_early(scmx):
     with pytest.raises(ValueError, match="drafts"):
         other.generate([1, 2, 3], 4, draft=gone)
     assert not other.live and not read
+
+
+def test_random_numbers_are_checked_in_every_pass(scmx):
+    """Numbers of another type or device are refused before any pass, a captured one too, which would take them through a copy."""
+    import importlib
+    from types import SimpleNamespace as N
+    DD = importlib.import_module(scmx.__name__ + ".decode").DecodeDraft
+    d, cache = DD.__new__(DD), [N(offset=4, capacity=8)]
+    d.f, d.dev, d.propose = N(args=N(vocab_size=16)), torch.device("cpu"), lambda text, most: ([3, 2], [-1, 0])
+    taken = []
+    d._captured = lambda tokens, parents, cache, u, temperature: taken.append(u) or torch.tensor([0, -1, 5])
+    for u in (torch.zeros(64, dtype=torch.float64), torch.zeros(64, dtype=torch.bfloat16), torch.zeros(64, device="meta"), torch.zeros(64, dtype=torch.long)):
+        with pytest.raises(TypeError, match="random numbers"):
+            d.step([1, 3], cache, 0.5, u)
+    assert not taken and cache[0].offset == 4
+    assert d.step([1, 3], cache, 0.5, torch.arange(128.0)[::2]) == [5]
+    assert taken[0].tolist() == [0.0, 2.0] and taken[0].is_contiguous() and cache[0].offset == 5
+    assert d.step([1, 3], cache, 0.0, torch.zeros(1, dtype=torch.float64)) == [5] and taken[1] is None      # greedy: not read

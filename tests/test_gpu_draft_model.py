@@ -334,6 +334,23 @@ def test_sampled_generation_repeats_with_its_generator(scmx):
     assert out[0] == out[1] and all(0 <= t < 512 for t in out[0])
 
 
+def test_replayed_passes_refuse_what_the_first_refuses(scmx):
+    """Random numbers of another type or place, at a pass launch by launch, at the one that is captured and at a replay."""
+    fused, _ = build(scmx, "qwen3")
+    d = mod(scmx, "decode").DecodeDraft(fused, lambda text, most: ([text[-1], 3], [-1, 0]))
+    cache, text = fused.make_cache(60), list(range(20))
+    fused.hidden(torch.tensor([text], device="cuda"), cache)
+    text.append(7)
+    for _ in range(4):
+        good = torch.rand(64, device="cuda")
+        for u in (good.cpu(), good.double(), good.to(BF)):
+            with pytest.raises(TypeError, match="random numbers"):
+                d.step(text, cache, 0.8, u)
+        text += d.step(text, cache, 0.8, good)
+    assert d._graphs[2][2, 0.8] is not None
+    scmx._lib.check_status()
+
+
 def test_engine_with_drafts(scmx):
     fused, decoder = build(scmx, "qwen3")
     R, E, DEC = mod(scmx, "registry"), mod(scmx, "engine"), mod(scmx, "decode")

@@ -319,7 +319,7 @@ class DecodeDraft:
             raise ValueError(f"attention of drafted rows: head size {a.head_dim} (64 or 128)")
         self.f, self.propose = fused, propose or LookupDraft()
         self.dev = fused.inv_freq.device
-        self._graphs = None                                       # (cache, memory pool, {(rows, temperature): captured pass})
+        self._graphs = None                                       # (a cache's layers, where their tensors are, {(rows, temperature): captured pass}, memory pool)
 
     @torch.no_grad()
     def read(self, tokens, tree, cache):
@@ -339,9 +339,7 @@ class DecodeDraft:
         n, f, a = len(tokens), self.f, self.f.args
         if not f._f4(n) or (cache[0].k.dtype == torch.int8 and a.num_attention_heads + 2 * a.num_key_value_heads > 96):
             return None
-        if self._graphs is None or self._graphs[0] is not cache or len(self._graphs[2]) >= 128:      # (128: temperatures that keep changing)
-            self._graphs = (cache, torch.cuda.graph_pool_handle(), {})
-        _, pool, known = self._graphs
+        known, pool = self._passes(cache)
         key = (n, float(temperature))
         if key not in known:
             known[key] = None
@@ -355,6 +353,14 @@ class DecodeDraft:
             numbers.copy_(u)
         g.replay()
         return out
+
+    def _passes(self, cache):
+        """The captured passes over a cache and their memory pool.  They name its layers' tensors: others in their place, or other layers in the list, are another cache."""
+        where = [(c.k.shape, *(t.data_ptr() for t in ((c.k, c.v, c.ks, c.vs) if c.k.dtype == torch.int8 else (c.k, c.v)))) for c in cache]
+        known = self._graphs
+        if known is None or known[1] != where or any(a is not b for a, b in zip(known[0], cache)) or len(known[2]) >= 128:      # (128: temperatures that keep changing)
+            self._graphs = (tuple(cache), where, {}, torch.cuda.graph_pool_handle())
+        return self._graphs[2:]
 
     def _capture(self, parents, cache, temperature, inputs, u, pool):
         """(graph, its inputs int64 [4 n + 1]: tokens, mask, parents, depths, position; its random numbers; its result; what it reads).  The warm-up is this very pass."""

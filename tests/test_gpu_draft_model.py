@@ -334,6 +334,52 @@ def test_sampled_generation_repeats_with_its_generator(scmx):
     assert out[0] == out[1] and all(0 <= t < 512 for t in out[0])
 
 
+@pytest.mark.parametrize("dtype", [None, torch.int8])
+def test_replays_follow_the_caches_tensors(scmx, dtype):
+    """After captured passes a layer's tensors are replaced, then the layer in the list, then the whole list by one of the same layers: passes write to what the cache holds now and to
+    nothing else.  (Everything replaced stays alive here.)"""
+    fused, _ = build(scmx, "qwen3")
+    HM, d = scmx.host_model, mod(scmx, "decode").DecodeDraft(fused, lambda text, most: ([text[-1], 3, 5], [-1, 0, 0]))
+    cache, text = fused.make_cache(80, dtype), list(range(20))
+    names = ("k", "v", "ks", "vs") if dtype else ("k", "v")
+    for c in cache:
+        for name in names:
+            getattr(c, name).zero_()
+    fused.hidden(torch.tensor([text], device="cuda"), cache)
+    text.append(7)
+    for _ in range(3):
+        text += d.step(text, cache)
+    captured = d._graphs[2][3, 0.0]
+    assert captured is not None
+    old = []
+
+    def check(c):
+        """Two passes (launched, captured) and a replay: the old tensors stay as they are, the new ones have the rows."""
+        first = c[1].offset
+        before = [t.clone() for t in old]
+        for _ in range(3):
+            for name in names:
+                getattr(c[1], name)[:, c[1].offset:].zero_()
+            text.extend(d.step(text, c))
+        assert all(torch.equal(a, b) for a, b in zip(before, old))
+        assert all((getattr(c[1], name)[:, first:c[1].offset] != 0).any(-1).all() for name in ("k", "v"))
+    for name in names:                               # a layer's tensors
+        old.append(getattr(cache[1], name))
+        setattr(cache[1], name, old[-1].clone())
+    check(cache)
+    assert d._graphs[2][3, 0.0] is not captured
+    layer = type(cache[1])(cache[1].k.shape[0], cache[1].k.shape[2], 80)      # the layer
+    for name in names:
+        old.append(getattr(cache[1], name))
+        getattr(layer, name).copy_(old[-1])
+    layer.offset, cache[1] = cache[1].offset, layer
+    check(cache)
+    captured = d._graphs[2][3, 0.0]
+    check(list(cache))                               # the list alone: the same cache
+    assert d._graphs[2][3, 0.0] is captured
+    scmx._lib.check_status()
+
+
 def test_replayed_passes_refuse_what_the_first_refuses(scmx):
     """Random numbers of another type or place, at a pass launch by launch, at the one that is captured and at a replay."""
     fused, _ = build(scmx, "qwen3")

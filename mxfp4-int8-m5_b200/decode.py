@@ -22,6 +22,7 @@ decide which of them are kept (speculative decoding).  The caches of all W4A8 de
 DecodeHybrid is the same for hybrid decoders (fused_hybrid.FusedHybrid): GEMVs on bfloat16 or float32 weights with the mixers'
 one-token kernels between them, float32 activations."""
 import ctypes
+import weakref
 
 import numpy as np
 import torch
@@ -301,6 +302,14 @@ class LookupDraft:
         return rows, parents
 
 
+def _reference(x):
+    """A weak reference, or a strong one to what has none (a SimpleNamespace)."""
+    try:
+        return weakref.ref(x)
+    except TypeError:
+        return lambda: x
+
+
 class DecodeDraft:
     """Speculative decoding over a FusedQwen3 or FusedOlmoe: `propose` drafts a tree of tokens, one pass of the model reads all its rows, and verify_draft
     keeps a path of them and draws the token after it, distributed as the model alone would draw (greedy at temperature 0).
@@ -309,7 +318,9 @@ class DecodeDraft:
     [rows, vocabulary] on the device where children were drawn from them (row i: what row i's children were drawn from).
 
     Where the model reads that many rows on digit planes (nothing beside the current stream, no buffers of its own), the second pass of as many rows
-    over a cache is captured and later ones are replays: the launches of a pass over 28 layers take the host 4.5 ms."""
+    over a cache is captured and later ones are replays (of up to 8 caches that take turns): the launches of a pass over 28 layers take the host 4.5 ms."""
+
+    CACHES = 8            # caches that are read in turn keep their captured passes
 
     def __init__(self, fused, propose=None):
         a = fused.args
@@ -319,7 +330,7 @@ class DecodeDraft:
             raise ValueError(f"attention of drafted rows: head size {a.head_dim} (64 or 128)")
         self.f, self.propose = fused, propose or LookupDraft()
         self.dev = fused.inv_freq.device
-        self._graphs = None                                       # (a cache's layers, where their tensors are, {(rows, temperature): captured pass}, memory pool)
+        self._graphs, self._kept = None, []                       # of the cache read last, and of others: (layers, where their tensors are, {(rows, temperature): captured pass}, memory pool)
 
     @torch.no_grad()
     def read(self, tokens, tree, cache):
@@ -357,9 +368,13 @@ class DecodeDraft:
     def _passes(self, cache):
         """The captured passes over a cache and their memory pool.  They name its layers' tensors: others in their place, or other layers in the list, are another cache."""
         where = [(c.k.shape, *(t.data_ptr() for t in ((c.k, c.v, c.ks, c.vs) if c.k.dtype == torch.int8 else (c.k, c.v)))) for c in cache]
-        known = self._graphs
-        if known is None or known[1] != where or any(a is not b for a, b in zip(known[0], cache)) or len(known[2]) >= 128:      # (128: temperatures that keep changing)
-            self._graphs = (tuple(cache), where, {}, torch.cuda.graph_pool_handle())
+        same = lambda e: e[1] == where and all(r() is c for r, c in zip(e[0], cache))      # noqa: E731
+        entry = next((e for e in self._kept if same(e)), None)
+        self._kept = [e for e in self._kept if e is not entry and all(r() is not None for r in e[0])]      # a cache that is gone takes its passes along
+        if entry is None or len(entry[2]) >= 128:                                                          # (128: temperatures that keep changing)
+            entry = (tuple(map(_reference, cache)), where, {}, torch.cuda.graph_pool_handle())
+        self._kept = self._kept[1 - self.CACHES:] + [entry]
+        self._graphs = entry
         return self._graphs[2:]
 
     def _capture(self, parents, cache, temperature, inputs, u, pool):

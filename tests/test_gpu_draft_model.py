@@ -380,6 +380,47 @@ def test_replays_follow_the_caches_tensors(scmx, dtype):
     scmx._lib.check_status()
 
 
+def test_caches_that_take_turns_keep_their_passes(scmx):
+    """Two texts in turn through one DecodeDraft: each cache's pass is captured once and replayed, with the tokens that each text gets alone; a cache that is given up is not
+    kept alive, and the least recently read of many gives its passes up."""
+    import gc
+    import weakref
+    fused, _ = build(scmx, "qwen3")
+    DEC = mod(scmx, "decode")
+    propose = lambda text, most: ([text[-1], 3, 5], [-1, 0, 0])      # noqa: E731
+    prompts = [list(range(20)), list(range(100, 130))]
+
+    def start(prompt):
+        cache = fused.make_cache(80)
+        fused.hidden(torch.tensor([prompt], device="cuda"), cache)
+        return cache
+    want = []
+    for prompt in prompts:
+        alone, cache, text = DEC.DecodeDraft(fused, propose), start(prompt), prompt + [7]
+        for _ in range(6):
+            text += alone.step(text, cache)
+        want.append(text)
+    d, caches, texts, captured = DEC.DecodeDraft(fused, propose), [start(p) for p in prompts], [p + [7] for p in prompts], [[], []]
+    for _ in range(6):
+        for i in (0, 1):
+            texts[i] += d.step(texts[i], caches[i])
+            captured[i].append(d._graphs[2][3, 0.0])
+    assert texts == want
+    for seen in captured:
+        assert seen[0] is None and seen[1] is not None and all(x is seen[1] for x in seen[1:])
+    layer = weakref.ref(caches[0][0])
+    caches[0] = None
+    gc.collect()
+    assert layer() is None
+    d.step(texts[1], caches[1])
+    assert len(d._kept) == 1
+    more = [start(prompts[0]) for _ in range(d.CACHES)]
+    for cache in more:
+        d.step(prompts[0] + [7], cache)
+    assert len(d._kept) == d.CACHES and all(e[0][0]() is c[0] for e, c in zip(d._kept, more))
+    scmx._lib.check_status()
+
+
 def test_replayed_passes_refuse_what_the_first_refuses(scmx):
     """Random numbers of another type or place, at a pass launch by launch, at the one that is captured and at a replay."""
     fused, _ = build(scmx, "qwen3")

@@ -119,6 +119,8 @@ def kv_keep(caches, rows, pos=None, pos_dev=None):
             layers += (k.data_ptr(), v.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr())
         else:
             layers += (k.data_ptr(), v.data_ptr(), 0, 0)
+    if len({*layers[::4], *layers[1::4]}) < 2 * len(caches):      # its rows would move twice, or while others move
+        raise ValueError("kv_keep: a cache's tensors are in the list twice")
     table = array("Q", layers)
     _lib.call("scmx_kv_keep", table.buffer_info()[0], len(caches), rows.data_ptr(), n, pos, dev, hk, d, cap, int8, _lib.stream())
 

@@ -135,6 +135,21 @@ def test_keep(scmx, int8, layers, hk, d, n, rows):
     assert all(torch.equal(getattr(a, m), getattr(c, m)) for a, c in zip(again, caches) for m in names)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_keep_refuses_a_cache_that_is_listed_twice(scmx, int8):
+    make = lambda: quant_cache(scmx, 2, 12, 64, 3) if int8 else scmx.host_model.KVCache(2, 64, 12)      # noqa: E731
+    a, b, rows = make(), make(), torch.tensor([0, 2, 1], dtype=torch.int32, device="cuda")
+    shared = SimpleNamespace(k=a.k, v=b.v, offset=3)
+    mirror = SimpleNamespace(k=b.k, v=b.k, offset=3)
+    if int8:
+        for c in (shared, mirror):
+            c.ks, c.vs = a.ks, b.vs
+    for caches in ([a, a], [a, b, a], [a, shared], [mirror]):
+        with pytest.raises(ValueError, match="twice"):
+            scmx.sc_cache.kv_keep(caches, rows, pos=3)
+    scmx.sc_cache.kv_keep([a, b], rows, pos=3)
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------------------
 
 def attention_case(scmx, hq, hk, n, T, d, int8, seed=0, extra=5, std=1.5):

@@ -271,6 +271,26 @@ def test_drafted_generation_is_the_models(scmx, kind, dtype):
 
 @pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
 @pytest.mark.parametrize("dtype", [None, torch.int8])
+def test_lookup_of_a_known_continuation(scmx, kind, dtype):
+    """A text that has the continuation in it: LookupDraft proposes it, and tokens of it are accepted: a pass adds one token and the accepted ones, so as many passes as
+    tokens would mean that none was.  (How many are depends on choices that roundings turn: the prompt repeats a token, and a random model has near ties there.)"""
+    fused, _ = build(scmx, kind)
+    DEC = mod(scmx, "decode")
+    prompt = [474] * 30
+
+    def run(propose, before):
+        cache, passes = fused.make_cache(len(prompt) + 24, dtype), []
+        first = int(fused.logits(fused.hidden(torch.tensor([prompt], device="cuda"), cache)[:, -1:]).argmax())
+        d = DEC.DecodeDraft(fused, lambda text, most: (passes.append(1), propose(text, most))[1])
+        return [first] + d.generate(torch.tensor([[first]], device="cuda"), cache, 24, before + prompt).tolist(), len(passes)
+    text, passes = run(lambda text, most: ([text[-1]], [-1]), [])
+    assert passes == 24
+    again, passes = run(DEC.LookupDraft(), prompt + text)
+    assert margins(fused, prompt, again, dtype) < MARGIN and passes < 24
+
+
+@pytest.mark.parametrize("kind", ["qwen3", "olmoe"])
+@pytest.mark.parametrize("dtype", [None, torch.int8])
 def test_replayed_passes(scmx, kind, dtype):
     """Passes of as many rows are replays from the second one on.  Trees, tokens and positions change between them: the rows that stay in the first layer's cache, which
     no attention has touched, are those of a pass launch by launch, and every token is the model's choice."""

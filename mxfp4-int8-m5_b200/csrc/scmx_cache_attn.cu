@@ -441,14 +441,27 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
     ca_output<D>(a, kvh, r, lane, v, l);
 }
 
-// A cluster's CTAs join their ranges without a second launch, but they are eight at most: up to so many positions.  Device us, cluster / two launches, 8 key/value
-// heads of 128, one token of two query heads each: 300 positions 5.4 / 6.6, 1500 6.3 / 7.8, 4000 7.6 / 8.7, 6000 8.7 / 9.6, 9000 10.1 / 9.6, 12000 12.0 / 11.7;
-// INT8 1500 6.3 / 7.8, 6000 9.4 / 9.6, 9000 11.2 / 10.4, 12000 12.8 / 11.2.  On the host it is 6 us sooner.
-// On tcgen05, 8 key/value heads of 128, cluster / two launches: 42 query rows over 1500 positions 10.4 / 10.7, 4000 12.7 / 14.0, 6000 15.0 / 15.9, INT8 4000 14.6 / 14.6,
-// 6000 17.3 / 16.6, 8000 20.5 / 17.6; 84 rows over 4000 16.3 / 15.0, 256 rows 25.3 / 19.9: for tiles that hold copies, and fewer positions.
-constexpr int64_t CA_CLUSTER_POSITIONS = 8192, CA_CLUSTER_POSITIONS_TC = 6144;
+// Whether the ranges of a head are one cluster of at most eight CTAs, which joins them without a second launch (and 6 us sooner on the host), or as many as the device
+// has room for.  Device us of a call among others, cluster / two launches, head size 128 (64 alike unless said):
+//   All clusters have to run at once: fifteen of eight did (120 CTAs), sixteen waited for one another, 32 of four did.  1000 positions, 2 query rows: 15 key/value heads 5.8 / 7.6, 16 heads
+//   9.7 / 7.7, 32 heads 14.5 / 9.0; INT8, 21 rows: 10.1 / 10.0, 18.2 / 10.6, 28.1 / 12.5.  500 positions, 21 rows in clusters of four: 32 heads 10.3 / 11.3.
+//   A single range is no cluster: 60 positions 4.5 / 3.4 (one launch), 21 rows 9.2 / 6.7.
+//   Few rows, 2 and 16 of them, bfloat16, 1 / 4 / 8 / 15 heads: 8000 positions 8.8 / 17.0, 9.2 / 11.9, 10.0 / 11.8, 13.4 / 15.1 and 12.2 / 19.3, 12.8 / 16.4, 13.8 / 15.3, 16.0 / 17.3;
+//   16000 12.9 / 20.2, 13.3 / 14.2, 14.7 / 16.1, 21.9 / 23.6 and 17.5 / 23.8, 18.0 / 18.0, 18.9 / 19.0, 24.8 / 26.4; 24000 and 4 heads 17.8 / 16.7 and 23.7 / 20.4.
+//   INT8: 8000 9.3 / 16.9, 10.0 / 11.8, 10.6 / 11.1, 11.6 / 13.4 and 13.3 / 18.9, 13.8 / 15.7, 14.4 / 14.9, 15.1 / 16.7; 12000 and 8 heads 12.9 / 12.8 and 17.3 / 16.2.
+//   On tcgen05 tiles that hold copies, 21 and 42 rows, bfloat16: 4000 10.6 / 11.6, 11.5 / 12.6, 12.3 / 13.2, 13.9 / 15.1 and 11.8 / 12.1, 12.5 / 13.6, 13.2 / 13.8, 14.9 / 16.1; 6000 12.7 / 13.6, 13.7 / 13.7,
+//   14.6 / 15.7, 16.6 / 17.7 and 14.2 / 14.6, 14.8 / 14.3, 15.6 / 16.2, 17.5 / 19.0; 10000 14.5 / 16.9, 15.0 / 13.2, 16.3 / 16.2 and 15.7 / 17.7, 16.3 / 13.9, 17.3 / 16.7.
+//   INT8, 1 / 4 / 8 / 15 heads: 2000 9.4 / 9.8, 9.6 / 9.7, 10.7 / 10.6, 11.5 / 12.2 and 10.9 / 10.6, 11.0 / 10.5, 12.2 / 12.5, 13.1 / 13.8; 4000 11.6 / 11.3, 12.5 / 12.0, 13.3 / 13.6, 14.7 / 15.3 and
+//   13.3 / 12.0, 14.2 / 13.1, 14.8 / 14.9, 16.1 / 17.2; 6000 13.9 / 12.7, 15.0 / 14.7, 16.1 / 15.2, 17.6 / 18.9 and 15.8 / 13.7, 16.8 / 16.1, 17.8 / 16.8, 19.4 / 20.6.  Here the device loses up to
+//   2 us with few heads, but calls that are not in a graph wait for the host: 42 rows over 6001 positions, 8 heads, 17.0 / 19.5 a call.
+//   Full tiles: 84 rows over 4000 positions, 8 heads, 16.3 / 15.0, 256 rows 25.3 / 19.9.
+static bool ca_joins_in_cluster(const CaPlan& p, int nsplit, int64_t positions, int hk, bool int8) {
+    if (nsplit < 2 || (p.tc && p.copies == 1)) return false;
+    if ((int64_t)hk * p.tiles * nsplit > sm_count() * (nsplit == 8 ? 13 : 14) / 16) return false;
+    return positions <= (p.tc ? 6144 : int8 ? 8192 : 16384);
+}
 
-static CaPlan ca_plan(int64_t positions, int R, int hk) {
+static CaPlan ca_plan(int64_t positions, int R, int hk, bool int8) {
     CaPlan p;
     p.cluster = 0;
     p.tc = R > 16;
@@ -467,9 +480,10 @@ static CaPlan ca_plan(int64_t positions, int R, int hk) {
     const int64_t most = (positions + p.unit - 1) / p.unit, want = sm_count() / ((int64_t)hk * p.tiles);
     const int64_t s = want < most ? want : most;
     p.nsplit = s < 1 ? 1 : (int)s;
-    if (p.tc ? p.copies > 1 && positions <= CA_CLUSTER_POSITIONS_TC : positions <= CA_CLUSTER_POSITIONS) {
+    const int ctas = most >= 8 ? 8 : most >= 3 ? 4 : most == 2 ? 2 : 1;
+    if (ca_joins_in_cluster(p, ctas, positions, hk, int8)) {
         p.cluster = 1;
-        p.nsplit = most >= 8 ? 8 : most >= 3 ? 4 : most == 2 ? 2 : 1;
+        p.nsplit = ctas;
     }
     if (!p.tc && positions > (int64_t)p.nsplit * p.unit) p.unit = CA_KEYS;      // long enough: ranges end at any block
     return p;
@@ -498,7 +512,8 @@ using namespace scmx;
 
 extern "C" int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int hk, int d) {
     if (positions < 1 || n < 1 || n > CA_MAX_ROWS || hk < 1 || hq < hk || hq % hk || (d != 64 && d != 128)) return 0;
-    return ca_states(ca_plan(positions, hq / hk * n, hk), hk) * (d + 2) * 4;
+    const int64_t bf16 = ca_states(ca_plan(positions, hq / hk * n, hk, false), hk), int8 = ca_states(ca_plan(positions, hq / hk * n, hk, true), hk);      // either type's
+    return (bf16 > int8 ? bf16 : int8) * (d + 2) * 4;
 }
 
 extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,
@@ -513,7 +528,7 @@ extern "C" int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t
     SCMX_REQUIRE(q_head_stride % 4 == 0 && q_row_stride % 4 == 0 && ((uintptr_t)q & 7) == 0 && ((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 &&
                      ((uintptr_t)out & 15) == 0, SCMX_EINVAL, "cache_attn: query rows must be 8-byte, caches and the output 16-byte aligned");
     CaArgs a;
-    const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk);
+    const CaPlan p = ca_plan(pos_dev ? capacity : pos + n, hq / hk * n, hk, int8 != 0);
     a.nsplit = p.nsplit; a.unit = p.unit; a.cluster = p.cluster;
     const int64_t states = ca_states(p, hk), need = states * (d + 2) * 4;
     SCMX_REQUIRE(scratch_bytes >= need && (need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0)), SCMX_EINVAL, "cache_attn: %lld bytes of scratch, %lld needed",

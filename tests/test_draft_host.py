@@ -79,6 +79,21 @@ def test_no_tokens_are_appended(scmx):
     _refused(scmx, "scmx_kv_append", append(0, d=24), "head size")
 
 
+def test_scratch_of_the_attention(scmx):
+    """Ranges whose CTAs are a cluster need none, nor does a single range; a second launch needs a state of every query row and range.  Heads and positions on both sides of the
+    borders, for a device of 148 multiprocessors."""
+    size = scmx._lib.lib().scmx_cache_attn_scratch
+    if torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        return
+    state = (128 + 2) * 4
+    assert size(60, 1, 16, 8, 128) == 0 and size(60, 1, 400, 400, 128) == 0                      # one range
+    assert size(1000, 1, 15, 15, 128) == 0 and size(1000, 1, 16, 16, 128) == 16 * 9 * 8 * state   # clusters of eight that run at once, or 148 / 16 ranges
+    assert size(500, 21, 32, 32, 128) == 0 and size(500, 21, 33, 33, 128) == 33 * 4 * 32 * state   # clusters of four
+    assert size(8192, 1, 16, 8, 128) == 0 and size(8193, 1, 16, 8, 128) == 8 * 18 * 8 * state      # INT8, few rows
+    assert size(6144, 21, 8, 8, 128) == 0 and size(6145, 21, 8, 8, 128) == 8 * 18 * 32 * state     # tcgen05
+    assert size(2000, 64, 16, 8, 128) == 8 * 16 * 128 * state                                      # 128 rows: a tile without copies
+
+
 def test_lookup_draft(scmx):
     import importlib
     L = importlib.import_module(scmx.__name__ + ".decode").LookupDraft

@@ -218,6 +218,21 @@ def test_attention_of_a_tree(scmx, int8, d, hq, hk, n, T):
     check_attention(scmx.sc_cache.cache_attention(q, c, scale), q, c, scale, None)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("hq,hk,n", [(15, 15, 1), (16, 16, 1), (20, 20, 7), (16, 16, 21), (33, 33, 21), (4, 4, 21), (8, 8, 33), (2, 1, 12)])
+@pytest.mark.parametrize("T", [20, 250, 500, 1100, 2047, 4100, 6150, 8200])
+def test_attention_on_both_sides_of_the_clusters_borders(scmx, int8, hq, hk, n, T):
+    """One range, clusters of two, four and eight, clusters that would not run at once, and two launches; the position on the host, and on the device in a larger cache,
+    which cuts it by its capacity."""
+    d, at = 64 if T == 500 else 128, max(T - n, 0)                       # T positions with the new rows
+    q, c = attention_case(scmx, hq, hk, n, at, d, int8, seed=T + hk)
+    mask = scmx.sc_draft.draft_mask(random_parents(random.Random(n), n))
+    check_attention(scmx.sc_cache.cache_attention(q, c, 0.09, mask), q, c, 0.09, mask)
+    if T >= 4100:
+        for pos in (at, T // 3, 3, 0):
+            check_attention(scmx.sc_cache.cache_attention(q, c, 0.09, mask, torch.tensor([pos], dtype=torch.int32, device="cuda")), q, c, 0.09, mask, T=pos)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("int8,hq,hk,n,T", [(False, 8, 4, 1, 900), (False, 4, 4, 11, 10000), (False, 2, 1, 8, 40), (True, 8, 4, 1, 900), (True, 2, 2, 16, 10000), (True, 16, 2, 3, 2500),
                                             (True, 16, 2, 7, 400), (True, 8, 2, 30, 7000), (True, 8, 1, 20, 9000), (True, 4, 1, 64, 5000)])

@@ -12,8 +12,8 @@
 // INT8 codes become operands exactly, keys bfloat16 like the queries, values float16; a position's key scale multiplies its scores, the log2 of its value
 // scale is added to them (CA_SHIFT), so that weights are float16.  Over bfloat16 a weight is two operands, what it rounds to and the rest (2^-16 of it):
 // the second product costs 1 to 5 %, a single one made the output's error 0.0023 where rounding it costs 0.0016.
-// Measured on a B200, one token, 8 key/value heads of 128: 1500 bfloat16 positions 5.6 us, launch latency and one round of loads; 65537 INT8
-// positions 28.8 us, 4.8 TB/s, of which 5 us start, drain and join; within the ranges the conversions' integer operations keep the warps as busy as
+// Measured on a B200, one token, 8 key/value heads of 128: 1500 bfloat16 positions 5.4 us, launch latency and one round of loads; 65537 INT8
+// positions 28.6 us, 4.8 TB/s, of which 5 us start, drain and join; within the ranges the conversions' integer operations keep the warps as busy as
 // the loads.
 #include <cooperative_groups.h>
 #include "scmx_cache_attn.cuh"
@@ -464,6 +464,10 @@ static bool ca_joins_in_cluster(const CaPlan& p, int nsplit, int64_t positions, 
 static CaPlan ca_plan(int64_t positions, int R, int hk, bool int8) {
     CaPlan p;
     p.cluster = 0;
+    // Up to 16 query rows two groups of eight read the cache once; more would read it again, and tcgen05's tile has 128 rows.  Device us, mma.sync / tcgen05, head size 128, over 1500, 6000,
+    // 20000 and 60000 positions of 8 key/value heads: bfloat16, 16 rows 8.9 / 9.8, 12.2 / 12.2, 21.7 / 21.0, 45.2 / 44.3, 20 rows 12.5 / 10.0, 18.8 / 12.4, 23.0 / 21.1, 48.9 / 44.4; INT8 8.4 / 10.2,
+    // 12.6 / 15.8, 18.9 / 25.2, 32.8 / 47.2 and 13.0 / 10.4, 20.6 / 16.0, 23.9 / 25.4, 51.1 / 47.5.  Of 2 heads: bfloat16, 16 rows 7.8 / 8.7, 11.3 / 11.1, 22.3 / 16.2, 27.2 / 23.7, 20 rows 8.0 / 8.8,
+    // 11.4 / 11.2, 17.7 / 16.3, 23.9 / 23.7; INT8 8.1 / 9.4, 11.9 / 14.2, 20.1 / 19.5, 23.4 / 30.0 and 8.4 / 9.6, 11.8 / 14.4, 17.2 / 20.3, 24.5 / 30.9.
     p.tc = R > 16;
     if (p.tc) {
         p.nt = R > 128 ? 2 : 1;

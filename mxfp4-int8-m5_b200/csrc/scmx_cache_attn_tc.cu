@@ -22,8 +22,8 @@
 // Measured on a B200 (8 key/value heads of 128): 60000 bfloat16 positions 45.2 us with 18 query rows (5.4 TB/s), 51.5 with 128, 68 with 256; INT8 49,
 // 63 and 107 us.  bfloat16 up to 128 rows waits for memory.  A pair of units of 256 rows takes 3400 cycles, and its bytes arrive in 2800: a stream's
 // scores, softmax (2050 cycles, half of them the exponentials' rate) and product follow on one another, and two streams are what tensor memory
-// holds.  A second softmax thread per row, or a third of the exponentials from a cubic, changed less than 2 %.  INT8 adds the scales and the conversions,
-// which share the issue slots: 6000 cycles for a pair; half of its exponents wait in tensor memory (all loaded and scaled twice: 67 us, not 63).  Weights in halves against whole tiles: 256 rows 72 -> 70 us, INT8 65 -> 62 us at
+// holds, although half of a stream's columns of scores are free while its softmax runs.  A second softmax thread per row, or a third of the exponentials from a cubic, changed less than 2 %.  INT8 adds
+// the scales and the conversions: 6000 cycles for a pair, with 48 % of the issue slots used and loads' latency the most frequent stall; half of its exponents wait in tensor memory (all loaded and scaled twice: 67 us, not 63).  Weights in halves against whole tiles: 256 rows 72 -> 70 us, INT8 65 -> 62 us at
 // 128 rows; for bfloat16 at 128 rows, which has its two streams on different tiles, 16.9 -> 17.6 us at 8000 positions, so there they stay whole.
 #include <cooperative_groups.h>
 #include "mixers/mix_tc.cuh"

@@ -11,9 +11,10 @@
 // to a node, took 19 us of the whole device where a pass of the walk takes 3).  The last token's weights, sums and cumulative
 // probabilities are float64: between 100000 neighbours float32 sums would pick another token once in a hundred draws.
 //
-// Measured on a B200: greedy, 5 rows of 32000 bfloat16 logits, 4.9 us (two launches); 21 rows of 50304 float32 logits by temperature 11.4 us; 64 rows of
-// 151936 with the draft's probabilities 23.8 us, against 9 us for all bytes once: the walk is a chain of dependent passes over single
-// rows, 3 us each, and all of the tree's rows are not its path's.
+// Measured on a B200: greedy, 5 rows of 32000 bfloat16 logits, 4.9 us (two launches); 21 rows of 50304 float32 logits by temperature 11.5 us, of which the two launches and the cluster's start and
+// barriers are 8.6 (one row of 8 logits), the last node's pass 1; 64 rows of 151936 with the draft's probabilities 23.8 us from memory, 17.1 from L2, against 9 us for all bytes once: the
+// walk is a chain of dependent passes over single rows, 3 us each, 8 us in a row of 151936, and all of the tree's rows are not its path's.  63 children of one node, all rejected: 30 us without
+// probabilities, 450 with them at 50304.
 #include <cooperative_groups.h>
 #include "scmx_common.cuh"
 

@@ -92,7 +92,7 @@ def kv_read(cache, start=0, end=None):
 
 def kv_keep(caches, rows, pos=None, pos_dev=None):
     """In every cache (of equal shape and type) row pos + rows[j] becomes row pos + j; pos defaults to the first cache's offset.  rows: int32 [n <= 64] on
-    the device, n the rows that were written from pos on; negative entries leave their row, as verify_draft pads its list."""
+    the device, n the rows that were written from pos on; negative entries leave their row, as verify_draft pads its list.  A cache is listed once."""
     _lib.require_here(rows)
     n = rows.numel()
     if rows.dtype != _I32 or not 1 <= n <= MAX_ROWS:
@@ -131,7 +131,7 @@ def attention_supported(hq, hk, d):
 
 def cache_attention(q, cache, scale, mask=None, pos_dev=None):
     """Attention of n <= 64 new rows, q bfloat16 [hq, n, d], to a cache that already holds their keys and values at rows offset .. offset + n - 1 (pos_dev[0] ..
-    if given, so that a captured call can be replayed while the sequence grows) -> bfloat16 [n, hq d].  Row i sees every position before
+    if given, so that a captured call can be replayed while the sequence grows; one outside the cache is taken as the nearest inside) -> bfloat16 [n, hq d].  Row i sees every position before
     them, and new row j if bit j of mask[i] is set (int64 [n], sc_draft.draft_mask; None: j <= i).  A row that sees nothing gives zeros."""
     int8, kc, vc, ks, vs, (hk, cap, d) = _tensors(cache)
     shape = q.shape

@@ -210,7 +210,16 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
         float kf[2] = {a.scale, a.scale}, lg[2] = {0.0f, 0.0f}, inv[2] = {1.0f, 1.0f};
         if constexpr (I8) {
             const float* scales = reinterpret_cast<const float*>(blk + 2 * L::BLOCK);
-            if (b == warp) ref = ca_reference(scales[16 + (lane & 15)]);
+            if (b == warp) {
+                const int key = b * CA_KEYS + (lane & 15);
+                const float first[1] = {scales[16 + (lane & 15)]};
+                bool from[1] = {key < ntail};
+                if (b * CA_KEYS >= ntail) {
+                    const uint64_t any = ca_seen_by_any(a, lane);
+                    from[0] = key - ntail < a.n && (any >> ((key - ntail) & 63) & 1);
+                }
+                ref = ca_reference(first, from);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 kf[h] *= scales[g + 8 * h];

@@ -10,8 +10,8 @@ constexpr int CA_KEYS = 16;             // positions of a block
 constexpr int CA_MAX_ROWS = 64;
 constexpr float CA_LOG2E = 1.4426950408889634f;
 constexpr float CA_GROWTH = 8.0f;      // log2 of how far a weight may exceed one before the maximum is raised
-// INT8: a weight and its value's scale s are one power of 2, w = 2^(score + log2(s / r) - max), whose maximum the rows keep, r the largest scale of the first
-// positions; what is summed is w / (s / r), and outputs are multiplied by r at the end.  So w never exceeds 2^8 whatever the scales, and it goes to
+// INT8: a weight and its value's scale s are one power of 2, w = 2^(score + log2(s / r) - max), whose maximum the rows keep, r the geometric mean of the scales of the
+// first positions; what is summed is w / (s / r), and outputs are multiplied by r at the end.  So w never exceeds 2^8 whatever the scales, and it goes to
 // the product as float16 (the codes are exact in it), 2^6 larger: from 2^14 down to 2^-24, 2^-12 of a weight off where bfloat16 is 2^-8.  Sums and outputs leave
 // 2^20 smaller, so that large values times r stay finite.
 constexpr float CA_SHIFT = 6.0f, CA_LEAST = -90.0f, CA_DOWN = 9.5367431640625e-07f;
@@ -53,14 +53,34 @@ __device__ __forceinline__ float ca_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// log2 r of the largest of a warp's scales.
-__device__ __forceinline__ float ca_reference(float s) {
-    const float r = warp_max(s != s ? 0.0f : s);
-    float lg;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(r));
-    return r > 0.0f && r < INFINITY ? lg : 0.0f;
+// New rows that some query row sees.
+__device__ __forceinline__ uint64_t ca_seen_by_any(const CaArgs& a, int lane) {
+    uint64_t bits = a.mask == nullptr ? ~0ull : (lane < a.n ? (uint64_t)a.mask[lane] : 0ull) | (lane + 32 < a.n ? (uint64_t)a.mask[lane + 32] : 0ull);
+    bits = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(bits >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)bits);
+    return a.n < 64 ? bits & ((1ull << a.n) - 1ull) : bits;
 }
-// log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends.  A vector of zeros has scale 0: any other is right for it, and the least
+// log2 r from PER scales of every lane, those `from` counts of: of positions before the new rows, which every row sees, or, where a range begins behind those, of the new rows
+// that some row sees.  What nobody sees may hold any scale, and must not set the range that the others have.  The mean of the logarithms: one scale far from all others
+// moves it least (a vector that is not finite, or of zeros, does not count).
+template <int PER>
+__device__ __forceinline__ float ca_reference(const float (&s)[PER], const bool (&from)[PER]) {
+    float sum = 0.0f;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        float lg;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s[i]));
+        if (from[i] && lg > -INFINITY && lg < INFINITY) {
+            sum += lg;
+            ++count;
+        }
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return count ? sum / (float)count : 0.0f;
+}
+// log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends (above, at 2^106 r).  A vector of zeros has scale 0: any other is right for it, and the least
 // keeps its weight out of the maximum (with r, a score 28 powers of two above all others left these so few bits that the output was half wrong).
 __device__ __forceinline__ void ca_scale(float s, float ref, float& lg, float& inv) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s));

@@ -558,14 +558,16 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         const float factor = fabsf(a.scale);
         float ref = 0.0f;                         // log2 of the scale that values are relative to
         if (t >= 128) {
-            float top = 0.0f;
+            float first[4];
+            bool from[4];
+            const uint64_t any = dnew >= 0 ? ca_seen_by_any(a, lane) : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = 32 * i + lane < nkeys ? 32 * i + lane : 0;
-                const float s = nkeys > 0 ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + r) : 0.0f;
-                top = fmaxf(top, s);
+                const int r = 32 * i + lane, d = dnew + r;         // d: counted from the first new row
+                first[i] = r < nkeys ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + r) : 0.0f;
+                from[i] = dnew < 0 ? d < 0 : d < a.n && (any >> (d & 63) & 1);
             }
-            ref = ca_reference(top);
+            ref = ca_reference(first, from);
             if (t == 128) *reinterpret_cast<float*>(smem + L::MISC_OFF + 16) = ref;
         }
         auto scale = [&](int j) { return 128 * j + (t & 127) < nkeys ? __ldg(scales + 128 * j) : 0.0f; };

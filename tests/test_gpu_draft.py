@@ -298,6 +298,37 @@ def test_values_of_zeros_with_the_largest_score(scmx, hq, hk, n, T, at):
         assert (off <= tol).all(), f"{powers}: off by {(off / tol).max().item():.3g} of the tolerance"
 
 
+@pytest.mark.parametrize("hq,hk,n,T", [(2, 2, 3, 0), (8, 2, 4, 0), (4, 4, 9, 7), (4, 2, 2, 16), (2, 1, 6, 300), (8, 2, 30, 0), (8, 2, 30, 100), (4, 1, 64, 700), (4, 4, 20, 3)])
+def test_scales_in_masked_places(scmx, hq, hk, n, T):
+    """Over INT8, new rows that no row sees hold any scale, and one that only its own row sees is 2^93 above or below all others: every other row is as without them.  Its own row is
+    what its scale makes it.  (A float16 weight: as in test_scales_of_all_sizes, with the largest scale that a row sees.)"""
+    rng = random.Random(n + T)
+    odd = n // 2
+    for value, alone in ((1e30, False), (1e-30, False), (2.0 ** -126, False), (float("nan"), False), (float("inf"), False), (1e28, True), (1e-28, True)):
+        q, c = attention_case(scmx, hq, hk, n, T, 128, True, seed=n)
+        bits = [(rng.getrandbits(n) | 1 << i) & ~(1 << odd) for i in range(n)]
+        bits[odd] = 1 << odd if alone else bits[odd] | (1 << (odd + 1) % n)
+        mask = torch.tensor([b - (1 << 64) if b >> 63 else b for b in bits], device="cuda")
+        others = [i for i in range(n) if not (alone and i == odd)]
+        amax = torch.cat((c.vs[:, :T + odd], c.vs[:, T + odd + 1:T + n]), 1).amax().double()
+        for rows in ([odd], [odd] + [j for j in range(n) if not any(b >> j & 1 for b in bits)]):
+            if alone:
+                c.vs[:, T + odd] = value
+                want, tol = attention_oracle(q, c, 0.09, mask, weight=2.0 ** -11)
+            else:
+                want, tol = attention_oracle(q, c, 0.09, mask, weight=2.0 ** -11)
+                c.vs[:, [T + j for j in rows]] = value
+                c.ks[:, [T + j for j in rows]] = float("nan")
+            got = scmx.sc_cache.cache_attention(q, c, 0.09, mask)
+            off = (got.double() - want).abs()
+            assert torch.isfinite(got).all()
+            assert (off[others] <= tol[others] + (T + n) * 2.0 ** -31 * 127 * amax).all(), f"{value}: off by {(off / tol)[others].max().item():.3g} of the tolerance"
+            if alone:
+                assert (off[odd] <= tol[odd] + (T + n) * 2.0 ** -31 * 127 * max(amax, value)).all(), f"{value}: its own row"
+            else:
+                c.vs[:, [T + j for j in rows]], c.ks[:, [T + j for j in rows]] = 0.01, 0.01
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hq,hk,n,T", [(8, 8, 4, 0), (8, 2, 40, 0), (4, 1, 64, 0), (4, 1, 3, 200), (8, 2, 64, 1)])
 def test_rows_that_see_nothing(scmx, int8, hq, hk, n, T):

@@ -483,7 +483,8 @@ int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stri
  * order: c is accepted if u[c] q(tokens[c]) < p(tokens[c]), q = probs[node] (float32 [n, V], children drawn from it independently) or 1
  * (probs null: a draft without chance); a rejected one leaves p <- max(p - q, 0) / Z, or p without its token (unchanged where Z = 0).  The path goes
  * on from an accepted row; at its end *token is the first index whose cumulative p exceeds u[0].  temperature 0: a child is
- * accepted if it is the largest logit of its parent (lowest index of equal ones), u unused.  rows int32 [n]: the accepted rows, first 0, then
+ * accepted if it is the largest logit of its parent (lowest index of equal ones), u unused.  By temperature a drafted token's weight below 2^-126 of its
+ * row's largest counts as none.  rows int32 [n]: the accepted rows, first 0, then
  * -1; count int32 [1].  Tokens outside 0 .. V - 1 are rejected; where the last row has no probabilities (all logits -inf, a
  * NaN or +inf among them) its children are rejected and, by temperature, *token = 0.
  * n <= 64; scratch: scmx_verify_scratch bytes, 16-byte aligned, used by this call alone. */

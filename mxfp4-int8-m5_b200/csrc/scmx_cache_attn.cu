@@ -213,11 +213,8 @@ __global__ void __launch_bounds__(CaShape<D, I8, NT>::THREADS, 1) cache_attn_ker
             if (b == warp) {
                 const int key = b * CA_KEYS + (lane & 15);
                 const float first[1] = {scales[16 + (lane & 15)]};
-                bool from[1] = {key < ntail};
-                if (b * CA_KEYS >= ntail) {
-                    const uint64_t any = ca_seen_by_any(a, lane);
-                    from[0] = key - ntail < a.n && (any >> ((key - ntail) & 63) & 1);
-                }
+                const uint64_t any = (b + 1) * CA_KEYS > ntail ? ca_seen_by_any(a, lane) : 0;
+                const bool from[1] = {key < ntail || (key - ntail < a.n && (any >> ((key - ntail) & 63) & 1))};
                 ref = ca_reference(first, from);
             }
 #pragma unroll

@@ -14,7 +14,7 @@ constexpr float CA_GROWTH = 8.0f;      // log2 of how far a weight may exceed on
 // first positions; what is summed is w / (s / r), and outputs are multiplied by r at the end.  So w never exceeds 2^8 whatever the scales, and it goes to
 // the product as float16 (the codes are exact in it), 2^6 larger: from 2^14 down to 2^-24, 2^-12 of a weight off where bfloat16 is 2^-8.  Sums and outputs leave
 // 2^20 smaller, so that large values times r stay finite.
-constexpr float CA_SHIFT = 6.0f, CA_LEAST = -90.0f, CA_DOWN = 9.5367431640625e-07f;
+constexpr float CA_SHIFT = 6.0f, CA_LEAST = -90.0f, CA_ZERO = -64.0f, CA_DOWN = 9.5367431640625e-07f;
 
 struct CaArgs {
     const uint16_t* q;               // bf16, heads q_hs and rows q_rs elements apart
@@ -59,9 +59,9 @@ __device__ __forceinline__ uint64_t ca_seen_by_any(const CaArgs& a, int lane) {
     bits = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(bits >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)bits);
     return a.n < 64 ? bits & ((1ull << a.n) - 1ull) : bits;
 }
-// log2 r from PER scales of every lane, those `from` counts of: of positions before the new rows, which every row sees, or, where a range begins behind those, of the new rows
-// that some row sees.  What nobody sees may hold any scale, and must not set the range that the others have.  The mean of the logarithms: one scale far from all others
-// moves it least (a vector that is not finite, or of zeros, does not count).
+// log2 r from PER scales of every lane, those that `from` names: positions before the new rows, which every row sees, and the new rows that some row sees.  What nobody sees may
+// hold any scale, and must not set the range that the others have.  The mean of the logarithms: one scale far from all others moves it least (a vector that is not finite, or of
+// zeros, does not count).
 template <int PER>
 __device__ __forceinline__ float ca_reference(const float (&s)[PER], const bool (&from)[PER]) {
     float sum = 0.0f;
@@ -80,11 +80,12 @@ __device__ __forceinline__ float ca_reference(const float (&s)[PER], const bool 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return count ? sum / (float)count : 0.0f;
 }
-// log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends (above, at 2^106 r).  A vector of zeros has scale 0: any other is right for it, and the least
-// keeps its weight out of the maximum (with r, a score 28 powers of two above all others left these so few bits that the output was half wrong).
+// log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends (above, at 2^106 r), and a weight counts in its row's sum down to 2^-132 of the largest
+// weight times the two scales' ratio.  A vector of zeros has scale 0: any other is right for it, and a small one keeps its weight out of the maximum (with r, a score 28 powers of two above
+// all others left these so few bits that the output was half wrong), one not too small keeps it in the sum.
 __device__ __forceinline__ void ca_scale(float s, float ref, float& lg, float& inv) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s));
-    lg = s != s ? s : fmaxf(lg - ref, CA_LEAST);      // (log2 of 0 is -inf)
+    lg = s == 0.0f ? CA_ZERO : s != s ? s : fmaxf(lg - ref, CA_LEAST);
     inv = ca_ex2(-lg);
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {

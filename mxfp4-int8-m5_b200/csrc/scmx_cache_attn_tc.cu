@@ -560,12 +560,12 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         if (t >= 128) {
             float first[4];
             bool from[4];
-            const uint64_t any = dnew >= 0 ? ca_seen_by_any(a, lane) : 0;
+            const uint64_t any = dnew + 128 > 0 ? ca_seen_by_any(a, lane) : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 32 * i + lane, d = dnew + r;         // d: counted from the first new row
                 first[i] = r < nkeys ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + r) : 0.0f;
-                from[i] = dnew < 0 ? d < 0 : d < a.n && (any >> (d & 63) & 1);
+                from[i] = d < 0 || (d < a.n && (any >> (d & 63) & 1));
             }
             ref = ca_reference(first, from);
             if (t == 128) *reinterpret_cast<float*>(smem + L::MISC_OFF + 16) = ref;

@@ -329,6 +329,23 @@ def test_scales_in_masked_places(scmx, hq, hk, n, T):
                 c.vs[:, [T + j for j in rows]], c.ks[:, [T + j for j in rows]] = 0.01, 0.01
 
 
+@pytest.mark.parametrize("hq,hk,n,T,first", [(2, 2, 4, 1, 1e-7), (2, 2, 4, 1, 1e5), (8, 2, 22, 1, 1e-7), (4, 4, 64, 1, 1e-7), (4, 4, 64, 2, 1e6), (1, 1, 12, 300, 1e-7), (4, 1, 20, 300, 1e-7)])
+def test_zeros_count_beside_values_of_all_sizes(scmx, hq, hk, n, T, first):
+    """The first position's scale is far from the others', which are 2^40 apart among themselves, and a third of the vectors are zeros: those have no value but their weight, and it
+    stays in the sum.  (The tolerance of test_scales_of_all_sizes.)"""
+    q, c = attention_case(scmx, hq, hk, n, T, 128, True, seed=n)
+    g = gen(4)
+    c.vs.mul_(2.0 ** torch.randint(-20, 21, c.vs.shape, generator=g, device="cuda").float())
+    gone = torch.rand(c.vs.shape, generator=g, device="cuda") < 0.33
+    c.vs[gone] = 0.0
+    c.v[gone] = 0
+    c.vs[:, 0], c.v[:, 0] = first, 1
+    for scale in (0.09, 1e-3, 0.0):
+        want, tol = attention_oracle(q, c, scale, None, weight=2.0 ** -11)
+        off = (scmx.sc_cache.cache_attention(q, c, scale).double() - want).abs()
+        assert (off <= tol + (T + n) * 2.0 ** -31 * 127 * c.vs.double().amax()).all(), f"off by {(off / tol).max().item():.3g} of the tolerance"
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hq,hk,n,T", [(8, 8, 4, 0), (8, 2, 40, 0), (4, 1, 64, 0), (4, 1, 3, 200), (8, 2, 64, 1)])
 def test_rows_that_see_nothing(scmx, int8, hq, hk, n, T):

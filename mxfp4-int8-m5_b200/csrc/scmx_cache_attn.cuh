@@ -64,21 +64,19 @@ __device__ __forceinline__ uint64_t ca_seen_by_any(const CaArgs& a, int lane) {
 // zeros, does not count).
 template <int PER>
 __device__ __forceinline__ float ca_reference(const float (&s)[PER], const bool (&from)[PER]) {
-    float sum = 0.0f;
-    int count = 0;
+    int sum = 0, count = 0;      // of sixteenths: r need not be the mean exactly, and whole numbers are added over a warp in one instruction
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         float lg;
         asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(s[i]));
         if (from[i] && lg > -INFINITY && lg < INFINITY) {
-            sum += lg;
+            sum += __float2int_rn(lg * 16.0f);
             ++count;
         }
     }
-    count = __reduce_add_sync(0xffffffffu, count);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return count ? sum / (float)count : 0.0f;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    count = PER == 1 ? __popc(__ballot_sync(0xffffffffu, count)) : __reduce_add_sync(0xffffffffu, count);
+    return count ? rintf(__fdividef((float)sum, 16.0f * (float)count)) : 0.0f;
 }
 // log2(s / r) and r / s of a value's scale, 2^-20 off at most; below 2^-90 r the sums' range ends (above, at 2^106 r), and a weight counts in its row's sum down to 2^-132 of the largest
 // weight times the two scales' ratio.  A vector of zeros has scale 0: any other is right for it, and a small one keeps its weight out of the maximum (with r, a score 28 powers of two above

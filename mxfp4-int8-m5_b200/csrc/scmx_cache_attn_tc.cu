@@ -560,11 +560,12 @@ __global__ void __launch_bounds__(CtSmem<D, I8, MQ>::THREADS, 1)
         if (t >= 128) {
             float first[4];
             bool from[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) first[i] = 32 * i + lane < nkeys ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + 32 * i + lane) : 0.0f;
             const uint64_t any = dnew + 128 > 0 ? ca_seen_by_any(a, lane) : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = 32 * i + lane, d = dnew + r;         // d: counted from the first new row
-                first[i] = r < nkeys ? __ldg(a.vs + (int64_t)kvh * a.cap + t0 + r) : 0.0f;
+                const int d = dnew + 32 * i + lane;         // counted from the first new row
                 from[i] = d < 0 || (d < a.n && (any >> (d & 63) & 1));
             }
             ref = ca_reference(first, from);

@@ -471,7 +471,7 @@ int scmx_kv_keep(const scmx_kv_layer* layers, int n_layers, const int32_t* rows,
  * if bit j of mask[i] is set (mask null: j <= i); a row that sees nothing gives zeros.  k, v [hk, capacity, d]: bf16, or int8 with scales.
  * pos_dev non-null: one device int32 instead of pos.  scratch: scmx_cache_attn_scratch(pos + n, or capacity with pos_dev; ..) bytes, 16-byte
  * aligned, used by this call alone.  float32 softmax and sums; weights enter the product as float16 over int8 (value scales are not negative, as
- * scmx_kv_append writes them), as two bf16 over bf16 (one beyond 16 query rows of a key/value head).  d 64 or 128.  status int32[4]: as in
+ * scmx_kv_append writes them, and 2^90 below to 2^106 above their usual size are told apart; those of rows that nobody sees may be anything), as two bf16 over bf16 (one beyond 16 query rows of a key/value head).  d 64 or 128.  status int32[4]: as in
  * scmx_mm_i8. */
 int64_t scmx_cache_attn_scratch(int64_t positions, int n, int hq, int hk, int d);
 int scmx_cache_attn(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* k, const void* v, const float* k_scales,

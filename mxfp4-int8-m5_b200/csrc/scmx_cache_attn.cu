@@ -13,7 +13,7 @@
 // scale is added to them (CA_SHIFT), so that weights are float16.  Over bfloat16 a weight is two operands, what it rounds to and the rest (2^-16 of it):
 // the second product costs 1 to 5 %, a single one made the output's error 0.0023 where rounding it costs 0.0016.
 // Measured on a B200, one token, 8 key/value heads of 128: 1500 bfloat16 positions 5.4 us, launch latency and one round of loads; 65537 INT8
-// positions 28.6 us, 4.8 TB/s, of which 5 us start, drain and join; within the ranges the conversions' integer operations keep the warps as busy as
+// positions 28.8 us, 4.8 TB/s, of which 5 us start, drain and join; within the ranges the conversions' integer operations keep the warps as busy as
 // the loads.
 #include <cooperative_groups.h>
 #include "scmx_cache_attn.cuh"
